@@ -132,9 +132,10 @@ def _rope(dim: int) -> tuple:
 
 
 class _Memory:
-    """Device memory of a pool, for torch to look at."""
+    """Device memory of a pool, for torch to look at; what looks at it keeps the pool."""
 
-    def __init__(self, ptr, shape, typestr):
+    def __init__(self, pool, ptr, shape, typestr):
+        self.pool = pool
         self.__cuda_array_interface__ = dict(data=(ptr, False), shape=shape, typestr=typestr, version=3)
 
 
@@ -149,7 +150,7 @@ def _handles(case: dict, s: dict) -> None:
     for name, ptr in (("k", pool.k_ptr), ("v", pool.v_ptr), ("mass", pool.mass_ptr)):
         if name in s:
             x = s[name]
-            there = torch.as_tensor(_Memory(ptr, tuple(x.shape), "<i2" if x.dtype == torch.bfloat16 else "<f4"), device=DEV).view(x.dtype)
+            there = torch.as_tensor(_Memory(pool, ptr, tuple(x.shape), "<i2" if x.dtype == torch.bfloat16 else "<f4"), device=DEV).view(x.dtype)
             there.copy_(x)
             s[name] = there
     q, kv = s["q_lens"], s["kv_lens"]
