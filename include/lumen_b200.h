@@ -52,6 +52,8 @@ typedef struct lumen_llama_kv_cache lumen_llama_kv_cache; /* LlamaKVCache */
 typedef struct lumen_self_attention lumen_self_attention;
 typedef struct lumen_llama lumen_llama;
 typedef struct lumen_model lumen_model; /* any language model */
+typedef struct lumen_page_pool lumen_page_pool;   /* pages of one layer's keys and values */
+typedef struct lumen_page_batch lumen_page_batch; /* sequences of one step: lengths, page tables, plan of the work */
 
 /* ---- context ------------------------------------------------------------------------------
  * No counterpart in the reference (it has no device or process boundary).  tp_size > 1 makes
@@ -133,8 +135,11 @@ int lumen_gemv_kn_static(lumen_ctx *ctx, const float *x_dev, const void *w_dev, 
 /* ---- RotaryEmbedding — src/layers/attention/encoding.rs ------------------------------------
  * new      <- RotaryEmbedding::new + precompute_freqs_cis (:17-54); tables are built on the host
  *             with the f32 recipe of :38-51 and uploaded.
+ * from_tables: the caller's own tables [max_seq_len, dim/2] (host), for scaled frequencies or angles computed
+ *             in more than 32 bits; no counterpart in the reference.
  * forward  <- RotaryEmbedding::forward(x[B,H,S,D], offset)   (:56-123) */
 int lumen_rope_new(lumen_ctx *ctx, size_t dim, size_t max_seq_len, float theta, lumen_rope **out);
+int lumen_rope_from_tables(lumen_ctx *ctx, size_t dim, size_t max_seq_len, const float *cos_host, const float *sin_host, lumen_rope **out);
 int lumen_rope_forward(lumen_rope *rope, const lumen_tensor *x_bhsd, size_t offset, lumen_tensor **out);
 int lumen_rope_free(lumen_rope *rope);
 
@@ -354,6 +359,64 @@ int lumen_model_forward_sample(lumen_model *m, const float *ids_host, size_t s, 
                                const lumen_sample_params *params, int32_t *token_out);
 size_t lumen_model_weight_bytes(const lumen_model *m);
 int lumen_model_free(lumen_model *m);
+
+/* ---- paged key/value cache ---------------------------------------------------------------------
+ * A cache for sequences of different lengths (no counterpart in the reference, whose caches advance in lock-step,
+ * self_attention.rs:24-44).  All pointers to queries, keys, values and outputs are device pointers.
+ *
+ * lumen_page_pool: the pages of ONE layer: keys and values [pages, h_kv, page_size, d] of type dtype and, per slot,
+ * the attention weight its position has received, f32 [pages, h_kv, page_size]; all zero at first.  page_size: a
+ * power of two from 8 to 256; d: 64 or 128.  _k, _v, _mass: the device addresses, in this layout.
+ *
+ * lumen_page_batch: what one step works on, for every pool of the same geometry.  Sequence s brings q_lens[s] new
+ * tokens; with them its cache holds kv_lens[s] positions; position p is in slot p % page_size of page
+ * tables[s * table_stride + p / page_size].  New tokens take the last q_lens[s] positions, and rows of queries and
+ * outputs follow one another, sequence by sequence.  first_pos[s] is the position that the rotation gives the first
+ * new token (NULL: its place in the cache, kv_lens[s] - q_lens[s]; another number after an eviction).  causal != 0: a
+ * new token sees the cached positions up to its own; 0: all kv_lens[s].  The arrays are HOST arrays and are read
+ * during the call, which checks every page number and copies the plan to the device; it may not be made while the
+ * context's stream is being captured.  Refused: q_lens[s] > kv_lens[s] with causal (LUMEN_ERR_SHAPE), more positions
+ * than the table's pages hold (LUMEN_ERR_KV_OVERFLOW), a page outside the pool or twice in a sequence
+ * (LUMEN_ERR_INVALID).  Sequences may share pages that they only read.
+ * The calls below allocate nothing and may be captured into graphs; a batch owns the workspace of its attention, so
+ * calls with ONE batch must not overlap, as those on one context's stream do not.  A batch or pool that a graph uses
+ * must live as long as that graph. */
+int lumen_page_pool_new(lumen_ctx *ctx, size_t pages, size_t page_size, size_t h_kv, size_t d, lumen_dtype dtype, lumen_page_pool **out);
+void *lumen_page_pool_k(const lumen_page_pool *pool);
+void *lumen_page_pool_v(const lumen_page_pool *pool);
+float *lumen_page_pool_mass(const lumen_page_pool *pool);
+int lumen_page_pool_free(lumen_page_pool *pool);
+int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_seq, const int32_t *q_lens, const int32_t *kv_lens,
+                         const int32_t *first_pos, const int32_t *tables, size_t table_stride, int causal, lumen_page_batch **out);
+int lumen_page_batch_free(lumen_page_batch *batch);
+/* The new tokens' projections into the cache, in one pass: q[tokens, n_head * d], k and v [tokens, h_kv * d] are f32 rows
+ * q_stride / kv_stride floats apart (parts of one fused product, say).  Per head of q and k: RMS norm with gains
+ * q_norm / k_norm [d] (NULL: none; rms_norm.rs:49-56), then the rotation of rope (NULL: none; encoding.rs:195-203);
+ * q goes to q_out[tokens, n_head, d], k and v to their slots, all of the pool's type, each rounded once; the slots'
+ * attention weight becomes 0.  Refused: pages that receive new rows and also belong to another sequence, positions
+ * beyond the tables (LUMEN_ERR_ROPE_RANGE).  q_out: 16-byte aligned. */
+int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, const lumen_rope *rope, const float *q_dev, const float *k_dev,
+                       const float *v_dev, size_t q_stride, size_t kv_stride, const float *q_norm_dev, const float *k_norm_dev, float eps,
+                       void *q_out_dev);
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the positions that token t sees, query head h reading key head
+ * h / (n_head / h_kv).  q: the pool's type; out: f32, or bf16 from a bf16 pool; [tokens, n_head, d], 16-byte aligned, not
+ * overlapping.  lse (NULL: not wanted): f32 [tokens, n_head], log of the sum of exp(scale * q . k).  A token that sees nothing
+ * gives zeros and -infinity.  Sums and softmax in f32; from a bf16 pool the weights are rounded to bf16 before they
+ * meet the values; an f32 pool is computed with all 24 bits.  Slots behind a sequence's end may hold anything. A value that is not
+ * finite, in a slot of the sequence, can reach every token whose call reads that slot. */
+int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *batch, const void *q_dev, float scale, void *out_dev,
+                          lumen_dtype out_dtype, float *lse_dev);
+/* What the cached positions were looked at: mass[slot of j] += sum over the new tokens that see j and the query heads of its key
+ * head of exp(scale * q . k_j - lse), with the lse of lumen_paged_attention for the same q and scale; the order of the sum is
+ * fixed.  Refused: sequences that share a page. */
+int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *batch, const void *q_dev, float scale, const float *lse_dev);
+/* Shrinks caches: of the kv_lens[s] positions of sequence s of `from`, to->kv_lens[s] stay: per key head the last `recent` (at most
+ * all that stay) and, of those before, the ones with the largest mass (equal: the lower position; NaN below all
+ * others).  Keys, values and mass of what stays move, in order, to the pages of `to`, which must belong to no other
+ * sequence of either batch; `from`'s pages stay as they were.  kept[s, h, i] (int32, rows of kept_stride) is the former
+ * position of the i-th; what lies behind to->kv_lens[s] is left as it was. */
+int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const lumen_page_batch *to, size_t recent, int32_t *kept_dev,
+                      size_t kept_stride);
 
 /* ---- measurement helpers (no counterpart in the reference) ----------------------------------
  * A kernel timed as a kernel: `iters` calls of lumen_gemv (src/ops/matmul.rs:42-69) / lumen_attention_decode

@@ -17,6 +17,7 @@ from .fegetar import FegetarConfig, FegetarModel  # noqa: E402
 from .fekorax import FekoraxConfig, FekoraxModel  # noqa: E402
 from .loader import load_llama_weights, load_weights  # noqa: E402
 from .model import LanguageModel  # noqa: E402
+from .paged import PageBatch, PagePool, paged_append, paged_attention, paged_attention_mass, paged_evict  # noqa: E402
 from .registry import load_model, model_config  # noqa: E402
 from .tokenizer import LlamaTokenizer  # noqa: E402
 from .tensor import (Context, Tensor, default_context, is_inference_mode, is_no_grad, no_grad,  # noqa: E402
@@ -28,4 +29,5 @@ __all__ = [
     "SelfAttention", "KVCache", "KVCacheInner", "LlamaKVCache", "LlamaConfig", "LlamaModel", "LlamaTokenizer", "load_llama_weights",
     "FegetarConfig", "FegetarModel", "FekoraxConfig", "FekoraxModel", "LanguageModel", "load_model", "load_weights", "model_config", "matmul", "reshape",
     "fused_softmax", "gemv", "gemv_kn_static", "gemv_repeat", "attention_decode", "attention_decode_repeat", "sample_top_p",
+    "PageBatch", "PagePool", "paged_append", "paged_attention", "paged_attention_mass", "paged_evict",
 ]

@@ -107,6 +107,7 @@ PROTOTYPES = {
     "lumen_attention_decode_repeat": (_I, [_P, _FP, _FP, _FP, _SZ, _P, _SZ, _P, _FP, _SZ, C.POINTER(C.c_float)]),
     "lumen_gemv_kn_static": (_I, [_P, _FP, _P, _I, _SZ, _SZ, _FP]),
     "lumen_rope_new": (_I, [_P, _SZ, _SZ, _F, _PP]),
+    "lumen_rope_from_tables": (_I, [_P, _SZ, _SZ, _FP, _FP, _PP]),
     "lumen_rope_forward": (_I, [_P, _P, _SZ, _PP]),
     "lumen_rope_free": (_I, [_P]),
     "lumen_kv_new": (_I, [_P, _SZ, _SZ, _SZ, _SZ, _PP]),
@@ -145,6 +146,17 @@ PROTOTYPES = {
     "lumen_model_forward_sample": (_I, [_P, _FP, _SZ, _PP, _SZ, C.POINTER(SampleParamsC), C.POINTER(C.c_int32)]),
     "lumen_model_weight_bytes": (_SZ, [_P]),
     "lumen_model_free": (_I, [_P]),
+    "lumen_page_pool_new": (_I, [_P, _SZ, _SZ, _SZ, _SZ, _I, _PP]),
+    "lumen_page_pool_k": (_P, [_P]),
+    "lumen_page_pool_v": (_P, [_P]),
+    "lumen_page_pool_mass": (_P, [_P]),
+    "lumen_page_pool_free": (_I, [_P]),
+    "lumen_page_batch_new": (_I, [_P, _SZ, _SZ, _P, _P, _P, _P, _SZ, _I, _PP]),
+    "lumen_page_batch_free": (_I, [_P]),
+    "lumen_paged_append": (_I, [_P, _P, _P, _FP, _FP, _FP, _SZ, _SZ, _FP, _FP, _F, _P]),
+    "lumen_paged_attention": (_I, [_P, _P, _P, _F, _P, _I, _FP]),
+    "lumen_paged_attention_mass": (_I, [_P, _P, _P, _F, _FP]),
+    "lumen_paged_evict": (_I, [_P, _P, _P, _SZ, _P, _SZ]),
     "lumen_llama_weight_bytes": (_SZ, [_P]),
     "lumen_llama_decode_trace": (_I, [_P, C.POINTER(C.c_uint64), _SZ, _SZP]),
 }

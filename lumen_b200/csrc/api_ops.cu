@@ -79,6 +79,24 @@ int require_f32(lumen_ctx *ctx, const lumen_tensor *t, const char *what) {
     return LUMEN_OK;
 }
 
+int new_rope(lumen_ctx *ctx, size_t dim, size_t max_seq_len, float theta, const float *cos_h, const float *sin_h, lumen_rope **out) {
+    auto *r = new lumen_rope();
+    r->ctx = ctx; r->dim = dim; r->max_seq = max_seq_len; r->theta = theta;
+    const size_t n = max_seq_len * (dim / 2), bytes = std::max<size_t>(n * 4, 16);
+    cudaError_t e;
+    if ((e = cudaMalloc(&r->cos_t, bytes)) != cudaSuccess || (e = cudaMalloc(&r->sin_t, bytes)) != cudaSuccess) {
+        if (r->cos_t) cudaFree(r->cos_t);
+        delete r;
+        return cuda_fail(ctx, e, "cudaMalloc(rope tables)");
+    }
+    if (n) {
+        LUMEN_CUDA(ctx, cudaMemcpyAsync(r->cos_t, cos_h, n * 4, cudaMemcpyHostToDevice, ctx->stream));
+        LUMEN_CUDA(ctx, cudaMemcpyAsync(r->sin_t, sin_h, n * 4, cudaMemcpyHostToDevice, ctx->stream));
+    }
+    *out = r;
+    return LUMEN_OK;
+}
+
 }  // namespace
 
 namespace {
@@ -262,20 +280,17 @@ int lumen_rope_new(lumen_ctx *ctx, size_t dim, size_t max_seq_len, float theta, 
     if (dim == 0 || (dim & 1)) return set_error(ctx, LUMEN_ERR_SHAPE, "RoPE dim must be even, got %zu", dim);
     std::vector<float> ch, sh;
     rope_tables_host(dim, max_seq_len, theta, ch, sh);
-    auto *r = new lumen_rope();
-    r->ctx = ctx; r->dim = dim; r->max_seq = max_seq_len; r->theta = theta;
-    const size_t bytes = std::max<size_t>(ch.size() * 4, 16);
-    cudaError_t e;
-    if ((e = cudaMalloc(&r->cos_t, bytes)) != cudaSuccess || (e = cudaMalloc(&r->sin_t, bytes)) != cudaSuccess) {
-        if (r->cos_t) cudaFree(r->cos_t);
-        delete r;
-        return cuda_fail(ctx, e, "cudaMalloc(rope tables)");
-    }
-    if (!ch.empty()) {
-        LUMEN_CUDA(ctx, cudaMemcpyAsync(r->cos_t, ch.data(), ch.size() * 4, cudaMemcpyHostToDevice, ctx->stream));
-        LUMEN_CUDA(ctx, cudaMemcpyAsync(r->sin_t, sh.data(), sh.size() * 4, cudaMemcpyHostToDevice, ctx->stream));
-    }
-    *out = r;
+    return new_rope(ctx, dim, max_seq_len, theta, ch.data(), sh.data(), out);
+}
+
+int lumen_rope_from_tables(lumen_ctx *ctx, size_t dim, size_t max_seq_len, const float *cos_host, const float *sin_host, lumen_rope **out) {
+    if (!ctx || !out) return LUMEN_ERR_INVALID;
+    *out = nullptr;
+    if (dim == 0 || (dim & 1)) return set_error(ctx, LUMEN_ERR_SHAPE, "RoPE dim must be even, got %zu", dim);
+    if (max_seq_len > SIZE_MAX / 2 / dim) return set_error(ctx, LUMEN_ERR_SHAPE, "RoPE tables of %zu positions", max_seq_len);
+    if (max_seq_len && (!cos_host || !sin_host)) return set_error(ctx, LUMEN_ERR_INVALID, "rope_from_tables: null argument");
+    LUMEN_TRY(new_rope(ctx, dim, max_seq_len, 0.f, cos_host, sin_host, out));
+    LUMEN_CUDA(ctx, cudaStreamSynchronize(ctx->stream));  // the host tables may be pinned, and reused on return
     return LUMEN_OK;
 }
 

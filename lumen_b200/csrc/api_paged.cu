@@ -1,0 +1,264 @@
+// C ABI of the paged key/value cache: pools of pages, batches of sequences, and the calls that fill, read, observe and shrink them.
+#include <cstdlib>
+#include <new>
+
+#include "paged.cuh"
+
+using namespace lumen;
+
+namespace {
+
+// The context's device is current while one of these lives (the caller's own is put back).
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(const lumen_ctx *ctx) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = now;
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+int log2_of(int x) {
+    int n = 0;
+    while ((1 << n) < x) ++n;
+    return n;
+}
+
+PagedView view_of(const lumen_page_pool *pool, const lumen_page_batch *b) {
+    PagedView v = {};
+    v.k = pool->k; v.v = pool->v; v.mass = pool->mass;
+    v.seqs = b->seqs; v.tables = b->tables; v.tok_slot = b->tok_slot; v.tok_pos = b->tok_pos;
+    v.page_shift = log2_of(b->g.page); v.h_kv = b->g.h_kv; v.n_head = b->plan.n_head; v.group = b->plan.group; v.causal = b->plan.causal;
+    v.n_seq = b->plan.n_seq; v.tokens = b->plan.tokens;
+    return v;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_pair(const lumen_page_pool *pool, const lumen_page_batch *b, const char *what) {
+    if (!pool) return LUMEN_ERR_INVALID;
+    if (!b) return set_error(pool->ctx, LUMEN_ERR_INVALID, "%s: null batch", what);
+    if (b->ctx != pool->ctx) return set_error(pool->ctx, LUMEN_ERR_INVALID, "%s: pool and batch of different contexts", what);
+    if (!(b->g == pool->g)) return set_error(pool->ctx, LUMEN_ERR_SHAPE, "%s: the batch was made for another geometry of pools", what);
+    return LUMEN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lumen_page_pool_new(lumen_ctx *ctx, size_t pages, size_t page_size, size_t h_kv, size_t d, lumen_dtype dtype, lumen_page_pool **out) {
+    if (!ctx || !out) return LUMEN_ERR_INVALID;
+    *out = nullptr;
+    if (dtype != LUMEN_F32 && dtype != LUMEN_BF16) return set_error(ctx, LUMEN_ERR_DTYPE, "page_pool: dtype %d", (int)dtype);
+    if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)))
+        return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "page_pool: page_size %zu is not a power of two from 8 to 256", page_size);
+    if (d != 64 && d != 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "page_pool: head size %zu is neither 64 nor 128", d);
+    if (pages == 0 || h_kv == 0 || h_kv > 65535 || pages > INT32_MAX / page_size)
+        return set_error(ctx, LUMEN_ERR_INVALID, "page_pool: %zu pages of %zu positions, %zu key heads", pages, page_size, h_kv);
+    OnDevice on(ctx);
+    auto *p = new (std::nothrow) lumen_page_pool();
+    if (!p) return set_error(ctx, LUMEN_ERR_INVALID, "page_pool: out of host memory");
+    p->ctx = ctx;
+    p->g.pages = (int)pages; p->g.page = (int)page_size; p->g.h_kv = (int)h_kv; p->g.d = (int)d; p->g.dtype = dtype;
+    const size_t slots = pages * page_size * h_kv, bytes = slots * d * (dtype == LUMEN_F32 ? 4 : 2);
+    char *mem = nullptr;  // (bytes is a multiple of 1024: all three parts start aligned)
+    cudaError_t e = cudaMalloc(&mem, 2 * bytes + slots * 4);
+    if (e == cudaSuccess) e = cudaMemsetAsync(mem, 0, 2 * bytes + slots * 4, ctx->stream);
+    if (e != cudaSuccess) {
+        if (mem) cudaFree(mem);
+        delete p;
+        return cuda_fail(ctx, e, "page_pool memory");
+    }
+    p->k = mem;
+    p->v = mem + bytes;
+    p->mass = reinterpret_cast<float *>(mem + 2 * bytes);
+    *out = p;
+    return LUMEN_OK;
+}
+
+void *lumen_page_pool_k(const lumen_page_pool *pool) { return pool ? pool->k : nullptr; }
+void *lumen_page_pool_v(const lumen_page_pool *pool) { return pool ? pool->v : nullptr; }
+float *lumen_page_pool_mass(const lumen_page_pool *pool) { return pool ? pool->mass : nullptr; }
+
+int lumen_page_pool_free(lumen_page_pool *pool) {
+    if (!pool) return LUMEN_ERR_INVALID;
+    OnDevice on(pool->ctx);
+    cudaStreamSynchronize(pool->ctx->stream);
+    cudaFree(pool->k);
+    delete pool;
+    return LUMEN_OK;
+}
+
+int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_seq, const int32_t *q_lens, const int32_t *kv_lens,
+                         const int32_t *first_pos, const int32_t *tables, size_t table_stride, int causal, lumen_page_batch **out) {
+    if (!pool || !out) return LUMEN_ERR_INVALID;
+    *out = nullptr;
+    lumen_ctx *ctx = pool->ctx;
+    OnDevice on(ctx);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    LUMEN_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+    if (capture != cudaStreamCaptureStatusNone) return set_error(ctx, LUMEN_ERR_INVALID, "page_batch: the context's stream is being captured");
+    lumen_page_batch *b = nullptr;
+    try {
+        b = new lumen_page_batch();
+        b->ctx = ctx;
+        b->g = pool->g;
+        std::string why;
+        int rc = paged_layout(b->g, n_head, n_seq, q_lens, kv_lens, first_pos, tables, table_stride, causal, b->plan, why);
+        if (rc != LUMEN_OK) {
+            delete b;
+            return set_error(ctx, rc, "page_batch: %s", why.c_str());
+        }
+        PagedPlan &p = b->plan;
+        std::vector<int> live;
+        for (int s = 0; s < p.n_seq; ++s)
+            if (p.seqs[(size_t)s].q_len) live.push_back(s);
+        paged_cut(p, b->g, paged_rows_shape(b->g, ctx->num_sms), live);
+        // everything the kernels read goes up in one copy, in front of the workspace
+        std::vector<char> up;
+        auto put = [&](const void *data, size_t bytes) {
+            const size_t at = (up.size() + 15) & ~(size_t)15;
+            up.resize(at + bytes);
+            if (bytes) memcpy(up.data() + at, data, bytes);
+            return at;
+        };
+        const size_t o_seqs = put(p.seqs.data(), p.seqs.size() * sizeof(PagedSeq)), o_tab = put(p.tables.data(), p.tables.size() * 4);
+        const size_t o_slot = put(p.tok_slot.data(), p.tok_slot.size() * 4), o_pos = put(p.tok_pos.data(), p.tok_pos.size() * 4);
+        const size_t o_it = put(p.items.data(), p.items.size() * sizeof(PagedItem)), o_jo = put(p.joins.data(), p.joins.size() * sizeof(PagedJoin));
+        const size_t o_part = (up.size() + 255) & ~(size_t)255;
+        rc = dev_alloc(ctx, o_part + (size_t)p.part_rows * (size_t)(b->g.d + 2) * 4, &b->dev);
+        if (rc == LUMEN_OK && !up.empty()) {
+            // (pageable memory: the call returns once it has been read)
+            const cudaError_t e = cudaMemcpyAsync(b->dev, up.data(), up.size(), cudaMemcpyHostToDevice, ctx->stream);
+            if (e != cudaSuccess) {
+                dev_free(ctx, b->dev);
+                rc = cuda_fail(ctx, e, "page_batch copy");
+            }
+        }
+        if (rc != LUMEN_OK) {
+            delete b;
+            return rc;
+        }
+        char *at = static_cast<char *>(b->dev);
+        b->seqs = reinterpret_cast<PagedSeq *>(at + o_seqs);
+        b->tables = reinterpret_cast<int *>(at + o_tab);
+        b->tok_slot = reinterpret_cast<int *>(at + o_slot);
+        b->tok_pos = reinterpret_cast<int *>(at + o_pos);
+        b->items = reinterpret_cast<PagedItem *>(at + o_it);
+        b->joins = reinterpret_cast<PagedJoin *>(at + o_jo);
+        b->part = reinterpret_cast<float *>(at + o_part);
+    } catch (const std::exception &) {
+        delete b;
+        return set_error(ctx, LUMEN_ERR_INVALID, "page_batch: out of host memory");
+    }
+    *out = b;
+    return LUMEN_OK;
+}
+
+int lumen_page_batch_free(lumen_page_batch *batch) {
+    if (!batch) return LUMEN_ERR_INVALID;
+    OnDevice on(batch->ctx);
+    const int rc = dev_free(batch->ctx, batch->dev);
+    delete batch;
+    return rc;
+}
+
+int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, const lumen_rope *rope, const float *q_dev, const float *k_dev,
+                       const float *v_dev, size_t q_stride, size_t kv_stride, const float *q_norm_dev, const float *k_norm_dev, float eps,
+                       void *q_out_dev) {
+    LUMEN_TRY(check_pair(pool, batch, "paged_append"));
+    lumen_ctx *ctx = pool->ctx;
+    const PagedPlan &p = batch->plan;
+    if (!q_dev || !k_dev || !v_dev || !q_out_dev) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: null argument");
+    if (!aligned16(q_out_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: q_out is not 16-byte aligned");
+    const size_t d = (size_t)pool->g.d;
+    if (q_stride < (size_t)p.n_head * d || kv_stride < (size_t)pool->g.h_kv * d)
+        return set_error(ctx, LUMEN_ERR_SHAPE, "paged_append: rows of %zu and %zu floats overlap", q_stride, kv_stride);
+    if (!p.can_append) return set_error(ctx, LUMEN_ERR_SHAPE, "paged_append: a sequence has more new tokens than positions");
+    if (p.write_shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: a page that receives rows belongs to two sequences");
+    if (rope) {
+        if (rope->ctx != ctx) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: tables of another context");
+        if (rope->dim != d) return set_error(ctx, LUMEN_ERR_SHAPE, "RoPE dimension mismatch");
+        if (p.max_pos >= (long long)rope->max_seq)
+            return set_error(ctx, LUMEN_ERR_ROPE_RANGE, "RoPE index out of range: pos %lld >= max %zu", p.max_pos, rope->max_seq);
+    }
+    if (p.tokens == 0) return LUMEN_OK;
+    OnDevice on(ctx);
+    PagedAppendArgs a = {};
+    a.q = q_dev; a.k = k_dev; a.v = v_dev; a.q_norm = q_norm_dev; a.k_norm = k_norm_dev;
+    a.cos_t = rope ? rope->cos_t : nullptr; a.sin_t = rope ? rope->sin_t : nullptr;
+    a.q_stride = q_stride; a.kv_stride = kv_stride; a.eps = eps; a.q_out = q_out_dev;
+    return launch_paged_append(ctx, pool->g, view_of(pool, batch), a, ctx->stream);
+}
+
+int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *batch, const void *q_dev, float scale, void *out_dev,
+                          lumen_dtype out_dtype, float *lse_dev) {
+    LUMEN_TRY(check_pair(pool, batch, "paged_attention"));
+    lumen_ctx *ctx = pool->ctx;
+    const PagedPlan &p = batch->plan;
+    if (!q_dev || !out_dev) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: null argument");
+    if (out_dtype != LUMEN_F32 && !(out_dtype == LUMEN_BF16 && pool->g.dtype == LUMEN_BF16))
+        return set_error(ctx, LUMEN_ERR_DTYPE, "paged_attention: output type %d from a pool of type %d", (int)out_dtype, (int)pool->g.dtype);
+    if (!aligned16(q_dev) || !aligned16(out_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q or out is not 16-byte aligned");
+    if (!(scale - scale == 0.f)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: scale is not finite");
+    const size_t n = (size_t)p.tokens * p.n_head * pool->g.d;
+    const char *q0 = static_cast<const char *>(q_dev), *o0 = static_cast<const char *>(out_dev);
+    if (q0 < o0 + n * (out_dtype == LUMEN_F32 ? 4 : 2) && o0 < q0 + n * (pool->g.dtype == LUMEN_F32 ? 4 : 2))
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q and out overlap");
+    if (p.tokens == 0) return LUMEN_OK;
+    OnDevice on(ctx);
+    PagedAttnArgs a = {};
+    a.q = q_dev; a.scale = scale; a.out = out_dev; a.out_dtype = out_dtype; a.lse = lse_dev;
+    a.items = batch->items; a.n_items = (int)p.items.size();
+    for (const PagedItem &it : p.items) a.max_rows = std::max(a.max_rows, it.rows);
+    a.part = batch->part; a.part_rows = p.part_rows; a.joins = batch->joins; a.n_joins = (int)p.joins.size();
+    for (const PagedJoin &j : p.joins) a.join_rows = std::max(a.join_rows, j.rows);
+    const PagedView v = view_of(pool, batch);
+    LUMEN_TRY(launch_paged_rows(ctx, pool->g, v, a, ctx->stream));
+    return a.n_joins ? launch_paged_join(ctx, pool->g, v, a, ctx->stream) : LUMEN_OK;
+}
+
+int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *batch, const void *q_dev, float scale, const float *lse_dev) {
+    LUMEN_TRY(check_pair(pool, batch, "paged_attention_mass"));
+    lumen_ctx *ctx = pool->ctx;
+    const PagedPlan &p = batch->plan;
+    if (!q_dev || !lse_dev) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: null argument");
+    if (!aligned16(q_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: q is not 16-byte aligned");
+    if (!(scale - scale == 0.f)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: scale is not finite");
+    if (p.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: two sequences share a page");
+    if (p.tokens == 0 || p.max_kv == 0) return LUMEN_OK;
+    OnDevice on(ctx);
+    return launch_paged_mass(ctx, pool->g, view_of(pool, batch), q_dev, scale, lse_dev, p.max_kv, ctx->stream);
+}
+
+int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const lumen_page_batch *to, size_t recent, int32_t *kept_dev,
+                      size_t kept_stride) {
+    LUMEN_TRY(check_pair(pool, from, "paged_evict"));
+    LUMEN_TRY(check_pair(pool, to, "paged_evict"));
+    lumen_ctx *ctx = pool->ctx;
+    const PagedPlan &a = from->plan, &b = to->plan;
+    if (!kept_dev) return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: null argument");
+    if (a.n_seq != b.n_seq) return set_error(ctx, LUMEN_ERR_SHAPE, "paged_evict: %d sequences into %d", a.n_seq, b.n_seq);
+    for (int s = 0; s < a.n_seq; ++s)
+        if (b.seqs[(size_t)s].kv_len > a.seqs[(size_t)s].kv_len)
+            return set_error(ctx, LUMEN_ERR_SHAPE, "paged_evict: sequence %d: %d of %d positions", s, b.seqs[(size_t)s].kv_len, a.seqs[(size_t)s].kv_len);
+    if ((size_t)b.max_kv > kept_stride) return set_error(ctx, LUMEN_ERR_SHAPE, "paged_evict: rows of %zu for %d positions", kept_stride, b.max_kv);
+    if (b.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: two sequences share a page of the destination");
+    try {
+        std::vector<char> used((size_t)pool->g.pages, 0);
+        for (int page : a.tables) used[(size_t)page] = 1;
+        for (int page : b.tables)
+            if (used[(size_t)page]) return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: page %d is source and destination", page);
+    } catch (const std::exception &) {
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: out of host memory");
+    }
+    if (b.max_kv == 0) return LUMEN_OK;
+    OnDevice on(ctx);
+    return launch_paged_evict(ctx, pool->g, view_of(pool, from), view_of(pool, to), (int)std::min<size_t>(recent, INT32_MAX), b.max_kv, kept_dev,
+                              kept_stride, ctx->stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,71 @@
+// Handles and launchers of the paged key/value cache (api_paged.cu).
+#pragma once
+
+#include "common.cuh"
+#include "paged_plan.cuh"
+
+struct lumen_page_pool {
+    lumen_ctx *ctx = nullptr;
+    lumen::PagedGeom g;
+    void *k = nullptr, *v = nullptr;  // [pages, h_kv, page, d]
+    float *mass = nullptr;            // [pages, h_kv, page]
+};
+
+struct lumen_page_batch {
+    lumen_ctx *ctx = nullptr;
+    lumen::PagedGeom g;
+    lumen::PagedPlan plan;
+    void *dev = nullptr;  // one allocation: what follows
+    lumen::PagedSeq *seqs = nullptr;
+    int *tables = nullptr, *tok_slot = nullptr, *tok_pos = nullptr;
+    lumen::PagedItem *items = nullptr;
+    lumen::PagedJoin *joins = nullptr;
+    float *part = nullptr;  // partial sums [part_rows, d], then their maxima and sums [part_rows, 2]
+};
+
+namespace lumen {
+
+// What the kernels read of a pool and a batch.
+struct PagedView {
+    void *k, *v;
+    float *mass;
+    const PagedSeq *seqs;
+    const int *tables, *tok_slot, *tok_pos;
+    int page_shift, h_kv, n_head, group, causal, n_seq, tokens;
+};
+
+// Slot of position `pos` of a key head, counted in rows of d numbers (or in single masses).
+__device__ __forceinline__ size_t paged_row(const PagedView &v, const int *table, int kvh, int pos) {
+    const int page = table[pos >> v.page_shift];
+    return (((size_t)page * v.h_kv + kvh) << v.page_shift) + (pos & ((1 << v.page_shift) - 1));
+}
+
+struct PagedAppendArgs {
+    const float *q, *k, *v, *q_norm, *k_norm, *cos_t, *sin_t;
+    size_t q_stride, kv_stride;
+    float eps;
+    void *q_out;
+};
+int launch_paged_append(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAppendArgs &a, cudaStream_t s);
+
+struct PagedAttnArgs {
+    const void *q;
+    float scale;
+    void *out;
+    lumen_dtype out_dtype;
+    float *lse;
+    const PagedItem *items;
+    int n_items, max_rows;
+    float *part;
+    long long part_rows;
+    const PagedJoin *joins;
+    int n_joins, join_rows;
+};
+PagedShape paged_rows_shape(const PagedGeom &g, int num_sms);
+int launch_paged_rows(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
+int launch_paged_join(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
+int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const void *q, float scale, const float *lse, int max_kv, cudaStream_t s);
+int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_keep, int *kept,
+                       size_t kept_stride, cudaStream_t s);
+
+}  // namespace lumen

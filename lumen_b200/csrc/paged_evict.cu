@@ -1,0 +1,136 @@
+// Eviction: the positions of a sequence that received most attention, and its last ones, go to new pages.
+//
+// paged_select_kernel, a CTA per sequence and key head: the weights as ordered 32-bit integers; four passes over 8 bits each narrow the
+// value of the last one that stays (a histogram in shared memory; whole numbers, so the order of its atomics changes nothing), a fifth
+// pass writes the positions in order, of the equal ones the lowest.  paged_move_kernel copies the rows: bound by HBM.
+#include "paged.cuh"
+
+namespace lumen {
+namespace {
+
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+
+// Larger weight, larger number; NaN the smallest of all.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    if (x != x) return 0u;
+    const uint32_t u = __float_as_uint(x + 0.f);  // (-0 becomes 0)
+    return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+// grid (key heads, sequences)
+__global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView from, const PagedSeq *to_seqs, int recent, int *kept, size_t kept_stride) {
+    __shared__ unsigned hist[256];
+    __shared__ unsigned prefix_s, want_s;
+    __shared__ unsigned warp_s[kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.x, s = blockIdx.y;
+    const PagedSeq sq = from.seqs[s];
+    const int len = sq.kv_len, keep = to_seqs[s].kv_len, last = min(recent, keep), old = len - last, pick = keep - last;
+    const int *table = from.tables + sq.table;
+    int *out = kept + ((size_t)s * from.h_kv + kvh) * kept_stride;
+    for (int i = tid; i < last; i += kThreads) out[pick + i] = old + i;
+    if (pick == 0) return;
+    auto value = [&](int pos) { return order_of(from.mass[paged_row(from, table, kvh, pos)]); };
+    // the pick-th largest value: `prefix` are its leading bits, `want` how many of those that share them are still to be taken
+    if (tid == 0) prefix_s = 0u, want_s = (unsigned)pick;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0u;
+        __syncthreads();
+        const unsigned prefix = prefix_s;
+        for (int i = tid; i < old; i += kThreads) {
+            const uint32_t u = value(i);
+            if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (warp == 0) {  // lane l: bins 255 - 8 l down to 248 - 8 l
+            unsigned c[8], mine = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = hist[255 - 8 * lane - i], mine += c[i];
+            unsigned incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned want = want_s;
+            unsigned before = incl - mine;
+            __syncwarp();
+            if (before < want && want <= incl)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (before < want && want <= before + c[i]) {
+                        prefix_s = prefix | ((unsigned)(255 - 8 * lane - i) << shift);
+                        want_s = want - before;
+                    }
+                    before += c[i];
+                }
+        }
+        __syncthreads();
+    }
+    const unsigned edge = prefix_s, ties = want_s;  // all above `edge` stay, and the first `ties` equal to it
+    unsigned above = 0u, equal = 0u;  // so far
+    for (int i0 = 0; i0 < old; i0 += kThreads) {
+        const int i = i0 + tid;
+        const uint32_t u = i < old ? value(i) : 0u;
+        const bool gt = i < old && u > edge, eq = i < old && u == edge;
+        const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq), low = (1u << lane) - 1u;
+        if (lane == 0) warp_s[warp] = (unsigned)__popc(mg) | ((unsigned)__popc(me) << 16);
+        __syncthreads();
+        unsigned before = 0u, all = 0u;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) before = all;
+            all += warp_s[w];
+        }
+        const unsigned g = above + (before & 0xffffu) + (unsigned)__popc(mg & low), e = equal + (before >> 16) + (unsigned)__popc(me & low);
+        if (gt || (eq && e < ties)) out[g + min(e, ties)] = i;
+        above += all & 0xffffu;
+        equal += all >> 16;
+        __syncthreads();
+    }
+}
+
+// grid (groups of rows, key heads, sequences): 16 bytes a thread
+template <int B>  // bytes of a row
+__global__ void __launch_bounds__(256) paged_move_kernel(const PagedView from, const PagedView to, const int *kept, size_t kept_stride) {
+    constexpr int kLanes = B / 16, kRowsPer = 256 / kLanes;
+    const int kvh = blockIdx.y, s = blockIdx.z, lane = threadIdx.x % kLanes, i = (int)blockIdx.x * kRowsPer + threadIdx.x / kLanes;
+    const PagedSeq a = from.seqs[s], b = to.seqs[s];
+    if (i >= b.kv_len) return;
+    const int pos = kept[((size_t)s * from.h_kv + kvh) * kept_stride + i];
+    const size_t src = paged_row(from, from.tables + a.table, kvh, pos), dst = paged_row(to, to.tables + b.table, kvh, i);
+    const size_t so = src * B + 16 * lane, d = dst * B + 16 * lane;
+    const uint4 k = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const char *>(from.k) + so));
+    const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const char *>(from.v) + so));
+    *reinterpret_cast<uint4 *>(static_cast<char *>(to.k) + d) = k;
+    *reinterpret_cast<uint4 *>(static_cast<char *>(to.v) + d) = v;
+    if (lane == 0) to.mass[dst] = from.mass[src];
+}
+
+template <int B>
+int move(lumen_ctx *ctx, const PagedView &from, const PagedView &to, int n, int max_keep, const int *kept, size_t kept_stride, cudaStream_t s) {
+    constexpr int kRowsPer = 256 / (B / 16);
+    const dim3 grid((unsigned)((max_keep + kRowsPer - 1) / kRowsPer), (unsigned)from.h_kv, (unsigned)n);
+    paged_move_kernel<B><<<grid, 256, 0, s>>>(from, to, kept, kept_stride);
+    LUMEN_LAUNCHED(ctx);
+    return LUMEN_OK;
+}
+
+}  // namespace
+
+int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_keep, int *kept,
+                       size_t kept_stride, cudaStream_t s) {
+    const int bytes = g.d * (g.dtype == LUMEN_F32 ? 4 : 2);
+    for (int s0 = 0; s0 < from.n_seq; s0 += 32768) {  // (the grid's extents)
+        const int n = std::min(from.n_seq - s0, 32768);
+        PagedView f = from, t = to;
+        f.seqs += s0;
+        t.seqs += s0;
+        int *k = kept + (size_t)s0 * from.h_kv * kept_stride;
+        paged_select_kernel<<<dim3((unsigned)from.h_kv, (unsigned)n), kThreads, 0, s>>>(f, t.seqs, recent, k, kept_stride);
+        LUMEN_LAUNCHED(ctx);
+        LUMEN_TRY(bytes == 128 ? move<128>(ctx, f, t, n, max_keep, k, kept_stride, s)
+                  : bytes == 256 ? move<256>(ctx, f, t, n, max_keep, k, kept_stride, s) : move<512>(ctx, f, t, n, max_keep, k, kept_stride, s));
+    }
+    return LUMEN_OK;
+}
+
+}  // namespace lumen

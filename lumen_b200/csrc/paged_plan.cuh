@@ -1,0 +1,172 @@
+// Plan of one step over a paged cache: checks of lengths and tables, and the work of the attention kernels as lists.  Plain host arithmetic
+// (no CUDA), so that programs of the host can check it.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+#include <string>
+#include <vector>
+
+#include "../../include/lumen_b200.h"
+
+namespace lumen {
+
+struct PagedGeom {
+    int pages = 0, page = 0, h_kv = 0, d = 0;
+    lumen_dtype dtype = LUMEN_F32;
+    bool operator==(const PagedGeom &o) const { return pages == o.pages && page == o.page && h_kv == o.h_kv && d == o.d && dtype == o.dtype; }
+};
+
+struct PagedSeq {
+    int tok0, q_len, kv_len;
+    int table;  // where its page numbers start
+};
+
+// Rows of one key head of a sequence: row r is new token r / group, query head kvh * group + r % group.  An item is `rows` of them from row0
+// against the cached positions [key0, key1); part < 0: the result is final, else its partial sums are rows part .. part + rows - 1.
+struct PagedItem {
+    int seq, kvh, row0, rows, key0, key1, part, pad;
+};
+// Rows whose partial sums are joined: split i's are the rows from part + i * rows.
+struct PagedJoin {
+    int seq, kvh, row0, rows, part, splits;
+};
+// What a kernel takes per item: its rows, the granularity in which it walks the positions, items that run at once.
+struct PagedShape {
+    int rows, keys, slots;
+};
+
+struct PagedPlan {
+    int n_seq = 0, n_head = 0, group = 0, tokens = 0, max_q = 0, max_kv = 0, causal = 1;
+    long long max_pos = -1;        // largest position a new token is rotated to
+    bool shared = false;           // a page belongs to two sequences
+    bool write_shared = false;     // such a page receives new rows
+    bool can_append = true;        // every new token has a slot
+    std::vector<PagedSeq> seqs;
+    std::vector<int> tables;       // page numbers, sequence after sequence
+    std::vector<int> tok_slot, tok_pos;  // of every new token: page * page_size + slot, position of the rotation
+    std::vector<PagedItem> items;
+    std::vector<PagedJoin> joins;
+    long long part_rows = 0;
+};
+
+inline int paged_refuse(std::string &err, int code, const char *fmt, long long a = 0, long long b = 0, long long c = 0) {
+    char buf[256];
+    snprintf(buf, sizeof(buf), fmt, a, b, c);
+    err = buf;
+    return code;
+}
+
+// Checks the arguments of lumen_page_batch_new and lays out sequences, tables and tokens.
+inline int paged_layout(const PagedGeom &g, size_t n_head, size_t n_seq, const int32_t *q_lens, const int32_t *kv_lens, const int32_t *first_pos,
+                        const int32_t *tables, size_t table_stride, int causal, PagedPlan &p, std::string &err) {
+    if (n_head == 0 || n_head > (1u << 20) || n_head % (size_t)g.h_kv) return paged_refuse(err, LUMEN_ERR_SHAPE, "%lld query heads over %lld key heads", (long long)n_head, g.h_kv);
+    if (n_seq > (1u << 24)) return paged_refuse(err, LUMEN_ERR_INVALID, "%lld sequences", (long long)n_seq);
+    if (n_seq && (!q_lens || !kv_lens || (table_stride && !tables))) return paged_refuse(err, LUMEN_ERR_INVALID, "null argument");
+    p.n_seq = (int)n_seq;
+    p.n_head = (int)n_head;
+    p.group = (int)n_head / g.h_kv;
+    p.causal = causal != 0;
+    p.seqs.resize(n_seq);
+    long long tokens = 0, entries = 0;
+    for (size_t s = 0; s < n_seq; ++s) {
+        const long long q = q_lens[s], kv = kv_lens[s];
+        if (q < 0 || kv < 0) return paged_refuse(err, LUMEN_ERR_INVALID, "sequence %lld: %lld new tokens, %lld positions", (long long)s, q, kv);
+        if (causal && q > kv) return paged_refuse(err, LUMEN_ERR_SHAPE, "sequence %lld: %lld new tokens but %lld positions", (long long)s, q, kv);
+        const long long need = (kv + g.page - 1) / g.page;
+        if (need > (long long)table_stride) return paged_refuse(err, LUMEN_ERR_KV_OVERFLOW, "sequence %lld: %lld positions in %lld pages", (long long)s, kv, (long long)table_stride);
+        if (first_pos && first_pos[s] < 0) return paged_refuse(err, LUMEN_ERR_INVALID, "sequence %lld: first position %lld", (long long)s, first_pos[s]);
+        p.seqs[s] = {(int)tokens, (int)q, (int)kv, (int)entries};
+        tokens += q;
+        entries += need;
+        if (tokens * p.group > INT32_MAX || entries > INT32_MAX) return paged_refuse(err, LUMEN_ERR_INVALID, "too many tokens or pages");
+        p.max_q = std::max(p.max_q, (int)q);
+        p.max_kv = std::max(p.max_kv, (int)kv);
+        if (q > kv) p.can_append = false;
+    }
+    p.tokens = (int)tokens;
+    p.tables.resize((size_t)entries);
+    std::vector<int> owner((size_t)g.pages, -1);      // the last sequence seen with a page
+    std::vector<char> many((size_t)g.pages, 0), written((size_t)g.pages, 0);
+    for (size_t s = 0; s < n_seq; ++s) {
+        const PagedSeq &q = p.seqs[s];
+        const int need = (q.kv_len + g.page - 1) / g.page, first_new = q.q_len && q.q_len <= q.kv_len ? (q.kv_len - q.q_len) / g.page : need;
+        for (int i = 0; i < need; ++i) {
+            const long long page = tables[s * table_stride + i];
+            if (page < 0 || page >= g.pages) return paged_refuse(err, LUMEN_ERR_INVALID, "sequence %lld: page %lld of a pool of %lld", (long long)s, page, g.pages);
+            if (owner[page] == (int)s) return paged_refuse(err, LUMEN_ERR_INVALID, "sequence %lld: page %lld twice", (long long)s, page);
+            if (owner[page] >= 0) many[page] = 1, p.shared = true;
+            if (i >= first_new) written[page] = 1;
+            if (many[page] && written[page]) p.write_shared = true;
+            owner[page] = (int)s;
+            p.tables[(size_t)q.table + i] = (int)page;
+        }
+    }
+    p.tok_slot.resize((size_t)tokens);
+    p.tok_pos.resize((size_t)tokens);
+    for (size_t s = 0; s < n_seq; ++s) {
+        const PagedSeq &q = p.seqs[s];
+        const long long pos0 = first_pos ? first_pos[s] : q.kv_len - q.q_len;
+        if (q.q_len) p.max_pos = std::max(p.max_pos, pos0 + q.q_len - 1);
+        for (int i = 0; i < q.q_len; ++i) {
+            const int at = q.kv_len - q.q_len + i;
+            p.tok_slot[(size_t)q.tok0 + i] = at < 0 ? -1 : p.tables[(size_t)q.table + at / g.page] * g.page + at % g.page;
+            p.tok_pos[(size_t)q.tok0 + i] = (int)std::min<long long>(pos0 + i, INT32_MAX);
+        }
+    }
+    return LUMEN_OK;
+}
+
+// Positions that a row of token t sees.
+inline int paged_visible(const PagedPlan &p, const PagedSeq &q, int t) { return p.causal ? q.kv_len - q.q_len + t + 1 : q.kv_len; }
+
+// Cuts the rows of `seqs` into items.  Where fewer items than `slots` would run, or some would run long behind the others, the positions are cut
+// too: into parts of at most `most` key tiles, where `most` is what every slot would get of the whole (found by trying, as parts round up).
+// The longest items come first.
+inline void paged_cut(PagedPlan &p, const PagedGeom &g, const PagedShape &shape, const std::vector<int> &seqs) {
+    struct Base {
+        PagedItem it;
+        int tiles;
+    };
+    std::vector<Base> base;
+    long long work = 0;
+    for (int s : seqs) {
+        const PagedSeq &q = p.seqs[(size_t)s];
+        const int rows = q.q_len * p.group;
+        for (int r = 0; r < rows; r += shape.rows) {
+            const int n = std::min(shape.rows, rows - r), end = paged_visible(p, q, (r + n - 1) / p.group), tiles = (end + shape.keys - 1) / shape.keys;
+            for (int h = 0; h < g.h_kv; ++h) base.push_back({{s, h, r, n, 0, end, -1, 0}, tiles}), work += tiles;
+        }
+    }
+    if (base.empty()) return;
+    long long most = std::max<long long>(1, (work + shape.slots - 1) / shape.slots);
+    if ((long long)base.size() <= shape.slots) {
+        auto count = [&](long long m) {
+            long long n = 0;
+            for (const Base &b : base) n += std::max<long long>(1, (b.tiles + m - 1) / m);
+            return n;
+        };
+        while (count(most) > shape.slots) ++most;  // (one part each at the latest: m = the largest number of tiles)
+    }
+    const size_t first = p.items.size();
+    for (const Base &b : base) {
+        const int splits = (int)std::max<long long>(1, (b.tiles + most - 1) / most);
+        if (splits == 1) {
+            p.items.push_back(b.it);
+            continue;
+        }
+        p.joins.push_back({b.it.seq, b.it.kvh, b.it.row0, b.it.rows, (int)p.part_rows, splits});
+        for (int i = 0; i < splits; ++i) {  // part i: tiles [i * tiles / splits, (i + 1) * tiles / splits)
+            PagedItem it = b.it;
+            it.key0 = (int)((long long)b.tiles * i / splits) * shape.keys;
+            it.key1 = std::min(it.key1, (int)((long long)b.tiles * (i + 1) / splits) * shape.keys);
+            it.part = (int)p.part_rows;
+            p.part_rows += it.rows;
+            p.items.push_back(it);
+        }
+    }
+    std::stable_sort(p.items.begin() + (long)first, p.items.end(), [](const PagedItem &a, const PagedItem &b) { return a.key1 - a.key0 > b.key1 - b.key0; });
+}
+
+}  // namespace lumen

@@ -148,6 +148,20 @@ class RotaryEmbedding:
         self.ctx.check(self.ctx._lib.lumen_rope_new(self.ctx.h, dim, max_seq_len, C.c_float(theta), C.byref(self.h)))
         self._finalizer = weakref.finalize(self, self.ctx._lib.lumen_rope_free, C.c_void_p(self.h.value))
 
+    @classmethod
+    def from_tables(cls, cos, sin, ctx: Context | None = None) -> "RotaryEmbedding":
+        """The caller's own tables [max_seq_len, dim / 2] (`lumen_rope_from_tables`): scaled frequencies, angles of 64 bits."""
+        cos, sin = np.ascontiguousarray(cos, np.float32), np.ascontiguousarray(sin, np.float32)
+        if cos.ndim != 2 or cos.shape != sin.shape:
+            raise _lib.LumenError(_lib.ERR_SHAPE, f"tables of {cos.shape} and {sin.shape}: two of [positions, dim / 2] are expected")
+        self = cls.__new__(cls)
+        self.ctx = ctx or default_context()
+        self.dim, self.max_seq_len, self.theta = 2 * cos.shape[1], cos.shape[0], None
+        self.h = C.c_void_p()
+        self.ctx.check(self.ctx._lib.lumen_rope_from_tables(self.ctx.h, self.dim, self.max_seq_len, cos.ctypes.data, sin.ctypes.data, C.byref(self.h)))
+        self._finalizer = weakref.finalize(self, self.ctx._lib.lumen_rope_free, C.c_void_p(self.h.value))
+        return self
+
     def forward(self, x: Tensor, offset: int) -> Tensor:
         h = C.c_void_p()
         self.ctx.check(self.ctx._lib.lumen_rope_forward(self.h, x.h, offset, C.byref(h)))

@@ -1,0 +1,102 @@
+"""Paged key/value cache: pools of pages, batches of sequences, and the calls that fill, read, observe and shrink them
+(`lumen_page_*`, `lumen_paged_*` of include/lumen_b200.h, which says what each takes and refuses).
+
+One step of a serving loop, for every layer:
+
+    batch = PageBatch(pool, n_head, q_lens, kv_lens, tables)            # once per step; fits the pools of all layers
+    paged_append(pool, batch, q, k, v, q_stride, kv_stride, q_out, rope=rope)
+    paged_attention(pool, batch, q_out, scale, out)
+
+Queries, keys, values and outputs are raw device pointers, as for `attention_decode`.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import weakref
+
+import numpy as np
+
+from . import _lib
+from ._lib import BF16, F32  # noqa: F401
+from .layers import RotaryEmbedding
+from .tensor import Context, default_context
+
+
+class PagePool:
+    """Pages of one layer: keys and values [pages, h_kv, page_size, d], attention weight received f32 [pages, h_kv, page_size]."""
+
+    def __init__(self, pages: int, page_size: int, h_kv: int, d: int, dtype: int = BF16, ctx: Context | None = None):
+        self.ctx = ctx or default_context()
+        self.shape, self.dtype = (pages, h_kv, page_size, d), dtype
+        self.h = C.c_void_p()
+        self.ctx.check(self.ctx._lib.lumen_page_pool_new(self.ctx.h, pages, page_size, h_kv, d, dtype, C.byref(self.h)))
+        self._finalizer = weakref.finalize(self, self.ctx._lib.lumen_page_pool_free, C.c_void_p(self.h.value))
+
+    @property
+    def k_ptr(self) -> int:
+        return int(self.ctx._lib.lumen_page_pool_k(self.h) or 0)
+
+    @property
+    def v_ptr(self) -> int:
+        return int(self.ctx._lib.lumen_page_pool_v(self.h) or 0)
+
+    @property
+    def mass_ptr(self) -> int:
+        return int(self.ctx._lib.lumen_page_pool_mass(self.h) or 0)
+
+
+def _int32(x, what: str, n: int) -> np.ndarray:
+    a = np.asarray(x)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -(2 ** 31) or a.max() >= 2 ** 31):
+        raise _lib.LumenError(_lib.ERR_INVALID, f"{what}: 32-bit whole numbers are expected")
+    a = np.ascontiguousarray(a, np.int32)
+    if a.shape != (n,):
+        raise _lib.LumenError(_lib.ERR_SHAPE, f"{what}: shape {a.shape}, {n} sequences")
+    return a
+
+
+class PageBatch:
+    """Sequences of one step: new tokens, cached positions and pages of each.  `tables` is an array [sequences, most pages] or one list of
+    pages per sequence.  Fits every pool of the geometry of `pool`."""
+
+    def __init__(self, pool: PagePool, n_head: int, q_lens, kv_lens, tables, first_pos=None, causal: bool = True):
+        self.ctx, self.n_head = pool.ctx, n_head
+        n = len(q_lens)
+        q, kv = _int32(q_lens, "q_lens", n), _int32(kv_lens, "kv_lens", n)
+        first = None if first_pos is None else _int32(first_pos, "first_pos", n)
+        if len(tables) != n:
+            raise _lib.LumenError(_lib.ERR_SHAPE, f"tables of {len(tables)} sequences, {n} sequences")
+        if isinstance(tables, np.ndarray) and tables.ndim == 2:
+            rows = _int32(tables.reshape(-1), "tables", tables.size).reshape(tables.shape)
+        else:  # (shorter lists are filled up with a page number that is refused if it is ever needed)
+            rows = np.full((n, max((len(t) for t in tables), default=0)), -1, np.int32)
+            for row, t in zip(rows, tables):
+                row[: len(t)] = _int32(t, "tables", len(t))
+        self.tokens, self.q_lens, self.kv_lens = int(q.sum()), q, kv
+        self.h = C.c_void_p()
+        self.ctx.check(self.ctx._lib.lumen_page_batch_new(pool.h, n_head, n, q.ctypes.data, kv.ctypes.data, None if first is None else first.ctypes.data,
+                                                          rows.ctypes.data, rows.shape[1], int(causal), C.byref(self.h)))
+        self._finalizer = weakref.finalize(self, self.ctx._lib.lumen_page_batch_free, C.c_void_p(self.h.value))
+
+
+def paged_append(pool: PagePool, batch: PageBatch, q_ptr: int, k_ptr: int, v_ptr: int, q_stride: int, kv_stride: int, q_out_ptr: int,
+                 rope: RotaryEmbedding | None = None, q_norm_ptr: int = 0, k_norm_ptr: int = 0, eps: float = 0.0) -> None:
+    """The new tokens' f32 projections: norms and rotation of queries and keys, queries to `q_out`, keys and values to their slots."""
+    pool.ctx.check(pool.ctx._lib.lumen_paged_append(pool.h, batch.h, rope.h if rope else None, q_ptr, k_ptr, v_ptr, q_stride, kv_stride,
+                                                    q_norm_ptr or None, k_norm_ptr or None, C.c_float(eps), q_out_ptr))
+
+
+def paged_attention(pool: PagePool, batch: PageBatch, q_ptr: int, scale: float, out_ptr: int, out_dtype: int | None = None, lse_ptr: int = 0) -> None:
+    """Attention of the new tokens over their pages; `out` is of the pool's type unless `out_dtype` says otherwise."""
+    pool.ctx.check(pool.ctx._lib.lumen_paged_attention(pool.h, batch.h, q_ptr, C.c_float(scale), out_ptr,
+                                                       pool.dtype if out_dtype is None else out_dtype, lse_ptr or None))
+
+
+def paged_attention_mass(pool: PagePool, batch: PageBatch, q_ptr: int, scale: float, lse_ptr: int) -> None:
+    """Adds the weights that the cached positions received from the new tokens to the pool's mass."""
+    pool.ctx.check(pool.ctx._lib.lumen_paged_attention_mass(pool.h, batch.h, q_ptr, C.c_float(scale), lse_ptr))
+
+
+def paged_evict(pool: PagePool, source: PageBatch, goal: PageBatch, recent: int, kept_ptr: int, kept_stride: int) -> None:
+    """Moves the positions of `source` that received most weight, and the last `recent`, to the pages of `goal`."""
+    pool.ctx.check(pool.ctx._lib.lumen_paged_evict(pool.h, source.h, goal.h, recent, kept_ptr, kept_stride))

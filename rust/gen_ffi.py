@@ -19,7 +19,7 @@ HEADER = ROOT / "include" / "lumen_b200.h"
 OUT = ROOT / "rust" / "src" / "ffi.rs"
 
 OPAQUE = ["lumen_ctx", "lumen_tensor", "lumen_rope", "lumen_kv_cache", "lumen_llama_kv_cache", "lumen_self_attention",
-          "lumen_llama", "lumen_model"]
+          "lumen_llama", "lumen_model", "lumen_page_pool", "lumen_page_batch"]
 STRUCTS = ["lumen_llama_config", "lumen_decoder_layer", "lumen_decoder_config", "lumen_sample_params"]
 SCALARS = {"int": "c_int", "float": "f32", "double": "f64", "size_t": "usize", "uint64_t": "u64", "int64_t": "i64", "int32_t": "i32",
            "uint16_t": "u16", "char": "c_char", "void": "c_void", "lumen_dtype": "c_int"}

@@ -61,6 +61,14 @@ pub struct lumen_llama {
 pub struct lumen_model {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct lumen_page_pool {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct lumen_page_batch {
+    _private: [u8; 0],
+}
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -173,6 +181,7 @@ extern "C" {
     pub fn lumen_gemv(ctx: *mut lumen_ctx, x_dev: *const f32, w_dev: *const c_void, w_dtype: c_int, layout_kn: c_int, k: usize, n: usize, y_dev: *mut f32) -> c_int;
     pub fn lumen_gemv_kn_static(ctx: *mut lumen_ctx, x_dev: *const f32, w_dev: *const c_void, w_dtype: c_int, k: usize, n: usize, y_dev: *mut f32) -> c_int;
     pub fn lumen_rope_new(ctx: *mut lumen_ctx, dim: usize, max_seq_len: usize, theta: f32, out: *mut *mut lumen_rope) -> c_int;
+    pub fn lumen_rope_from_tables(ctx: *mut lumen_ctx, dim: usize, max_seq_len: usize, cos_host: *const f32, sin_host: *const f32, out: *mut *mut lumen_rope) -> c_int;
     pub fn lumen_rope_forward(rope: *mut lumen_rope, x_bhsd: *const lumen_tensor, offset: usize, out: *mut *mut lumen_tensor) -> c_int;
     pub fn lumen_rope_free(rope: *mut lumen_rope) -> c_int;
     pub fn lumen_kv_new(ctx: *mut lumen_ctx, b: usize, h_kv: usize, max_seq: usize, d: usize, out: *mut *mut lumen_kv_cache) -> c_int;
@@ -213,6 +222,17 @@ extern "C" {
     pub fn lumen_model_forward_sample(m: *mut lumen_model, ids_host: *const f32, s: usize, caches: *mut *mut lumen_kv_cache, n_caches: usize, params: *const lumen_sample_params, token_out: *mut i32) -> c_int;
     pub fn lumen_model_weight_bytes(m: *const lumen_model) -> usize;
     pub fn lumen_model_free(m: *mut lumen_model) -> c_int;
+    pub fn lumen_page_pool_new(ctx: *mut lumen_ctx, pages: usize, page_size: usize, h_kv: usize, d: usize, dtype: c_int, out: *mut *mut lumen_page_pool) -> c_int;
+    pub fn lumen_page_pool_k(pool: *const lumen_page_pool) -> *mut c_void;
+    pub fn lumen_page_pool_v(pool: *const lumen_page_pool) -> *mut c_void;
+    pub fn lumen_page_pool_mass(pool: *const lumen_page_pool) -> *mut f32;
+    pub fn lumen_page_pool_free(pool: *mut lumen_page_pool) -> c_int;
+    pub fn lumen_page_batch_new(pool: *const lumen_page_pool, n_head: usize, n_seq: usize, q_lens: *const i32, kv_lens: *const i32, first_pos: *const i32, tables: *const i32, table_stride: usize, causal: c_int, out: *mut *mut lumen_page_batch) -> c_int;
+    pub fn lumen_page_batch_free(batch: *mut lumen_page_batch) -> c_int;
+    pub fn lumen_paged_append(pool: *mut lumen_page_pool, batch: *const lumen_page_batch, rope: *const lumen_rope, q_dev: *const f32, k_dev: *const f32, v_dev: *const f32, q_stride: usize, kv_stride: usize, q_norm_dev: *const f32, k_norm_dev: *const f32, eps: f32, q_out_dev: *mut c_void) -> c_int;
+    pub fn lumen_paged_attention(pool: *const lumen_page_pool, batch: *const lumen_page_batch, q_dev: *const c_void, scale: f32, out_dev: *mut c_void, out_dtype: c_int, lse_dev: *mut f32) -> c_int;
+    pub fn lumen_paged_attention_mass(pool: *mut lumen_page_pool, batch: *const lumen_page_batch, q_dev: *const c_void, scale: f32, lse_dev: *const f32) -> c_int;
+    pub fn lumen_paged_evict(pool: *mut lumen_page_pool, from: *const lumen_page_batch, to: *const lumen_page_batch, recent: usize, kept_dev: *mut i32, kept_stride: usize) -> c_int;
     pub fn lumen_gemv_repeat(ctx: *mut lumen_ctx, x_dev: *const f32, w_devs: *const *const c_void, n_w: usize, w_dtype: c_int, layout_kn: c_int, k: usize, n: usize, y_dev: *mut f32, iters: usize, us_per_call_out: *mut f32) -> c_int;
     pub fn lumen_attention_decode_repeat(ctx: *mut lumen_ctx, q_dev: *const f32, k_new_dev: *const f32, v_new_dev: *const f32, n_head: usize, caches: *const *mut lumen_kv_cache, n_caches: usize, rope: *mut lumen_rope, out_dev: *mut f32, iters: usize, us_per_call_out: *mut f32) -> c_int;
 }
