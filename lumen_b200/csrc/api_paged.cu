@@ -75,6 +75,15 @@ int lumen_page_pool_new(lumen_ctx *ctx, size_t pages, size_t page_size, size_t h
     p->k = mem;
     p->v = mem + bytes;
     p->mass = reinterpret_cast<float *>(mem + 2 * bytes);
+    if (dtype == LUMEN_BF16) {
+        const int rc = paged_tc_maps(ctx, p->g, p->k, p->v, &p->k_map, &p->v_map);
+        if (rc != LUMEN_OK) {
+            cudaStreamSynchronize(ctx->stream);
+            cudaFree(mem);
+            delete p;
+            return rc;
+        }
+    }
     *out = p;
     return LUMEN_OK;
 }
@@ -116,7 +125,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         std::vector<int> live;
         for (int s = 0; s < p.n_seq; ++s)
             if (p.seqs[(size_t)s].q_len) live.push_back(s);
-        paged_cut(p, b->g, paged_rows_shape(b->g, ctx->num_sms), live);
+        paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, ctx->num_sms) : paged_rows_shape(b->g, ctx->num_sms), live);
         // everything the kernels read goes up in one copy, in front of the workspace
         std::vector<char> up;
         auto put = [&](const void *data, size_t bytes) {
@@ -217,7 +226,8 @@ int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *b
     a.part = batch->part; a.part_rows = p.part_rows; a.joins = batch->joins; a.n_joins = (int)p.joins.size();
     for (const PagedJoin &j : p.joins) a.join_rows = std::max(a.join_rows, j.rows);
     const PagedView v = view_of(pool, batch);
-    LUMEN_TRY(launch_paged_rows(ctx, pool->g, v, a, ctx->stream));
+    LUMEN_TRY(pool->g.dtype == LUMEN_BF16 ? launch_paged_attn_tc(ctx, pool->g, v, pool->k_map, pool->v_map, a, ctx->stream)
+                                          : launch_paged_rows(ctx, pool->g, v, a, ctx->stream));
     return a.n_joins ? launch_paged_join(ctx, pool->g, v, a, ctx->stream) : LUMEN_OK;
 }
 

@@ -1,6 +1,8 @@
 // Handles and launchers of the paged key/value cache (api_paged.cu).
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 #include "paged_plan.cuh"
 
@@ -9,6 +11,7 @@ struct lumen_page_pool {
     lumen::PagedGeom g;
     void *k = nullptr, *v = nullptr;  // [pages, h_kv, page, d]
     float *mass = nullptr;            // [pages, h_kv, page]
+    CUtensorMap k_map, v_map;         // bf16: boxes of a page's positions x 64 numbers
 };
 
 struct lumen_page_batch {
@@ -63,6 +66,11 @@ struct PagedAttnArgs {
 };
 PagedShape paged_rows_shape(const PagedGeom &g, int num_sms);
 int launch_paged_rows(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
+// bf16 pools (paged_attn_tc.cu)
+PagedShape paged_tc_shape(int max_rows, int num_sms);
+int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *k, const void *v, CUtensorMap *k_map, CUtensorMap *v_map);
+int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a,
+                         cudaStream_t s);
 int launch_paged_join(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const void *q, float scale, const float *lse, int max_kv, cudaStream_t s);
 int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_keep, int *kept,

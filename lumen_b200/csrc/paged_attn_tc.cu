@@ -1,0 +1,403 @@
+// Attention over a paged cache of 16 bits on the 5th-generation tensor cores.
+//
+// o = sum_j 2^(s_j - m) v_j / l, s_j = scale * log2(e) * q . k_j.  A CTA takes an item: up to QT tiles of 128 rows of one key head (a row is one
+// new token and one of the query heads that read this key head, so the group shares every key and value) against a range of
+// positions, in tiles of 128:
+//   - warp 4 QT + 1 brings keys and values page by page (TMA boxes of one page x 64 numbers, 128-byte swizzle) into a ring;
+//   - one lane of warp 4 QT issues S = Q.K^T (both from shared memory) and O += P.V, with the weights P read from tensor memory and V as it
+//     lies in the cache (positions x numbers: the MN-major form of the second operand, no transposition);
+//   - the warpgroup of a tile, a thread a row, turns scores into weights where they are: scores come out of tensor memory, the weights go
+//     back over them as bf16.  O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since
+//     it last was (the weights are then at most 256, which neither bf16 nor the f32 sums mind).
+// Two tiles (QT 2) share a ring: while one's weights are computed, the other's products run.  One tile (QT 1) has two score
+// buffers instead.  Positions behind the end: scores are replaced, and the values' rows in shared memory are zeroed before
+// the product (weights of zero do not silence a NaN).  Long ranges are cut over the CTAs and joined by paged_join_kernel.
+//
+// Every wait is bounded; a wait that gives up records LUMEN_ERR_TIMEOUT, the roles run on without acting, copies and products in flight
+// are waited for, tensor memory is freed and the CTA returns.
+#include "paged.cuh"
+#include "tc_common.cuh"
+
+namespace lumen {
+namespace {
+
+using namespace tc;
+
+constexpr int kKeys = 128;      // positions per tile
+constexpr int kMma = 128;       // rows per tile
+constexpr float kLazy = 8.f;    // how far a maximum may grow before O is rescaled
+
+template <int D, int QT>
+struct TcGeom {
+    static constexpr int kBlocks = D / kBK;                     // 64-number blocks of a row
+    static constexpr uint32_t kTile = kKeys * kBK * 2;          // one block of 128 rows: 16 KB
+    static constexpr uint32_t kKBytes = kBlocks * kTile;        // keys (or values) of a tile
+    static constexpr int kStages = D == 128 ? (QT == 2 ? 2 : 3) : 4;
+    static constexpr int kBuffers = QT == 1 ? 2 : 1;            // of scores, per tile of rows
+    static constexpr size_t kSmem = (size_t)QT * kKBytes + (size_t)kStages * 2 * kKBytes + 1024;
+    static constexpr int kTmemCols = 512;                       // scores: kBuffers * QT * 128, then O: QT * D
+    static constexpr uint32_t kO = kBuffers * QT * kKeys;
+    static constexpr int kThreads = QT * 128 + 64;
+    static constexpr uint32_t kIdescS = idesc_bf16(kMma, kKeys);
+    static constexpr uint32_t kIdescO = idesc_bf16(kMma, D) | (1u << 16);  // second operand MN-major
+};
+
+// The second operand as it lies in the cache: rows of 64 numbers (128 bytes, swizzled), 8 positions every 1024 bytes, the next 64 numbers a tile further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next_block) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next_block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// First operand from tensor memory.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+          "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+          "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+          "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int D, int QT>
+__global__ void __launch_bounds__(TcGeom<D, QT>::kThreads, 1)
+paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedView p, const PagedAttnArgs a,
+                     DeviceStatus *status) {
+    using G = TcGeom<D, QT>;
+    constexpr int kStages = G::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    // the swizzle pattern repeats every 1024 bytes
+    unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char *ring = q_s + QT * G::kKBytes;  // stage: keys, values
+    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers], o_bar[QT][G::kBuffers], quiet;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int failed_s;
+    volatile int *failed = &failed_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const PagedItem it = a.items[blockIdx.x];
+    const PagedSeq sq = p.seqs[it.seq];
+    const int past = sq.kv_len - sq.q_len, nt = (it.key1 - it.key0 + kKeys - 1) / kKeys;
+    const int active = min(QT, (it.rows + kMma - 1) / kMma);  // tiles of rows in use
+    auto warps_of = [&](int q) { return min(4, (it.rows - q * kMma + 31) / 32); };  // of a tile, with rows
+
+    if (tid == 0) {
+        int loaders = 0;
+        for (int q = 0; q < active; ++q) {
+            loaders += 32 * warps_of(q);
+            for (int i = 0; i < G::kBuffers; ++i) {
+                bar_init(&s_bar[q][i], 1);
+                bar_init(&p_bar[q][i], (uint32_t)(32 * warps_of(q)));
+                bar_init(&o_bar[q][i], 1);
+            }
+        }
+        bar_init(&q_bar, (uint32_t)loaders);
+        for (int s = 0; s < kStages; ++s) {
+            bar_init(&k_full[s], 1);
+            bar_init(&v_full[s], 1);
+            bar_init(&k_free[s], 1);
+            bar_init(&v_free[s], 1);
+        }
+        bar_init(&quiet, 1);
+        failed_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == QT * 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_base_s)), "r"(G::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_base_s;
+    int k_issued = 0, v_issued = 0;  // tiles whose copies are on their way (producer warp)
+
+    if (warp == QT * 4 + 1) {
+        // ---- copies: the lanes of the warp take the boxes of a tile in turn (a box: up to one page, 64 numbers) ----
+        const int box = min(1 << p.page_shift, kKeys), per = kKeys / box;
+        const int *table = p.tables + sq.table;
+        // box b of tile j: positions from key0 + j * 128 + (b % per) * box, numbers from 64 * (b / per); where in the pool, or nothing
+        auto where = [&](int j, int b) {
+            const int pos = it.key0 + j * kKeys + b % per * box;
+            return b < per * G::kBlocks && pos < it.key1 ? table[pos >> p.page_shift] : -1;
+        };
+        constexpr int kMost = (G::kBlocks * (kKeys / 8) + 31) / 32;  // boxes of a lane, pages of eight
+        int page[kMost], next[kMost];
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) page[i] = where(0, lane + 32 * i);
+        auto load = [&](const CUtensorMap *map, unsigned char *dst, uint64_t *bar, int j) {
+            const int live = min(kKeys, it.key1 - it.key0 - j * kKeys), boxes = (live + box - 1) / box * G::kBlocks;
+            if (lane == 0) bar_expect(bar, (uint32_t)(boxes * box * kBK * 2));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kMost; ++i)
+                if (page[i] >= 0) {
+                    const int b = lane + 32 * i, c = b / per, r = b % per * box;
+                    tma_load_3d(dst + c * G::kTile + r * 128, map, c * kBK, (it.key0 + j * kKeys + r) & ((1 << p.page_shift) - 1), page[i] * p.h_kv + it.kvh, bar);
+                }
+        };
+#pragma unroll 1
+        for (int j = 0; j < nt; ++j) {
+            const int s = j % kStages;
+            const uint32_t par = (uint32_t)((j / kStages - 1) & 1);
+            unsigned char *st = ring + (size_t)s * 2 * G::kKBytes;
+#pragma unroll
+            for (int i = 0; i < kMost; ++i) next[i] = j + 1 < nt ? where(j + 1, lane + 32 * i) : -1;
+            bool ok = j < kStages || wait_or_failed(&k_free[s], par, failed, status, 740);
+            if (__all_sync(0xffffffffu, ok)) {
+                load(&map_k, st, &k_full[s], j);
+                ++k_issued;
+            }
+            ok = j < kStages || wait_or_failed(&v_free[s], par, failed, status, 741);
+            if (__all_sync(0xffffffffu, ok)) {
+                load(&map_v, st + G::kKBytes, &v_full[s], j);
+                ++v_issued;
+            }
+#pragma unroll
+            for (int i = 0; i < kMost; ++i) page[i] = next[i];
+        }
+    } else if (warp == QT * 4) {
+        if (lane == 0 && nt > 0) {
+            // ---- products ----
+            wait_or_failed(&q_bar, 0, failed, status, 700);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            auto scores = [&](int q, int j) {
+                const int s = j % kStages;
+                if (wait_or_failed(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
+                    const uint32_t qa = saddr(q_s + q * G::kKBytes), ka = saddr(ring + (size_t)s * 2 * G::kKBytes);
+                    const uint32_t acc = tmem + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys);
+#pragma unroll
+                    for (int kb = 0; kb < G::kBlocks; ++kb)
+#pragma unroll
+                        for (int kk = 0; kk < kBK / 16; ++kk)  // 16 numbers: 32 bytes, two units of the descriptor
+                            umma_bf16(acc, smem_desc(qa + kb * G::kTile) + 2 * kk, smem_desc(ka + kb * G::kTile) + 2 * kk, G::kIdescS, kb + kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
+            };
+            auto values = [&](int q, int j) {
+                const int s = j % kStages;
+                bool ok = wait_or_failed(&p_bar[q][j & (G::kBuffers - 1)], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
+                if (ok) ok = wait_or_failed(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (ok) {
+                    const uint64_t v = desc_mn(saddr(ring + (size_t)s * 2 * G::kKBytes + G::kKBytes), G::kTile);
+                    const uint32_t w = tmem + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys), acc = tmem + G::kO + (uint32_t)(q * D);
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 positions: 8 columns of weights, 2048 bytes of values
+                        umma_bf16_ts(acc, w + 8 * kk, v + (uint64_t)(kk * 2048 >> 4), G::kIdescO, j + kk > 0 ? 1u : 0u);
+                }
+            };
+            // Products run in the order in which they are issued: scores go over weights whose product stands before them.
+            for (int q = 0; q < active; ++q) scores(q, 0);
+            umma_commit(&k_free[0]);
+#pragma unroll 1
+            for (int j = 0; j < nt; ++j) {
+                if (QT == 1 && j + 1 < nt) {
+                    scores(0, j + 1);
+                    umma_commit(&k_free[(j + 1) % kStages]);
+                }
+                for (int q = 0; q < active; ++q) {
+                    values(q, j);
+                    if (QT == 1) umma_commit(&o_bar[0][j & (G::kBuffers - 1)]);
+                    else if (j + 1 < nt) scores(q, j + 1);
+                    else umma_commit(&o_bar[q][0]);
+                }
+                if (QT == 2 && j + 1 < nt) umma_commit(&k_free[(j + 1) % kStages]);
+                umma_commit(&v_free[j % kStages]);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- weights: a thread a row ----
+        const int q = warp >> 2, row = tid & 127, r = q * kMma + row;
+        if (q < active && (warp & 3) < warps_of(q)) {
+            const int row_t = it.row0 + min(r, it.rows - 1), t = row_t / p.group, head = it.kvh * p.group + row_t % p.group;
+            {  // the warp's 32 rows of queries into the swizzled layout of the tensor core: 16 bytes a thread, whole rows by neighbours
+                constexpr int kPer = D / 8;  // 16-byte pieces of a row
+#pragma unroll 4
+                for (int i = lane; i < 32 * kPer; i += 32) {
+                    const int rr = (warp & 3) * 32 + i / kPer, c = i % kPer, rg = q * kMma + rr;
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (rg < it.rows) {
+                        const int g = it.row0 + rg;
+                        x = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) +
+                                                             ((size_t)(sq.tok0 + g / p.group) * p.n_head + it.kvh * p.group + g % p.group) * D + c * 8);
+                    }
+                    *reinterpret_cast<uint4 *>(q_s + q * G::kKBytes + (c / 8) * G::kTile + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(&q_bar);
+            }
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t o_at = tmem + lanes + G::kO + (uint32_t)(q * D);
+            const float scale2 = a.scale * 1.4426950408889634f;
+            const int end = p.causal ? min(it.key1, past + t + 1) : it.key1;                                      // of what the row sees
+            const int end_min = p.causal ? min(it.key1, past + (it.row0 + q * kMma + (warp & 3) * 32) / p.group + 1) : it.key1;  // of the warp's first row
+            float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+            for (int j = 0; j < nt; ++j) {
+                const int buffer = j & (G::kBuffers - 1), tile0 = it.key0 + j * kKeys;
+                const uint32_t s_at = tmem + lanes + (uint32_t)((q * G::kBuffers + buffer) * kKeys);
+                wait_or_failed(&s_bar[q][buffer], (uint32_t)((j / G::kBuffers) & 1), failed, status, 730);
+                __syncwarp();
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t s[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32_issue(s_at + 32 * i, s[i]);
+                tmem_ld_wait();
+                if (tile0 + kKeys > end_min) {
+                    const int lim = end - tile0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            // -infinity after the scale, whatever its sign
+                            s[i][c] = 32 * i + c < lim ? __float_as_uint(__uint_as_float(s[i][c]) * scale2) : 0xff800000u;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) s[i][c] = __float_as_uint(__uint_as_float(s[i][c]) * scale2);
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(s[i][c]));
+                // O is multiplied by 2^(m - new maximum) where that is needed (a warp at a time); the first tile overwrites O
+                const bool grow = top > m + kLazy || m == -INFINITY;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float next = grow ? fmaxf(m, top) : m, f = next == -INFINITY ? 1.f : ex2(m - next);
+                    m = next;
+                    l *= f;
+                    if (j > 0) {
+                        if (QT == 1) {  // the product before this tile's
+                            wait_or_failed(&o_bar[q][(j - 1) & (G::kBuffers - 1)], (uint32_t)(((j - 1) / G::kBuffers) & 1), failed, status, 731);
+                            __syncwarp();
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            uint32_t o[32];
+                            tmem_ld32(o_at + 32 * i, o);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+                            tmem_st32(o_at + 32 * i, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const float x = ex2(__uint_as_float(s[2 * h + c / 16][2 * (c % 16)]) - base), y = ex2(__uint_as_float(s[2 * h + c / 16][2 * (c % 16) + 1]) - base);
+                        sum[c & 3] += x + y;
+                        w[c] = pack_bf16(x, y);
+                    }
+                    tmem_st32(s_at + 32 * h, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (q == 0 && tile0 + kKeys > it.key1) {
+                    // the last tile ends behind the positions: zeros instead of the values there (both tiles of rows multiply this one later)
+                    const int s_i = j % kStages, dead = kKeys - (it.key1 - tile0), all = 32 * warps_of(0);
+                    wait_or_failed(&v_full[s_i], (uint32_t)((j / kStages) & 1), failed, status, 732);
+                    unsigned char *v = ring + (size_t)s_i * 2 * G::kKBytes + G::kKBytes;
+                    for (int i = tid; i < dead * (D / 8); i += all) {
+                        const int pos = kKeys - dead + i / (D / 8), c = i % (D / 8);
+                        *reinterpret_cast<uint4 *>(v + (c / 8) * G::kTile + pos * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                tmem_st_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                bar_arrive(&p_bar[q][buffer]);
+            }
+            // ---- results ----
+            if (nt > 0) {
+                // (one tile: a barrier for every other product; two: one arrival at the end)
+                if (QT == 1) wait_or_failed(&o_bar[q][(nt - 1) & (G::kBuffers - 1)], (uint32_t)(((nt - 1) / G::kBuffers) & 1), failed, status, 733);
+                else wait_or_failed(&o_bar[q][0], 0, failed, status, 733);
+                __syncwarp();
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            const bool live = r < it.rows && !*failed, part = it.part >= 0;
+            const float inv = part ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+            const size_t o_row = part ? (size_t)it.part + r : (size_t)(sq.tok0 + t) * p.n_head + head;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) o[c] = 0u;
+                if (nt > 0) tmem_ld32(o_at + 32 * i, o);
+                if (!live) continue;
+                if (part || a.out_dtype == LUMEN_F32) {
+                    float *dst = (part ? a.part : static_cast<float *>(a.out)) + o_row * D + 32 * i;
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4)
+                        *reinterpret_cast<float4 *>(dst + c) = make_float4(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv,
+                                                                           __uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
+                } else {
+                    __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + o_row * D + 32 * i;
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8)
+                        *reinterpret_cast<uint4 *>(dst + c) = make_uint4(
+                            pack_bf16(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv), pack_bf16(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv),
+                            pack_bf16(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv), pack_bf16(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv));
+                }
+            }
+            if (live) {
+                if (part) *reinterpret_cast<float2 *>(a.part + (size_t)a.part_rows * D + 2 * o_row) = make_float2(m, l);
+                else if (a.lse) a.lse[o_row] = m * 0.6931471805599453f + logf(l);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        }
+    }
+    __syncthreads();
+    if (*failed) {
+        if (tid == QT * 128 + 32) {  // a wait gave up
+            drain_ring(k_full, kStages, k_issued);
+            drain_ring(v_full, kStages, v_issued);
+        } else if (tid == QT * 128) {
+            drain_mmas(&quiet);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == QT * 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kTmemCols) : "memory");
+}
+
+template <int D, int QT>
+int launch(lumen_ctx *ctx, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a, cudaStream_t s) {
+    using G = TcGeom<D, QT>;
+    static_assert(G::kSmem <= 227 * 1024 - 512 && G::kO + QT * D <= (uint32_t)G::kTmemCols, "fits shared and tensor memory");
+    LUMEN_TRY(allow_smem(ctx, paged_attn_tc_kernel<D, QT>, G::kSmem));
+    paged_attn_tc_kernel<D, QT><<<(unsigned)a.n_items, G::kThreads, G::kSmem, s>>>(k_map, v_map, v, a, ctx->d_status);
+    LUMEN_LAUNCHED(ctx);
+    return LUMEN_OK;
+}
+
+}  // namespace
+
+PagedShape paged_tc_shape(int max_rows, int num_sms) { return {max_rows > kMma ? 2 * kMma : kMma, kKeys, num_sms}; }
+
+int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *k, const void *v, CUtensorMap *k_map, CUtensorMap *v_map) {
+    const size_t slabs = (size_t)g.pages * g.h_kv, page = (size_t)g.page, d = (size_t)g.d;
+    const int box = std::min(g.page, kKeys);
+    LUMEN_TRY(make_map_3d(ctx, k_map, k, d, page, d, slabs, page * d, box, 1));
+    return make_map_3d(ctx, v_map, v, d, page, d, slabs, page * d, box, 1);
+}
+
+int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a,
+                         cudaStream_t s) {
+    if (g.d == 64) return a.max_rows > kMma ? launch<64, 2>(ctx, v, k_map, v_map, a, s) : launch<64, 1>(ctx, v, k_map, v_map, a, s);
+    return a.max_rows > kMma ? launch<128, 2>(ctx, v, k_map, v_map, a, s) : launch<128, 1>(ctx, v, k_map, v_map, a, s);
+}
+
+}  // namespace lumen
