@@ -241,7 +241,14 @@ int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *ba
     if (p.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: two sequences share a page");
     if (p.tokens == 0 || p.max_kv == 0) return LUMEN_OK;
     OnDevice on(ctx);
-    return launch_paged_mass(ctx, pool->g, view_of(pool, batch), q_dev, scale, lse_dev, p.max_kv, ctx->stream);
+    PagedMassArgs a = {q_dev, scale, lse_dev, 0, INT32_MAX, 0};
+    for (const PagedSeq &q : p.seqs)
+        if (q.q_len && q.kv_len) {
+            a.max_kv = std::max(a.max_kv, q.kv_len);
+            a.min_rows = std::min(a.min_rows, q.q_len * p.group);
+            a.max_rows = std::max(a.max_rows, q.q_len * p.group);
+        }
+    return a.max_rows ? launch_paged_mass(ctx, pool->g, view_of(pool, batch), pool->k_map, a, ctx->stream) : (int)LUMEN_OK;
 }
 
 int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const lumen_page_batch *to, size_t recent, int32_t *kept_dev,

@@ -72,7 +72,13 @@ int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *k, const void 
 int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a,
                          cudaStream_t s);
 int launch_paged_join(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
-int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const void *q, float scale, const float *lse, int max_kv, cudaStream_t s);
+struct PagedMassArgs {
+    const void *q;
+    float scale;
+    const float *lse;
+    int max_kv, min_rows, max_rows;  // of the sequences with new tokens: positions, rows of a key head
+};
+int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s);
 int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_keep, int *kept,
                        size_t kept_stride, cudaStream_t s);
 

@@ -1,26 +1,280 @@
-// What the cached positions were looked at: mass[j] += sum over the rows that see j of exp(scale * q . k_j - lse).
+// What the cached positions were looked at: mass[j] += sum over the rows that see j of exp(scale * q . k_j - lse).  (A row is one new token and one
+// of the query heads that read the key head.)
 //
-// Every position belongs to one thread, which walks the rows in their order: nothing is exchanged, no atomics, the same sum every time.
+// Every position belongs to one thread or one group of lanes, which walks the rows in their order: no atomics, the same sum every time.
+//   few rows, 16 bits: paged_mass_few_kernel, bound by reading the keys once
+//   many rows, 16 bits: paged_mass_tc_kernel, scores on the 5th-generation tensor cores, bound by the exponentials (16 a cycle and SM)
+//   32 bits: paged_mass_kernel, FMA pipe
 #include "paged.cuh"
+#include "mma_common.cuh"
+#include "tc_common.cuh"
 
 namespace lumen {
 namespace {
 
+using namespace tc;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+constexpr int kFewThreads = 128, kFewKeys = 256;  // of a CTA: a warp takes 4 groups of 16 positions
+
+// Scores of 16 positions x 8 rows from m16n8k16 products.  The sum over the numbers of a head may run in any order, so lane (g, t) loads pieces of
+// 16 bytes of the keys g and g + 8 straight into the operand's registers - no shared memory on the way - and the queries are put in
+// shared memory in the order that this gives: the i-th pair of products uses numbers 32 i + 8 t .. 32 i + 8 t + 7.
+// grid (blocks of 256 positions of the longest sequence, key heads, sequences)
+template <int D>
+__global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const PagedView p, const __nv_bfloat16 *__restrict__ q, float scale, const float *__restrict__ lse) {
+    constexpr int kPieces = D / 32;  // of 16 bytes, per lane and key
+    extern __shared__ uint4 q_s[];   // [blocks of 8 rows][kPieces][32 lanes]: row g of the block, numbers 32 i + 8 t ..
+    __shared__ float l_s[kFewRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
+    const PagedSeq sq = p.seqs[blockIdx.z];
+    const int rows = sq.q_len * p.group, key0 = blockIdx.x * kFewKeys, past = sq.kv_len - sq.q_len;
+    if (key0 >= sq.kv_len || rows == 0 || rows > kFewRows) return;
+    const int *table = p.tables + sq.table;
+    const int blocks = (rows + 7) / 8;
+    const float scale2 = scale * kLog2e;
+    for (int i = tid; i < blocks * kPieces * 32; i += kFewThreads) {
+        const int ln = i & 31, pc = i / 32 % kPieces, row = i / (32 * kPieces) * 8 + (ln >> 2);
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows)
+            x = *reinterpret_cast<const uint4 *>(q + ((size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group) * D + 32 * pc + 8 * (ln & 3));
+        q_s[i] = x;
+    }
+    if (tid < kFewRows) l_s[tid] = tid < rows ? lse[(size_t)(sq.tok0 + tid / p.group) * p.n_head + kvh * p.group + tid % p.group] * kLog2e : 0.f;
+    constexpr int kGroups = 2;  // of 16 positions at once
+    const uint4 *keys = static_cast<const uint4 *>(p.k);
+#pragma unroll 1
+    for (int round = 0; round < kFewKeys / (kFewThreads / 32 * 16 * kGroups); ++round) {
+        uint4 k[kGroups][2][kPieces];
+        size_t at[kGroups][2];
+        const int base = key0 + (round * (kFewThreads / 32) + warp) * 16 * kGroups;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) at[i][h] = paged_row(p, table, kvh, min(base + 16 * i + 8 * h + g, sq.kv_len - 1));
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < kPieces; ++c) k[i][h][c] = __ldcs(keys + at[i][h] * (D / 8) + 4 * c + t);
+        if (round == 0) __syncthreads();  // the queries are there
+        if (base >= sq.kv_len) continue;
+        float sum[kGroups][2] = {};
+        for (int b = 0; b < blocks; ++b) {
+            float s[kGroups][4] = {};
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c) {
+                const uint4 x = q_s[(b * kPieces + c) * 32 + lane];
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    const uint32_t a0[4] = {k[i][0][c].x, k[i][1][c].x, k[i][0][c].y, k[i][1][c].y}, a1[4] = {k[i][0][c].z, k[i][1][c].z, k[i][0][c].w, k[i][1][c].w};
+                    mma16816(s[i], a0, x.x, x.y);
+                    mma16816(s[i], a1, x.z, x.w);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * b + 2 * t + e;
+                const float l = l_s[row];
+                const int last = row >= rows ? -1 : p.causal ? past + row / p.group : sq.kv_len - 1;
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    sum[i][0] += base + 16 * i + g <= last ? ex2(fmaf(s[i][e], scale2, -l)) : 0.f;
+                    sum[i][1] += base + 16 * i + 8 + g <= last ? ex2(fmaf(s[i][2 + e], scale2, -l)) : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sum[i][h] += __shfl_xor_sync(0xffffffffu, sum[i][h], 1);
+                sum[i][h] += __shfl_xor_sync(0xffffffffu, sum[i][h], 2);
+                if (t == 0 && base + 16 * i + 8 * h + g < sq.kv_len) p.mass[at[i][h]] += sum[i][h];
+            }
+    }
+}
+
+// ---- many rows --------------------------------------------------------------------------------------------------------
+constexpr int kTcKeys = 256, kTcRows = 128, kTcLoaders = 96, kTcStages = 3, kTcThreads = 256 + 32 + kTcLoaders;
+
+template <int D>
+struct MassGeom {
+    static constexpr int kBlocks = D / kBK;
+    static constexpr uint32_t kTile = 128 * kBK * 2;
+    static constexpr uint32_t kOperand = kBlocks * kTile;  // 128 keys or 128 rows
+    static constexpr size_t kSmem = (2 + kTcStages) * (size_t)kOperand + 1024;
+};
+
+// A CTA owns 256 positions of a key head (their keys stay in shared memory) and walks the rows that see any of them, 128 at a time: scores
+// transposed, S^T = K.Q^T, so that a thread holds one position and sums over the columns.  Warps 0-7: exponentials and sums (a
+// warpgroup per 128 positions, two score buffers each); warp 8: products; warps 9-11: queries and log-sums into a ring.
+// grid (blocks of 256 positions of the longest sequence, key heads, sequences)
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView p, const __nv_bfloat16 *__restrict__ q, float scale, const float *__restrict__ lse,
+                     DeviceStatus *status) {
+    using G = MassGeom<D>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *k_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *ring = k_s + 2 * G::kOperand;
+    __shared__ uint64_t k_bar, q_full[kTcStages], q_free[kTcStages], s_full[2][2], s_free[2][2], quiet;
+    __shared__ __align__(16) float l_s[kTcStages][kTcRows];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int failed_s;
+    volatile int *failed = &failed_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
+    const PagedSeq sq = p.seqs[blockIdx.z];
+    const int rows = sq.q_len * p.group, key0 = blockIdx.x * kTcKeys, past = sq.kv_len - sq.q_len;
+    if (key0 >= sq.kv_len || rows <= kFewRows) return;
+    const int start = p.causal ? max(0, key0 - past) * p.group : 0, steps = (rows - start + kTcRows - 1) / kTcRows;  // (start < rows: key0 < kv_len)
+    const int tiles = min(2, (sq.kv_len - key0 + 127) / 128);  // of 128 positions
+    if (tid == 0) {
+        bar_init(&k_bar, 1);
+        for (int s = 0; s < kTcStages; ++s) {
+            bar_init(&q_full[s], kTcLoaders);
+            bar_init(&q_free[s], 1 + 32 * 4 * (uint32_t)tiles);
+        }
+        for (int i = 0; i < 4; ++i) {
+            bar_init(&s_full[i >> 1][i & 1], 1);
+            bar_init(&s_free[i >> 1][i & 1], 128);
+        }
+        bar_init(&quiet, 1);
+        failed_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_base_s)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_base_s;  // scores: tile 0 even, odd steps, tile 1 even, odd steps
+
+    if (warp >= 9) {
+        const int id = tid - 288;
+        if (warp == 9) {  // the keys, page by page
+            const int box = min(1 << p.page_shift, 128), live = min(kTcKeys, sq.kv_len - key0), boxes = (live + box - 1) / box * G::kBlocks;
+            const int *table = p.tables + sq.table;
+            if (lane == 0) bar_expect(&k_bar, (uint32_t)(boxes * box * kBK * 2));
+            __syncwarp();
+            for (int b = lane; b < boxes; b += 32) {
+                const int c = b % G::kBlocks, r = b / G::kBlocks * box, pos = key0 + r;
+                tma_load_3d(k_s + (r / 128) * G::kOperand + c * G::kTile + r % 128 * 128, &map_k, c * kBK, pos & ((1 << p.page_shift) - 1),
+                            table[pos >> p.page_shift] * p.h_kv + kvh, &k_bar);
+            }
+        }
+        constexpr int kPer = D / 8;  // 16-byte pieces of a row
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+            const int s = i % kTcStages, r0 = start + i * kTcRows;
+            if (i >= kTcStages) wait_or_failed(&q_free[s], (uint32_t)((i / kTcStages - 1) & 1), failed, status, 760);
+            unsigned char *dst = ring + (size_t)s * G::kOperand;
+#pragma unroll 8
+            for (int x = id; x < kTcRows * kPer; x += kTcLoaders) {
+                const int r = x / kPer, c = x % kPer, row = r0 + r, tok = row / p.group;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (row < rows) v = *reinterpret_cast<const uint4 *>(q + ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + row - tok * p.group) * D + 8 * c);
+                *reinterpret_cast<uint4 *>(dst + (c / 8) * G::kTile + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+            }
+            for (int r = id; r < kTcRows; r += kTcLoaders) {
+                const int row = r0 + r;
+                l_s[s][r] = row < rows ? lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] * kLog2e : 0.f;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(&q_full[s]);
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            wait_or_failed(&k_bar, 0, failed, status, 761);
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                const int s = i % kTcStages, b = i & 1;
+                const bool ok = wait_or_failed(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 762);
+                for (int kt = 0; kt < tiles; ++kt) {
+                    const bool free = i < 2 || wait_or_failed(&s_free[kt][b], (uint32_t)((i / 2 - 1) & 1), failed, status, 763);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (ok && free) {
+                        const uint32_t ka = saddr(k_s + kt * G::kOperand), qa = saddr(ring + (size_t)s * G::kOperand);
+#pragma unroll
+                        for (int kb = 0; kb < G::kBlocks; ++kb)
+#pragma unroll
+                            for (int kk = 0; kk < kBK / 16; ++kk)
+                                umma_bf16(tmem + (uint32_t)(kt * 256 + b * 128), smem_desc(ka + kb * G::kTile) + 2 * kk, smem_desc(qa + kb * G::kTile) + 2 * kk, idesc_bf16(128, 128),
+                                          kb + kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[kt][b]);
+                }
+                umma_commit(&q_free[s]);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int kt = warp >> 2, key = key0 + 128 * kt + (tid & 127);
+        if (kt < tiles) {
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const float scale2 = scale * kLog2e;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const int first = p.causal ? (key - past) * p.group : 0;  // the first row that sees the position
+            const int key_max = key0 + 128 * kt + (warp & 3) * 32 + 31;
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                const int s = i % kTcStages, b = i & 1, r0 = start + i * kTcRows;
+                wait_or_failed(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 764);  // the log-sums
+                wait_or_failed(&s_full[kt][b], (uint32_t)((i / 2) & 1), failed, status, 765);
+                __syncwarp();
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32_issue(tmem + lanes + (uint32_t)(kt * 256 + b * 128 + 32 * c), x[c]);
+                tmem_ld_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                bar_arrive(&s_free[kt][b]);
+                const bool masked = r0 + kTcRows > rows || (p.causal && past + r0 / p.group < key_max);
+                const int lo = first - r0, hi = rows - r0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 l4 = *reinterpret_cast<const float4 *>(&l_s[s][32 * c + e]);
+                        const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int col = 32 * c + e + u;
+                            const float w = ex2(fmaf(__uint_as_float(x[c][e + u]), scale2, -l[u]));
+                            sum[u] += !masked || (col >= lo && col < hi) ? w : 0.f;
+                        }
+                    }
+                bar_arrive(&q_free[s]);
+            }
+            if (key < sq.kv_len && !*failed) p.mass[paged_row(p, p.tables + sq.table, kvh, key)] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+    }
+    __syncthreads();
+    if (*failed) {
+        if (tid == 288) drain_ring(&k_bar, 1, 1);  // a wait gave up
+        else if (tid == 256) drain_mmas(&quiet);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---- 32 bits --------------------------------------------------------------------------------------------------------------
 constexpr int kKeys = 64, kRows = 16, kThreads = 128;
 
 __device__ __forceinline__ void four(const float *p, float (&v)[4]) {
     const float4 x = *reinterpret_cast<const float4 *>(p);
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
 }
-__device__ __forceinline__ void four(const __nv_bfloat16 *p, float (&v)[4]) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(p);
-    v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
-    v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
-}
 
 // grid (tiles of the longest sequence, key heads, sequences)
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) paged_mass_kernel(const PagedView p, const T *__restrict__ q, float scale, const float *__restrict__ lse) {
+template <int D>
+__global__ void __launch_bounds__(kThreads) paged_mass_kernel(const PagedView p, const float *__restrict__ q, float scale, const float *__restrict__ lse) {
     __shared__ __align__(16) float k_s[kKeys][D + 4];
     __shared__ __align__(16) float q_s[kRows][D];
     __shared__ float l_s[kRows], half_s[kKeys];
@@ -32,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) paged_mass_kernel(const PagedView p,
     for (int i = tid; i < kKeys * (D / 4); i += kThreads) {
         const int r = i / (D / 4), e = i % (D / 4) * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (key0 + r < sq.kv_len) four(static_cast<const T *>(p.k) + paged_row(p, table, kvh, key0 + r) * D + e, v);
+        if (key0 + r < sq.kv_len) four(static_cast<const float *>(p.k) + paged_row(p, table, kvh, key0 + r) * D + e, v);
         *reinterpret_cast<float4 *>(&k_s[r][e]) = make_float4(v[0], v[1], v[2], v[3]);
     }
     const int key = tid % kKeys, half = tid / kKeys, rows = sq.q_len * p.group;
@@ -72,24 +326,38 @@ __global__ void __launch_bounds__(kThreads) paged_mass_kernel(const PagedView p,
     if (!half && key0 + key < sq.kv_len) p.mass[paged_row(p, table, kvh, key0 + key)] += gained + half_s[key];
 }
 
-template <typename T, int D>
-int launch(lumen_ctx *ctx, const PagedView &v, const void *q, float scale, const float *lse, int max_kv, cudaStream_t s) {
-    // (sequences beyond the grid's third extent go in further launches)
-    for (int s0 = 0; s0 < v.n_seq; s0 += 32768) {
-        PagedView w = v;
-        w.seqs += s0;
-        const dim3 grid((unsigned)((max_kv + kKeys - 1) / kKeys), (unsigned)v.h_kv, (unsigned)std::min(v.n_seq - s0, 32768));
-        paged_mass_kernel<T, D><<<grid, kThreads, 0, s>>>(w, static_cast<const T *>(q), scale, lse);
-        LUMEN_LAUNCHED(ctx);
+dim3 grid_of(const PagedMassArgs &a, const PagedView &v, int keys, int n) { return dim3((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)v.h_kv, (unsigned)n); }
+
+template <int D>
+int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
+    for (int s0 = 0; s0 < all.n_seq; s0 += 32768) {  // (the grid's third extent)
+        const int n = std::min(all.n_seq - s0, 32768);
+        PagedView v = all;
+        v.seqs += s0;
+        if (g.dtype == LUMEN_F32) {
+            paged_mass_kernel<D><<<grid_of(a, v, kKeys, n), kThreads, 0, s>>>(v, static_cast<const float *>(a.q), a.scale, a.lse);
+            LUMEN_LAUNCHED(ctx);
+            continue;
+        }
+        const auto *q = static_cast<const __nv_bfloat16 *>(a.q);
+        if (a.min_rows <= kFewRows) {
+            const size_t bytes = (size_t)(std::min(kFewRows, a.max_rows) + 7) / 8 * 8 * D * 2;
+            paged_mass_few_kernel<D><<<grid_of(a, v, kFewKeys, n), kFewThreads, bytes, s>>>(v, q, a.scale, a.lse);
+            LUMEN_LAUNCHED(ctx);
+        }
+        if (a.max_rows > kFewRows) {
+            LUMEN_TRY(allow_smem(ctx, paged_mass_tc_kernel<D>, MassGeom<D>::kSmem));
+            paged_mass_tc_kernel<D><<<grid_of(a, v, kTcKeys, n), kTcThreads, MassGeom<D>::kSmem, s>>>(k_map, v, q, a.scale, a.lse, ctx->d_status);
+            LUMEN_LAUNCHED(ctx);
+        }
     }
     return LUMEN_OK;
 }
 
 }  // namespace
 
-int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const void *q, float scale, const float *lse, int max_kv, cudaStream_t s) {
-    if (g.dtype == LUMEN_F32) return g.d == 64 ? launch<float, 64>(ctx, v, q, scale, lse, max_kv, s) : launch<float, 128>(ctx, v, q, scale, lse, max_kv, s);
-    return g.d == 64 ? launch<__nv_bfloat16, 64>(ctx, v, q, scale, lse, max_kv, s) : launch<__nv_bfloat16, 128>(ctx, v, q, scale, lse, max_kv, s);
+int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
+    return g.d == 64 ? launch<64>(ctx, g, v, k_map, a, s) : launch<128>(ctx, g, v, k_map, a, s);
 }
 
 }  // namespace lumen
