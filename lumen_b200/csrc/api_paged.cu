@@ -76,7 +76,11 @@ int lumen_page_pool_new(lumen_ctx *ctx, size_t pages, size_t page_size, size_t h
     p->v = mem + bytes;
     p->mass = reinterpret_cast<float *>(mem + 2 * bytes);
     if (dtype == LUMEN_BF16) {
-        const int rc = paged_tc_maps(ctx, p->g, p->k, p->v, &p->k_map, &p->v_map);
+        int rc = LUMEN_OK;
+        for (int i = 0; i < 2 && rc == LUMEN_OK; ++i) {
+            rc = paged_tc_maps(ctx, p->g, p->k, 64 << i, &p->k_map[i]);
+            if (rc == LUMEN_OK) rc = paged_tc_maps(ctx, p->g, p->v, 64 << i, &p->v_map[i]);
+        }
         if (rc != LUMEN_OK) {
             cudaStreamSynchronize(ctx->stream);
             cudaFree(mem);
@@ -248,7 +252,7 @@ int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *ba
             a.min_rows = std::min(a.min_rows, q.q_len * p.group);
             a.max_rows = std::max(a.max_rows, q.q_len * p.group);
         }
-    return a.max_rows ? launch_paged_mass(ctx, pool->g, view_of(pool, batch), pool->k_map, a, ctx->stream) : (int)LUMEN_OK;
+    return a.max_rows ? launch_paged_mass(ctx, pool->g, view_of(pool, batch), pool->k_map[1], a, ctx->stream) : (int)LUMEN_OK;
 }
 
 int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const lumen_page_batch *to, size_t recent, int32_t *kept_dev,

@@ -11,7 +11,7 @@ struct lumen_page_pool {
     lumen::PagedGeom g;
     void *k = nullptr, *v = nullptr;  // [pages, h_kv, page, d]
     float *mass = nullptr;            // [pages, h_kv, page]
-    CUtensorMap k_map, v_map;         // bf16: boxes of a page's positions x 64 numbers
+    CUtensorMap k_map[2], v_map[2];   // bf16: boxes of up to 64 and up to 128 positions of a page x 64 numbers
 };
 
 struct lumen_page_batch {
@@ -68,8 +68,8 @@ PagedShape paged_rows_shape(const PagedGeom &g, int num_sms);
 int launch_paged_rows(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
 // bf16 pools (paged_attn_tc.cu)
 PagedShape paged_tc_shape(int max_rows, int num_sms);
-int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *k, const void *v, CUtensorMap *k_map, CUtensorMap *v_map);
-int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a,
+int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *mem, int most, CUtensorMap *map);
+int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap (&k_map)[2], const CUtensorMap (&v_map)[2], const PagedAttnArgs &a,
                          cudaStream_t s);
 int launch_paged_join(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
 struct PagedMassArgs {

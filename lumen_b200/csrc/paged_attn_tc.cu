@@ -2,19 +2,24 @@
 //
 // o = sum_j 2^(s_j - m) v_j / l, s_j = scale * log2(e) * q . k_j.  A CTA takes an item: up to QT tiles of 128 rows of one key head (a row is one
 // new token and one of the query heads that read this key head, so the group shares every key and value) against a range of
-// positions, in tiles of 128:
-//   - warp 4 QT + 1 brings keys and values page by page (TMA boxes of one page x 64 numbers, 128-byte swizzle) into a ring;
-//   - one lane of warp 4 QT issues S = Q.K^T (both from shared memory) and O += P.V, with the weights P read from tensor memory and V as it
+// positions, in tiles of KT:
+//   - one warp brings keys and values page by page (TMA boxes of one page x 64 numbers, 128-byte swizzle) into a ring;
+//   - one lane of another issues S = Q.K^T (both from shared memory) and O += P.V, with the weights P read from tensor memory and V as it
 //     lies in the cache (positions x numbers: the MN-major form of the second operand, no transposition);
 //   - the warpgroup of a tile, a thread a row, turns scores into weights where they are: scores come out of tensor memory, the weights go
 //     back over them as bf16.  O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since
 //     it last was (the weights are then at most 256, which neither bf16 nor the f32 sums mind).
-// Two tiles (QT 2) share a ring: while one's weights are computed, the other's products run.  One tile (QT 1) has two score
-// buffers instead.  Positions behind the end: scores are replaced, and the values' rows in shared memory are zeroed before
-// the product (weights of zero do not silence a NaN).  Long ranges are cut over the CTAs and joined by paged_join_kernel.
+// Many rows (QT 2, tiles of 128 positions): two tiles of rows share a ring; while one's weights are computed, the other's products run.  The
+// exponentials (16 a cycle and SM) would take as long as the products, so a part of them is computed on the FMA pipe.
+// Up to 128 rows (QT 1, tiles of 64 positions, two score buffers): bound by reading the cache; two CTAs share an SM, so that one streams while the
+// other starts or ends.
+// Positions behind the end: scores are replaced, and the values' rows in shared memory are zeroed before the product
+// (weights of zero do not silence a NaN).  Long ranges are cut over the CTAs and joined by paged_join_kernel.
 //
 // Every wait is bounded; a wait that gives up records LUMEN_ERR_TIMEOUT, the roles run on without acting, copies and products in flight
 // are waited for, tensor memory is freed and the CTA returns.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "tc_common.cuh"
 
@@ -23,21 +28,27 @@ namespace {
 
 using namespace tc;
 
-constexpr int kKeys = 128;      // positions per tile
 constexpr int kMma = 128;       // rows per tile
 constexpr float kLazy = 8.f;    // how far a maximum may grow before O is rescaled
+constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int QT>
 struct TcGeom {
+    static constexpr int kKeys = QT == 2 ? 128 : 64;            // positions per tile
     static constexpr int kBlocks = D / kBK;                     // 64-number blocks of a row
-    static constexpr uint32_t kTile = kKeys * kBK * 2;          // one block of 128 rows: 16 KB
-    static constexpr uint32_t kKBytes = kBlocks * kTile;        // keys (or values) of a tile
-    static constexpr int kStages = D == 128 ? (QT == 2 ? 2 : 3) : 4;
+    static constexpr uint32_t kQTile = kMma * kBK * 2;          // one block of 128 rows of queries
+    static constexpr uint32_t kQBytes = kBlocks * kQTile;
+    static constexpr uint32_t kTile = kKeys * kBK * 2;          // one block of a tile of keys or values
+    static constexpr uint32_t kKBytes = kBlocks * kTile;
+    static constexpr int kStages = D == 128 ? 2 : 4;
     static constexpr int kBuffers = QT == 1 ? 2 : 1;            // of scores, per tile of rows
-    static constexpr size_t kSmem = (size_t)QT * kKBytes + (size_t)kStages * 2 * kKBytes + 1024;
-    static constexpr int kTmemCols = 512;                       // scores: kBuffers * QT * 128, then O: QT * D
+    static constexpr int kHalves = QT;                          // the weights of a tile are handed over in so many parts
+    static constexpr size_t kSmem = (size_t)QT * kQBytes + (size_t)kStages * 2 * kKBytes + 1024;
+    static constexpr int kTmemCols = QT == 2 ? 512 : 256;       // scores: kBuffers * QT * kKeys, then O: QT * D
     static constexpr uint32_t kO = kBuffers * QT * kKeys;
-    static constexpr int kThreads = QT * 128 + 64;
+    // Two tiles: three warpgroups, so that the two with the weights can take registers from the one without (168 a thread at launch; 2 x 224 + 56 = 3 x 168)
+    static constexpr int kThreads = QT == 2 ? 384 : 192;
+    static constexpr int kRegsMore = 224, kRegsLess = 56;
     static constexpr uint32_t kIdescS = idesc_bf16(kMma, kKeys);
     static constexpr uint32_t kIdescO = idesc_bf16(kMma, D) | (1u << 16);  // second operand MN-major
 };
@@ -62,19 +73,69 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
           "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr) : "memory");
+    tmem_ld_wait();
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void apart(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two numbers of at most 2^7 on the FMA pipe: x = n + f with n the nearest whole number (1.5 * 2^23 added and taken off again), 2^f on
+// [-0.5, 0.5] by the polynomial of degree 5 with the least largest relative error (7.5e-8; found by Remez exchange), n added to the
+// exponent.  Below -126 it gives about 2^-126 instead of less.
+__device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
+    float x, y;
+    apart(x2, x, y);
+    x2 = two(fmaxf(x, -126.f), fmaxf(y, -126.f));
+    const uint64_t magic = two(12582912.f, 12582912.f), t = add2(x2, magic);
+    const uint64_t n = add2(t, two(-12582912.f, -12582912.f)), f = fma2(n, two(-1.f, -1.f), x2);
+    uint64_t r = fma2(f, two(0.0013276472454890609f, 0.0013276472454890609f), two(0.009675540961325169f, 0.009675540961325169f));
+    r = fma2(r, f, two(0.05550713092088699f, 0.05550713092088699f));
+    r = fma2(r, f, two(0.24022120237350464f, 0.24022120237350464f));
+    r = fma2(r, f, two(0.6931469440460205f, 0.6931469440460205f));
+    r = fma2(r, f, two(1.0000001192092896f, 1.0000001192092896f));
+    float ra, rb, ta, tb;
+    apart(r, ra, rb);
+    apart(t, ta, tb);
+    a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
+    b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int D, int QT>
-__global__ void __launch_bounds__(TcGeom<D, QT>::kThreads, 1)
+__global__ void __launch_bounds__(TcGeom<D, QT>::kThreads, 3 - QT)
 paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedView p, const PagedAttnArgs a,
                      DeviceStatus *status) {
     using G = TcGeom<D, QT>;
-    constexpr int kStages = G::kStages;
+    constexpr int kStages = G::kStages, kKeys = G::kKeys;
     extern __shared__ unsigned char smem_raw[];
     // the swizzle pattern repeats every 1024 bytes
     unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *ring = q_s + QT * G::kKBytes;  // stage: keys, values
-    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers], o_bar[QT][G::kBuffers], quiet;
+    unsigned char *ring = q_s + QT * G::kQBytes;  // stage: keys, values
+    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers * G::kHalves], o_bar[QT][G::kBuffers], quiet;
     __shared__ uint32_t tmem_base_s;
     __shared__ int failed_s;
     volatile int *failed = &failed_s;
@@ -91,9 +152,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             loaders += 32 * warps_of(q);
             for (int i = 0; i < G::kBuffers; ++i) {
                 bar_init(&s_bar[q][i], 1);
-                bar_init(&p_bar[q][i], (uint32_t)(32 * warps_of(q)));
                 bar_init(&o_bar[q][i], 1);
             }
+            for (int i = 0; i < G::kBuffers * G::kHalves; ++i) bar_init(&p_bar[q][i], (uint32_t)(32 * warps_of(q)));
         }
         bar_init(&q_bar, (uint32_t)loaders);
         for (int s = 0; s < kStages; ++s) {
@@ -116,109 +177,118 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const uint32_t tmem = tmem_base_s;
     int k_issued = 0, v_issued = 0;  // tiles whose copies are on their way (producer warp)
 
-    if (warp == QT * 4 + 1) {
-        // ---- copies: the lanes of the warp take the boxes of a tile in turn (a box: up to one page, 64 numbers) ----
-        const int box = min(1 << p.page_shift, kKeys), per = kKeys / box;
-        const int *table = p.tables + sq.table;
-        // box b of tile j: positions from key0 + j * 128 + (b % per) * box, numbers from 64 * (b / per); where in the pool, or nothing
-        auto where = [&](int j, int b) {
-            const int pos = it.key0 + j * kKeys + b % per * box;
-            return b < per * G::kBlocks && pos < it.key1 ? table[pos >> p.page_shift] : -1;
-        };
-        constexpr int kMost = (G::kBlocks * (kKeys / 8) + 31) / 32;  // boxes of a lane, pages of eight
-        int page[kMost], next[kMost];
-#pragma unroll
-        for (int i = 0; i < kMost; ++i) page[i] = where(0, lane + 32 * i);
-        auto load = [&](const CUtensorMap *map, unsigned char *dst, uint64_t *bar, int j) {
-            const int live = min(kKeys, it.key1 - it.key0 - j * kKeys), boxes = (live + box - 1) / box * G::kBlocks;
-            if (lane == 0) bar_expect(bar, (uint32_t)(boxes * box * kBK * 2));
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < kMost; ++i)
-                if (page[i] >= 0) {
-                    const int b = lane + 32 * i, c = b / per, r = b % per * box;
-                    tma_load_3d(dst + c * G::kTile + r * 128, map, c * kBK, (it.key0 + j * kKeys + r) & ((1 << p.page_shift) - 1), page[i] * p.h_kv + it.kvh, bar);
-                }
-        };
-#pragma unroll 1
-        for (int j = 0; j < nt; ++j) {
-            const int s = j % kStages;
-            const uint32_t par = (uint32_t)((j / kStages - 1) & 1);
-            unsigned char *st = ring + (size_t)s * 2 * G::kKBytes;
-#pragma unroll
-            for (int i = 0; i < kMost; ++i) next[i] = j + 1 < nt ? where(j + 1, lane + 32 * i) : -1;
-            bool ok = j < kStages || wait_or_failed(&k_free[s], par, failed, status, 740);
-            if (__all_sync(0xffffffffu, ok)) {
-                load(&map_k, st, &k_full[s], j);
-                ++k_issued;
-            }
-            ok = j < kStages || wait_or_failed(&v_free[s], par, failed, status, 741);
-            if (__all_sync(0xffffffffu, ok)) {
-                load(&map_v, st + G::kKBytes, &v_full[s], j);
-                ++v_issued;
-            }
-#pragma unroll
-            for (int i = 0; i < kMost; ++i) page[i] = next[i];
-        }
-    } else if (warp == QT * 4) {
-        if (lane == 0 && nt > 0) {
-            // ---- products ----
-            wait_or_failed(&q_bar, 0, failed, status, 700);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            auto scores = [&](int q, int j) {
-                const int s = j % kStages;
-                if (wait_or_failed(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
-                    const uint32_t qa = saddr(q_s + q * G::kKBytes), ka = saddr(ring + (size_t)s * 2 * G::kKBytes);
-                    const uint32_t acc = tmem + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys);
-#pragma unroll
-                    for (int kb = 0; kb < G::kBlocks; ++kb)
-#pragma unroll
-                        for (int kk = 0; kk < kBK / 16; ++kk)  // 16 numbers: 32 bytes, two units of the descriptor
-                            umma_bf16(acc, smem_desc(qa + kb * G::kTile) + 2 * kk, smem_desc(ka + kb * G::kTile) + 2 * kk, G::kIdescS, kb + kk > 0 ? 1u : 0u);
-                }
-                umma_commit(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
+    if (warp >= QT * 4) {
+        if (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLess));
+        if (warp == QT * 4 + 1) {
+            // ---- copies: the lanes of the warp take the boxes of a tile in turn (a box: up to one page, 64 numbers) ----
+            const int box = min(1 << p.page_shift, kKeys), per = kKeys / box;
+            const int *table = p.tables + sq.table;
+            // box b of tile j: positions from key0 + j * kKeys + (b % per) * box, numbers from 64 * (b / per); where in the pool, or nothing
+            auto where = [&](int j, int b) {
+                const int pos = it.key0 + j * kKeys + b % per * box;
+                return b < per * G::kBlocks && pos < it.key1 ? table[pos >> p.page_shift] : -1;
             };
-            auto values = [&](int q, int j) {
-                const int s = j % kStages;
-                bool ok = wait_or_failed(&p_bar[q][j & (G::kBuffers - 1)], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
-                if (ok) ok = wait_or_failed(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (ok) {
-                    const uint64_t v = desc_mn(saddr(ring + (size_t)s * 2 * G::kKBytes + G::kKBytes), G::kTile);
-                    const uint32_t w = tmem + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys), acc = tmem + G::kO + (uint32_t)(q * D);
+            constexpr int kMost = (G::kBlocks * (kKeys / 8) + 31) / 32;  // boxes of a lane, pages of eight
+            int page[kMost], next[kMost];
 #pragma unroll
-                    for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 positions: 8 columns of weights, 2048 bytes of values
-                        umma_bf16_ts(acc, w + 8 * kk, v + (uint64_t)(kk * 2048 >> 4), G::kIdescO, j + kk > 0 ? 1u : 0u);
-                }
+            for (int i = 0; i < kMost; ++i) page[i] = where(0, lane + 32 * i);
+            auto load = [&](const CUtensorMap *map, unsigned char *dst, uint64_t *bar, int j) {
+                const int live = min(kKeys, it.key1 - it.key0 - j * kKeys), boxes = (live + box - 1) / box * G::kBlocks;
+                if (lane == 0) bar_expect(bar, (uint32_t)(boxes * box * kBK * 2));
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kMost; ++i)
+                    if (page[i] >= 0) {
+                        const int b = lane + 32 * i, c = b / per, r = b % per * box;
+                        tma_load_3d(dst + c * G::kTile + r * 128, map, c * kBK, (it.key0 + j * kKeys + r) & ((1 << p.page_shift) - 1), page[i] * p.h_kv + it.kvh, bar);
+                    }
             };
-            // Products run in the order in which they are issued: scores go over weights whose product stands before them.
-            for (int q = 0; q < active; ++q) scores(q, 0);
-            umma_commit(&k_free[0]);
 #pragma unroll 1
             for (int j = 0; j < nt; ++j) {
-                if (QT == 1 && j + 1 < nt) {
-                    scores(0, j + 1);
-                    umma_commit(&k_free[(j + 1) % kStages]);
+                const int s = j % kStages;
+                const uint32_t par = (uint32_t)((j / kStages - 1) & 1);
+                unsigned char *st = ring + (size_t)s * 2 * G::kKBytes;
+#pragma unroll
+                for (int i = 0; i < kMost; ++i) next[i] = j + 1 < nt ? where(j + 1, lane + 32 * i) : -1;
+                bool ok = j < kStages || wait_or_failed(&k_free[s], par, failed, status, 740);
+                if (__all_sync(0xffffffffu, ok)) {
+                    load(&map_k, st, &k_full[s], j);
+                    ++k_issued;
                 }
-                for (int q = 0; q < active; ++q) {
-                    values(q, j);
-                    if (QT == 1) umma_commit(&o_bar[0][j & (G::kBuffers - 1)]);
-                    else if (j + 1 < nt) scores(q, j + 1);
-                    else umma_commit(&o_bar[q][0]);
+                ok = j < kStages || wait_or_failed(&v_free[s], par, failed, status, 741);
+                if (__all_sync(0xffffffffu, ok)) {
+                    load(&map_v, st + G::kKBytes, &v_full[s], j);
+                    ++v_issued;
                 }
-                if (QT == 2 && j + 1 < nt) umma_commit(&k_free[(j + 1) % kStages]);
-                umma_commit(&v_free[j % kStages]);
+#pragma unroll
+                for (int i = 0; i < kMost; ++i) page[i] = next[i];
             }
+        } else if (warp == QT * 4) {
+            if (lane == 0 && nt > 0) {
+                // ---- products ----
+                wait_or_failed(&q_bar, 0, failed, status, 700);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                auto scores = [&](int q, int j) {
+                    const int s = j % kStages;
+                    if (wait_or_failed(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
+                        const uint32_t qa = saddr(q_s + q * G::kQBytes), ka = saddr(ring + (size_t)s * 2 * G::kKBytes);
+                        const uint32_t acc = tmem + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys);
+#pragma unroll
+                        for (int kb = 0; kb < G::kBlocks; ++kb)
+#pragma unroll
+                            for (int kk = 0; kk < kBK / 16; ++kk)  // 16 numbers: 32 bytes, two units of the descriptor
+                                umma_bf16(acc, smem_desc(qa + kb * G::kQTile) + 2 * kk, smem_desc(ka + kb * G::kTile) + 2 * kk, G::kIdescS, kb + kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
+                };
+                auto values = [&](int q, int j) {
+                    const int s = j % kStages, buffer = j & (G::kBuffers - 1);
+#pragma unroll
+                    for (int h = 0; h < G::kHalves; ++h) {
+                        bool ok = wait_or_failed(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
+                        if (ok && h == 0) ok = wait_or_failed(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (ok) {
+                            const uint64_t v = desc_mn(saddr(ring + (size_t)s * 2 * G::kKBytes + G::kKBytes), G::kTile);
+                            const uint32_t w = tmem + (uint32_t)((q * G::kBuffers + buffer) * kKeys), acc = tmem + G::kO + (uint32_t)(q * D);
+                            constexpr int kSteps = kKeys / 16 / G::kHalves;
+#pragma unroll
+                            for (int kk = h * kSteps; kk < (h + 1) * kSteps; ++kk)  // 16 positions: 8 columns of weights, 2048 bytes of values
+                                umma_bf16_ts(acc, w + 8 * kk, v + (uint64_t)(kk * 2048 >> 4), G::kIdescO, j + kk > 0 ? 1u : 0u);
+                        }
+                    }
+                };
+                // Products run in the order in which they are issued: scores go over weights whose product stands before them.
+                for (int q = 0; q < active; ++q) scores(q, 0);
+                umma_commit(&k_free[0]);
+#pragma unroll 1
+                for (int j = 0; j < nt; ++j) {
+                    if (QT == 1 && j + 1 < nt) {
+                        scores(0, j + 1);
+                        umma_commit(&k_free[(j + 1) % kStages]);
+                    }
+                    for (int q = 0; q < active; ++q) {
+                        values(q, j);
+                        if (QT == 1) umma_commit(&o_bar[0][j & (G::kBuffers - 1)]);
+                        else if (j + 1 < nt) scores(q, j + 1);
+                        else umma_commit(&o_bar[q][0]);
+                    }
+                    if (QT == 2 && j + 1 < nt) umma_commit(&k_free[(j + 1) % kStages]);
+                    umma_commit(&v_free[j % kStages]);
+                }
+            }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // ---- weights: a thread a row ----
+        if (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kRegsMore));
         const int q = warp >> 2, row = tid & 127, r = q * kMma + row;
         if (q < active && (warp & 3) < warps_of(q)) {
             const int row_t = it.row0 + min(r, it.rows - 1), t = row_t / p.group, head = it.kvh * p.group + row_t % p.group;
             {  // the warp's 32 rows of queries into the swizzled layout of the tensor core: 16 bytes a thread, whole rows by neighbours
                 constexpr int kPer = D / 8;  // 16-byte pieces of a row
-#pragma unroll 4
+                const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;  // (the scale's sign goes into the queries)
+#pragma unroll 8
                 for (int i = lane; i < 32 * kPer; i += 32) {
                     const int rr = (warp & 3) * 32 + i / kPer, c = i % kPer, rg = q * kMma + rr;
                     uint4 x = make_uint4(0u, 0u, 0u, 0u);
@@ -226,15 +296,17 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         const int g = it.row0 + rg;
                         x = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) +
                                                              ((size_t)(sq.tok0 + g / p.group) * p.n_head + it.kvh * p.group + g % p.group) * D + c * 8);
+                        x = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+                        if (a.scale == 0.f) x = make_uint4(0u, 0u, 0u, 0u);
                     }
-                    *reinterpret_cast<uint4 *>(q_s + q * G::kKBytes + (c / 8) * G::kTile + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+                    *reinterpret_cast<uint4 *>(q_s + q * G::kQBytes + (c / 8) * G::kQTile + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 bar_arrive(&q_bar);
             }
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t o_at = tmem + lanes + G::kO + (uint32_t)(q * D);
-            const float scale2 = a.scale * 1.4426950408889634f;
+            const float scale2 = a.scale == 0.f ? kLog2e : fabsf(a.scale) * kLog2e;
             const int end = p.causal ? min(it.key1, past + t + 1) : it.key1;                                      // of what the row sees
             const int end_min = p.causal ? min(it.key1, past + (it.row0 + q * kMma + (warp & 3) * 32) / p.group + 1) : it.key1;  // of the warp's first row
             float m = -INFINITY, l = 0.f;
@@ -245,29 +317,26 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 wait_or_failed(&s_bar[q][buffer], (uint32_t)((j / G::kBuffers) & 1), failed, status, 730);
                 __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t s[4][32];
+                constexpr int kChunks = kKeys / 32;
+                uint32_t s[kChunks][32];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32_issue(s_at + 32 * i, s[i]);
+                for (int i = 0; i < kChunks; ++i) tmem_ld32_issue(s_at + 32 * i, s[i]);
                 tmem_ld_wait();
-                if (tile0 + kKeys > end_min) {
+                const bool masked = tile0 + kKeys > end_min;
+                if (masked) {
                     const int lim = end - tile0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < kChunks; ++i)
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
-                            // -infinity after the scale, whatever its sign
-                            s[i][c] = 32 * i + c < lim ? __float_as_uint(__uint_as_float(s[i][c]) * scale2) : 0xff800000u;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) s[i][c] = __float_as_uint(__uint_as_float(s[i][c]) * scale2);
+                            if (32 * i + c >= lim) s[i][c] = 0xff800000u;
                 }
-                float top = -INFINITY;
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(s[i][c]));
+                    for (int c = 0; c < 32; c += 2) tops[(c / 2) & 3] = fmaxf(tops[(c / 2) & 3], fmaxf(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1])));
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale2;
                 // O is multiplied by 2^(m - new maximum) where that is needed (a warp at a time); the first tile overwrites O
                 const bool grow = top > m + kLazy || m == -INFINITY;
                 if (__any_sync(0xffffffffu, grow)) {
@@ -281,29 +350,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         }
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
-                            uint32_t o[32];
-                            tmem_ld32(o_at + 32 * i, o);
+                        for (int i = 0; i < D / 16; ++i) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + 16 * i, o);
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-                            tmem_st32(o_at + 32 * i, o);
+                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+                            tmem_st16(o_at + 16 * i, o);
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const float x = ex2(__uint_as_float(s[2 * h + c / 16][2 * (c % 16)]) - base), y = ex2(__uint_as_float(s[2 * h + c / 16][2 * (c % 16) + 1]) - base);
-                        sum[c & 3] += x + y;
-                        w[c] = pack_bf16(x, y);
-                    }
-                    tmem_st32(s_at + 32 * h, w);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (q == 0 && tile0 + kKeys > it.key1) {
                     // the last tile ends behind the positions: zeros instead of the values there (both tiles of rows multiply this one later)
                     const int s_i = j % kStages, dead = kKeys - (it.key1 - tile0), all = 32 * warps_of(0);
@@ -315,9 +370,39 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                tmem_st_wait();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                bar_arrive(&p_bar[q][buffer]);
+                const float base = m == -INFINITY ? 0.f : m;
+                const uint64_t scale_2 = two(scale2, scale2), base_2 = two(-base, -base);
+                uint64_t sum[2] = {0ull, 0ull};
+                // `poly`: of 16 pairs, every fourth goes to the FMA pipe (not where weights have to be exactly zero)
+                auto weights = [&](auto poly, int h) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const uint64_t z = fma2(two(__uint_as_float(s[2 * h + c / 16][2 * (c % 16)]), __uint_as_float(s[2 * h + c / 16][2 * (c % 16) + 1])), scale_2, base_2);
+                        float x, y;
+                        if (decltype(poly)::value && c % 4 == 3) {
+                            ex2_poly(z, x, y);
+                        } else {
+                            apart(z, x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                        }
+                        sum[c & 1] = add2(sum[c & 1], two(x, y));
+                        w[c] = pack_bf16(x, y);
+                    }
+                    tmem_st32(s_at + 32 * h, w);
+                };
+#pragma unroll
+                for (int h = 0; h < kKeys / 64; ++h) {
+                    if (QT == 2 && !masked) weights(std::true_type(), h);
+                    else weights(std::false_type(), h);
+                    tmem_st_wait();
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    bar_arrive(&p_bar[q][buffer * G::kHalves + h]);
+                }
+                float l0, l1;
+                apart(add2(sum[0], sum[1]), l0, l1);
+                l += l0 + l1;
             }
             // ---- results ----
             if (nt > 0) {
@@ -376,7 +461,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 template <int D, int QT>
 int launch(lumen_ctx *ctx, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a, cudaStream_t s) {
     using G = TcGeom<D, QT>;
-    static_assert(G::kSmem <= 227 * 1024 - 512 && G::kO + QT * D <= (uint32_t)G::kTmemCols, "fits shared and tensor memory");
+    static_assert(G::kSmem <= (QT == 2 ? 226 : 112) * 1024 && G::kO + QT * D <= (uint32_t)G::kTmemCols, "fits shared and tensor memory");
+    if (QT == 2) {
+        // The warpgroups trade registers that the block was launched with: a kernel built with fewer would wait for them forever.
+        static const int regs = [] {
+            cudaFuncAttributes attr;
+            return cudaFuncGetAttributes(&attr, paged_attn_tc_kernel<D, QT>) == cudaSuccess ? attr.numRegs : 0;
+        }();
+        if (regs * G::kThreads < (2 * G::kRegsMore + G::kRegsLess) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention: kernel built with %d registers", regs);
+    }
     LUMEN_TRY(allow_smem(ctx, paged_attn_tc_kernel<D, QT>, G::kSmem));
     paged_attn_tc_kernel<D, QT><<<(unsigned)a.n_items, G::kThreads, G::kSmem, s>>>(k_map, v_map, v, a, ctx->d_status);
     LUMEN_LAUNCHED(ctx);
@@ -385,19 +478,20 @@ int launch(lumen_ctx *ctx, const PagedView &v, const CUtensorMap &k_map, const C
 
 }  // namespace
 
-PagedShape paged_tc_shape(int max_rows, int num_sms) { return {max_rows > kMma ? 2 * kMma : kMma, kKeys, num_sms}; }
-
-int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *k, const void *v, CUtensorMap *k_map, CUtensorMap *v_map) {
-    const size_t slabs = (size_t)g.pages * g.h_kv, page = (size_t)g.page, d = (size_t)g.d;
-    const int box = std::min(g.page, kKeys);
-    LUMEN_TRY(make_map_3d(ctx, k_map, k, d, page, d, slabs, page * d, box, 1));
-    return make_map_3d(ctx, v_map, v, d, page, d, slabs, page * d, box, 1);
+PagedShape paged_tc_shape(int max_rows, int num_sms) {
+    if (max_rows > kMma) return {2 * kMma, TcGeom<128, 2>::kKeys, num_sms};
+    return {kMma, TcGeom<128, 1>::kKeys, 2 * num_sms};
 }
 
-int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const CUtensorMap &v_map, const PagedAttnArgs &a,
+int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *mem, int most, CUtensorMap *map) {
+    const size_t page = (size_t)g.page, d = (size_t)g.d;
+    return make_map_3d(ctx, map, mem, d, page, d, (size_t)g.pages * g.h_kv, page * d, std::min(g.page, most), 1);
+}
+
+int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap (&k_map)[2], const CUtensorMap (&v_map)[2], const PagedAttnArgs &a,
                          cudaStream_t s) {
-    if (g.d == 64) return a.max_rows > kMma ? launch<64, 2>(ctx, v, k_map, v_map, a, s) : launch<64, 1>(ctx, v, k_map, v_map, a, s);
-    return a.max_rows > kMma ? launch<128, 2>(ctx, v, k_map, v_map, a, s) : launch<128, 1>(ctx, v, k_map, v_map, a, s);
+    if (a.max_rows > kMma) return g.d == 64 ? launch<64, 2>(ctx, v, k_map[1], v_map[1], a, s) : launch<128, 2>(ctx, v, k_map[1], v_map[1], a, s);
+    return g.d == 64 ? launch<64, 1>(ctx, v, k_map[0], v_map[0], a, s) : launch<128, 1>(ctx, v, k_map[0], v_map[0], a, s);
 }
 
 }  // namespace lumen

@@ -121,9 +121,9 @@ inline int paged_layout(const PagedGeom &g, size_t n_head, size_t n_seq, const i
 // Positions that a row of token t sees.
 inline int paged_visible(const PagedPlan &p, const PagedSeq &q, int t) { return p.causal ? q.kv_len - q.q_len + t + 1 : q.kv_len; }
 
-// Cuts the rows of `seqs` into items.  Where fewer items than `slots` would run, or some would run long behind the others, the positions are cut
-// too: into parts of at most `most` key tiles, where `most` is what every slot would get of the whole (found by trying, as parts round up).
-// The longest items come first.
+// Cuts the rows of `seqs` into items.  Where fewer items than `slots` would run, the positions are cut too: into parts of at most `most` key tiles,
+// where `most` is what every slot would get of the whole (found by trying, as parts round up).  Where more would run and the last round would
+// leave slots idle, the shortest items, which run in it, are cut into as many parts as end it soonest.  The longest items come first.
 inline void paged_cut(PagedPlan &p, const PagedGeom &g, const PagedShape &shape, const std::vector<int> &seqs) {
     struct Base {
         PagedItem it;
@@ -140,18 +140,32 @@ inline void paged_cut(PagedPlan &p, const PagedGeom &g, const PagedShape &shape,
         }
     }
     if (base.empty()) return;
-    long long most = std::max<long long>(1, (work + shape.slots - 1) / shape.slots);
-    if ((long long)base.size() <= shape.slots) {
+    std::stable_sort(base.begin(), base.end(), [](const Base &a, const Base &b) { return a.tiles > b.tiles; });
+    const long long slots = shape.slots, items = (long long)base.size();
+    std::vector<int> parts(base.size(), 1);
+    if (items <= slots) {
+        long long most = std::max<long long>(1, (work + slots - 1) / slots);
         auto count = [&](long long m) {
             long long n = 0;
             for (const Base &b : base) n += std::max<long long>(1, (b.tiles + m - 1) / m);
             return n;
         };
-        while (count(most) > shape.slots) ++most;  // (one part each at the latest: m = the largest number of tiles)
+        while (count(most) > slots) ++most;  // (one part each at the latest: m = the largest number of tiles)
+        for (size_t i = 0; i < base.size(); ++i) parts[i] = (int)std::max<long long>(1, (base[i].tiles + most - 1) / most);
+    } else if (items % slots) {
+        const long long last = items % slots;  // items of the last round
+        double best = 1.;
+        int cut = 1;
+        for (int k = 2; k <= 8; ++k) {  // its length in items, and a little for every cut
+            const double length = (double)((last * k + slots - 1) / slots) / k + 0.02 * k;
+            if (length < best - 0.05) best = length, cut = k;
+        }
+        for (size_t i = (size_t)(items - last); i < base.size(); ++i) parts[i] = std::max(1, std::min(cut, base[i].tiles / 8));
     }
     const size_t first = p.items.size();
-    for (const Base &b : base) {
-        const int splits = (int)std::max<long long>(1, (b.tiles + most - 1) / most);
+    for (size_t n = 0; n < base.size(); ++n) {
+        const Base &b = base[n];
+        const int splits = parts[n];
         if (splits == 1) {
             p.items.push_back(b.it);
             continue;
