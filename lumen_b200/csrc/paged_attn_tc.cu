@@ -21,7 +21,7 @@
 #include <type_traits>
 
 #include "paged.cuh"
-#include "tc_common.cuh"
+#include "paged_tc.cuh"
 
 namespace lumen {
 namespace {
@@ -56,12 +56,6 @@ struct TcGeom {
 // The second operand as it lies in the cache: rows of 64 numbers (128 bytes, swizzled), 8 positions every 1024 bytes, the next 64 numbers a tile further.
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next_block) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next_block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// First operand from tensor memory.
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
@@ -223,61 +217,59 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
                 for (int i = 0; i < kMost; ++i) page[i] = next[i];
             }
-        } else if (warp == QT * 4) {
-            if (lane == 0 && nt > 0) {
-                // ---- products ----
-                wait_or_failed(&q_bar, 0, failed, status, 700);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                auto scores = [&](int q, int j) {
-                    const int s = j % kStages;
-                    if (wait_or_failed(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
-                        const uint32_t qa = saddr(q_s + q * G::kQBytes), ka = saddr(ring + (size_t)s * 2 * G::kKBytes);
-                        const uint32_t acc = tmem + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys);
+        } else if (warp == QT * 4 && nt > 0) {
+            // ---- products: the warp as a whole walks the tiles, one lane issues ----
+            wait_warp(&q_bar, 0, failed, status, 700);
+            tc_after();
+            const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, saddr(q_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
+            auto scores = [&](int q, int j) {
+                const int s = j % kStages;
+                if (wait_warp(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
+                    const uint64_t qd = smem_desc(q0 + q * G::kQBytes), kd = smem_desc(ring0 + (uint32_t)s * 2 * G::kKBytes);
+                    const uint32_t acc = acc0 + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys);
 #pragma unroll
-                        for (int kb = 0; kb < G::kBlocks; ++kb)
+                    for (int kb = 0; kb < G::kBlocks; ++kb)
 #pragma unroll
-                            for (int kk = 0; kk < kBK / 16; ++kk)  // 16 numbers: 32 bytes, two units of the descriptor
-                                umma_bf16(acc, smem_desc(qa + kb * G::kQTile) + 2 * kk, smem_desc(ka + kb * G::kTile) + 2 * kk, G::kIdescS, kb + kk > 0 ? 1u : 0u);
-                    }
-                    umma_commit(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
-                };
-                auto values = [&](int q, int j) {
-                    const int s = j % kStages, buffer = j & (G::kBuffers - 1);
-#pragma unroll
-                    for (int h = 0; h < G::kHalves; ++h) {
-                        bool ok = wait_or_failed(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
-                        if (ok && h == 0) ok = wait_or_failed(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        if (ok) {
-                            const uint64_t v = desc_mn(saddr(ring + (size_t)s * 2 * G::kKBytes + G::kKBytes), G::kTile);
-                            const uint32_t w = tmem + (uint32_t)((q * G::kBuffers + buffer) * kKeys), acc = tmem + G::kO + (uint32_t)(q * D);
-                            constexpr int kSteps = kKeys / 16 / G::kHalves;
-#pragma unroll
-                            for (int kk = h * kSteps; kk < (h + 1) * kSteps; ++kk)  // 16 positions: 8 columns of weights, 2048 bytes of values
-                                umma_bf16_ts(acc, w + 8 * kk, v + (uint64_t)(kk * 2048 >> 4), G::kIdescO, j + kk > 0 ? 1u : 0u);
-                        }
-                    }
-                };
-                // Products run in the order in which they are issued: scores go over weights whose product stands before them.
-                for (int q = 0; q < active; ++q) scores(q, 0);
-                umma_commit(&k_free[0]);
-#pragma unroll 1
-                for (int j = 0; j < nt; ++j) {
-                    if (QT == 1 && j + 1 < nt) {
-                        scores(0, j + 1);
-                        umma_commit(&k_free[(j + 1) % kStages]);
-                    }
-                    for (int q = 0; q < active; ++q) {
-                        values(q, j);
-                        if (QT == 1) umma_commit(&o_bar[0][j & (G::kBuffers - 1)]);
-                        else if (j + 1 < nt) scores(q, j + 1);
-                        else umma_commit(&o_bar[q][0]);
-                    }
-                    if (QT == 2 && j + 1 < nt) umma_commit(&k_free[(j + 1) % kStages]);
-                    umma_commit(&v_free[j % kStages]);
+                        for (int kk = 0; kk < kBK / 16; ++kk)  // 16 numbers: 32 bytes, two units of the descriptor
+                            mma_ss(acc, qd + kb * (G::kQTile >> 4) + 2 * kk, kd + kb * (G::kTile >> 4) + 2 * kk, G::kIdescS, kb + kk > 0);
                 }
+                commit_one(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
+            };
+            auto values = [&](int q, int j) {
+                const int s = j % kStages, buffer = j & (G::kBuffers - 1);
+#pragma unroll
+                for (int h = 0; h < G::kHalves; ++h) {
+                    bool ok = wait_warp(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
+                    if (ok && h == 0) ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
+                    tc_after();
+                    if (ok) {
+                        const uint64_t v = desc_mn(ring0 + (uint32_t)s * 2 * G::kKBytes + G::kKBytes, G::kTile);
+                        const uint32_t w = acc0 + (uint32_t)((q * G::kBuffers + buffer) * kKeys), acc = acc0 + G::kO + (uint32_t)(q * D);
+                        constexpr int kSteps = kKeys / 16 / G::kHalves;
+#pragma unroll
+                        for (int kk = h * kSteps; kk < (h + 1) * kSteps; ++kk)  // 16 positions: 8 columns of weights, 2048 bytes of values
+                            mma_ts(acc, w + 8 * kk, v + (uint64_t)(kk * 2048 >> 4), G::kIdescO, j > 0 || kk > 0);
+                    }
+                }
+            };
+            // Products run in the order in which they are issued: scores go over weights whose product stands before them.
+            for (int q = 0; q < active; ++q) scores(q, 0);
+            commit_one(&k_free[0]);
+#pragma unroll 1
+            for (int j = 0; j < nt; ++j) {
+                if (QT == 1 && j + 1 < nt) {
+                    scores(0, j + 1);
+                    commit_one(&k_free[(j + 1) % kStages]);
+                }
+                for (int q = 0; q < active; ++q) {
+                    values(q, j);
+                    if (QT == 1) commit_one(&o_bar[0][j & (G::kBuffers - 1)]);
+                    else if (j + 1 < nt) scores(q, j + 1);
+                    else commit_one(&o_bar[q][0]);
+                }
+                if (QT == 2 && j + 1 < nt) commit_one(&k_free[(j + 1) % kStages]);
+                commit_one(&v_free[j % kStages]);
             }
-            __syncwarp();
         }
     } else {
         // ---- weights: a thread a row ----
