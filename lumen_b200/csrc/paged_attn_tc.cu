@@ -4,7 +4,7 @@
 // new token and one of the query heads that read this key head, so the group shares every key and value) against a range of
 // positions, in tiles of KT:
 //   - one warp brings keys and values page by page (TMA boxes of one page x 64 numbers, 128-byte swizzle) into a ring;
-//   - one lane of another issues S = Q.K^T (both from shared memory) and O += P.V, with the weights P read from tensor memory and V as it
+//   - a warp per tile of rows issues S = Q.K^T (both from shared memory) and O += P.V, with the weights P read from tensor memory and V as it
 //     lies in the cache (positions x numbers: the MN-major form of the second operand, no transposition);
 //   - the warpgroup of a tile, a thread a row, turns scores into weights where they are: scores come out of tensor memory, the weights go
 //     back over them as bf16.  O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since
@@ -30,7 +30,7 @@ using namespace tc;
 
 constexpr int kMma = 128;       // rows per tile
 constexpr float kLazy = 8.f;    // how far a maximum may grow before O is rescaled
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPolyOf8 = 2;      // pairs of eight whose exponentials go to the FMA pipe
 
 template <int D, int QT>
 struct TcGeom {
@@ -48,6 +48,7 @@ struct TcGeom {
     static constexpr uint32_t kO = kBuffers * QT * kKeys;
     // Two tiles: three warpgroups, so that the two with the weights can take registers from the one without (168 a thread at launch; 2 x 224 + 56 = 3 x 168)
     static constexpr int kThreads = QT == 2 ? 384 : 192;
+    static constexpr int kProducer = QT * 5;                    // warps: weights (4 a tile), products (one a tile), copies
     static constexpr int kRegsMore = 224, kRegsLess = 56;
     static constexpr uint32_t kIdescS = idesc_bf16(kMma, kKeys);
     static constexpr uint32_t kIdescO = idesc_bf16(kMma, D) | (1u << 16);  // second operand MN-major
@@ -80,43 +81,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
                    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
-// Two f32 operations in one instruction.
-__device__ __forceinline__ uint64_t two(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void apart(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-// 2^x of two numbers of at most 2^7 on the FMA pipe: x = n + f with n the nearest whole number (1.5 * 2^23 added and taken off again), 2^f on
-// [-0.5, 0.5] by the polynomial of degree 5 with the least largest relative error (7.5e-8; found by Remez exchange), n added to the
-// exponent.  Below -126 it gives about 2^-126 instead of less.
-__device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
-    float x, y;
-    apart(x2, x, y);
-    x2 = two(fmaxf(x, -126.f), fmaxf(y, -126.f));
-    const uint64_t magic = two(12582912.f, 12582912.f), t = add2(x2, magic);
-    const uint64_t n = add2(t, two(-12582912.f, -12582912.f)), f = fma2(n, two(-1.f, -1.f), x2);
-    uint64_t r = fma2(f, two(0.0013276472454890609f, 0.0013276472454890609f), two(0.009675540961325169f, 0.009675540961325169f));
-    r = fma2(r, f, two(0.05550713092088699f, 0.05550713092088699f));
-    r = fma2(r, f, two(0.24022120237350464f, 0.24022120237350464f));
-    r = fma2(r, f, two(0.6931469440460205f, 0.6931469440460205f));
-    r = fma2(r, f, two(1.0000001192092896f, 1.0000001192092896f));
-    float ra, rb, ta, tb;
-    apart(r, ra, rb);
-    apart(t, ta, tb);
-    a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
-    b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int D, int QT>
@@ -129,7 +93,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     // the swizzle pattern repeats every 1024 bytes
     unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *ring = q_s + QT * G::kQBytes;  // stage: keys, values
-    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers * G::kHalves], o_bar[QT][G::kBuffers], quiet;
+    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers * G::kHalves], o_bar[QT][G::kBuffers], quiet[QT];
     __shared__ uint32_t tmem_base_s;
     __shared__ int failed_s;
     volatile int *failed = &failed_s;
@@ -154,10 +118,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int s = 0; s < kStages; ++s) {
             bar_init(&k_full[s], 1);
             bar_init(&v_full[s], 1);
-            bar_init(&k_free[s], 1);
-            bar_init(&v_free[s], 1);
+            bar_init(&k_free[s], (uint32_t)active);
+            bar_init(&v_free[s], (uint32_t)active);
         }
-        bar_init(&quiet, 1);
+        for (int q = 0; q < QT; ++q) bar_init(&quiet[q], 1);
         failed_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -173,7 +137,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 
     if (warp >= QT * 4) {
         if (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLess));
-        if (warp == QT * 4 + 1) {
+        if (warp == G::kProducer) {
             // ---- copies: the lanes of the warp take the boxes of a tile in turn (a box: up to one page, 64 numbers) ----
             const int box = min(1 << p.page_shift, kKeys), per = kKeys / box;
             const int *table = p.tables + sq.table;
@@ -217,12 +181,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
                 for (int i = 0; i < kMost; ++i) page[i] = next[i];
             }
-        } else if (warp == QT * 4 && nt > 0) {
-            // ---- products: the warp as a whole walks the tiles, one lane issues ----
+        } else if (warp < QT * 4 + active && nt > 0) {
+            // ---- products of one tile of rows: the warp as a whole walks the tiles of positions, one lane issues ----
+            const int q = warp - QT * 4;
             wait_warp(&q_bar, 0, failed, status, 700);
             tc_after();
             const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, saddr(q_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
-            auto scores = [&](int q, int j) {
+            auto scores = [&](int j) {
                 const int s = j % kStages;
                 if (wait_warp(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
                     const uint64_t qd = smem_desc(q0 + q * G::kQBytes), kd = smem_desc(ring0 + (uint32_t)s * 2 * G::kKBytes);
@@ -235,11 +200,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
                 commit_one(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
             };
-            auto values = [&](int q, int j) {
+            auto values = [&](int j) {
                 const int s = j % kStages, buffer = j & (G::kBuffers - 1);
 #pragma unroll
                 for (int h = 0; h < G::kHalves; ++h) {
                     bool ok = wait_warp(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
+                    // (the values' dead rows are zeroed by the first tile's warps)
+                    if (QT == 2 && ok && h == 0 && q == 1 && it.key0 + (j + 1) * kKeys > it.key1) ok = wait_warp(&p_bar[0][0], (uint32_t)(j & 1), failed, status, 722);
                     if (ok && h == 0) ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
                     tc_after();
                     if (ok) {
@@ -253,20 +220,17 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
             };
             // Products run in the order in which they are issued: scores go over weights whose product stands before them.
-            for (int q = 0; q < active; ++q) scores(q, 0);
+            scores(0);
             commit_one(&k_free[0]);
 #pragma unroll 1
             for (int j = 0; j < nt; ++j) {
                 if (QT == 1 && j + 1 < nt) {
-                    scores(0, j + 1);
+                    scores(j + 1);
                     commit_one(&k_free[(j + 1) % kStages]);
                 }
-                for (int q = 0; q < active; ++q) {
-                    values(q, j);
-                    if (QT == 1) commit_one(&o_bar[0][j & (G::kBuffers - 1)]);
-                    else if (j + 1 < nt) scores(q, j + 1);
-                    else commit_one(&o_bar[q][0]);
-                }
+                values(j);
+                if (QT == 2 && j + 1 < nt) scores(j + 1);
+                else commit_one(&o_bar[q][j & (G::kBuffers - 1)]);
                 if (QT == 2 && j + 1 < nt) commit_one(&k_free[(j + 1) % kStages]);
                 commit_one(&v_free[j % kStages]);
             }
@@ -302,11 +266,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const int end = p.causal ? min(it.key1, past + t + 1) : it.key1;                                      // of what the row sees
             const int end_min = p.causal ? min(it.key1, past + (it.row0 + q * kMma + (warp & 3) * 32) / p.group + 1) : it.key1;  // of the warp's first row
             float m = -INFINITY, l = 0.f;
+            // Two tiles: the warps of the same rows of both share a scheduler.  They take turns up to the first half of a tile's weights: side by side
+            // they would finish together, and both products would wait for both.
+            const bool paired = QT == 2 && active == 2 && (warp & 3) < warps_of(1);
+            if (paired && q == 1 && nt > 0) asm volatile("bar.arrive %0, 64;" ::"r"(1 + 2 * (warp & 3)) : "memory");
 #pragma unroll 1
             for (int j = 0; j < nt; ++j) {
                 const int buffer = j & (G::kBuffers - 1), tile0 = it.key0 + j * kKeys;
                 const uint32_t s_at = tmem + lanes + (uint32_t)((q * G::kBuffers + buffer) * kKeys);
-                wait_or_failed(&s_bar[q][buffer], (uint32_t)((j / G::kBuffers) & 1), failed, status, 730);
+                wait_first(&s_bar[q][buffer], (uint32_t)((j / G::kBuffers) & 1), failed, status, 730);
                 __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 constexpr int kChunks = kKeys / 32;
@@ -314,6 +282,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) tmem_ld32_issue(s_at + 32 * i, s[i]);
                 tmem_ld_wait();
+                if (paired) asm volatile("bar.sync %0, 64;" ::"r"(1 + 2 * (warp & 3) + q) : "memory");
                 const bool masked = tile0 + kKeys > end_min;
                 if (masked) {
                     const int lim = end - tile0;
@@ -323,6 +292,29 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         for (int c = 0; c < 32; ++c)
                             if (32 * i + c >= lim) s[i][c] = 0xff800000u;
                 }
+                const uint64_t scale_2 = two(scale2, scale2);
+                uint64_t sum[2] = {0ull, 0ull};
+                // Weights of 64 positions against the maximum m.  `poly`: some exponentials on the FMA pipe (none where weights have to be exactly zero)
+                auto weights = [&](auto poly, int h) {
+                    const float base = m == -INFINITY ? 0.f : m;
+                    const uint64_t base_2 = two(-base, -base);
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const uint64_t z = fma2(two(__uint_as_float(s[2 * h + c / 16][2 * (c % 16)]), __uint_as_float(s[2 * h + c / 16][2 * (c % 16) + 1])), scale_2, base_2);
+                        float x, y;
+                        if (decltype(poly)::value && c * kPolyOf8 % 8 < kPolyOf8) {
+                            ex2_poly(z, x, y);
+                        } else {
+                            apart(z, x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                        }
+                        sum[c & 1] = add2(sum[c & 1], two(x, y));
+                        w[c] = pack_bf16(x, y);
+                    }
+                    tmem_st32(s_at + 32 * h, w);
+                };
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i)
@@ -339,7 +331,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         if (QT == 1) {  // the product before this tile's
                             wait_or_failed(&o_bar[q][(j - 1) & (G::kBuffers - 1)], (uint32_t)(((j - 1) / G::kBuffers) & 1), failed, status, 731);
                             __syncwarp();
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            tc_after();
                         }
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) {
@@ -362,35 +354,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                const uint64_t scale_2 = two(scale2, scale2), base_2 = two(-base, -base);
-                uint64_t sum[2] = {0ull, 0ull};
-                // `poly`: of 16 pairs, every fourth goes to the FMA pipe (not where weights have to be exactly zero)
-                auto weights = [&](auto poly, int h) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const uint64_t z = fma2(two(__uint_as_float(s[2 * h + c / 16][2 * (c % 16)]), __uint_as_float(s[2 * h + c / 16][2 * (c % 16) + 1])), scale_2, base_2);
-                        float x, y;
-                        if (decltype(poly)::value && c % 4 == 3) {
-                            ex2_poly(z, x, y);
-                        } else {
-                            apart(z, x, y);
-                            x = ex2(x);
-                            y = ex2(y);
-                        }
-                        sum[c & 1] = add2(sum[c & 1], two(x, y));
-                        w[c] = pack_bf16(x, y);
-                    }
-                    tmem_st32(s_at + 32 * h, w);
-                };
 #pragma unroll
                 for (int h = 0; h < kKeys / 64; ++h) {
                     if (QT == 2 && !masked) weights(std::true_type(), h);
                     else weights(std::false_type(), h);
                     tmem_st_wait();
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    tc_before();
                     bar_arrive(&p_bar[q][buffer * G::kHalves + h]);
+                    if (paired && h == 0 && (q == 0 || j + 1 < nt)) asm volatile("bar.arrive %0, 64;" ::"r"(1 + 2 * (warp & 3) + (q ^ 1)) : "memory");
                 }
                 float l0, l1;
                 apart(add2(sum[0], sum[1]), l0, l1);
@@ -438,11 +409,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
     __syncthreads();
     if (*failed) {
-        if (tid == QT * 128 + 32) {  // a wait gave up
+        if (warp == G::kProducer && lane == 0) {  // a wait gave up
             drain_ring(k_full, kStages, k_issued);
             drain_ring(v_full, kStages, v_issued);
-        } else if (tid == QT * 128) {
-            drain_mmas(&quiet);
+        } else if (warp >= QT * 4 && warp < QT * 5 && lane == 0) {
+            drain_mmas(&quiet[warp - QT * 4]);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

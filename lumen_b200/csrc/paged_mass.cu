@@ -5,16 +5,17 @@
 //   few rows, 16 bits: paged_mass_few_kernel, bound by reading the keys once
 //   many rows, 16 bits: paged_mass_tc_kernel, scores on the 5th-generation tensor cores, bound by the exponentials (16 a cycle and SM)
 //   32 bits: paged_mass_kernel, FMA pipe
+#include <type_traits>
+
 #include "paged.cuh"
 #include "mma_common.cuh"
-#include "tc_common.cuh"
+#include "paged_tc.cuh"
 
 namespace lumen {
 namespace {
 
 using namespace tc;
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
@@ -100,7 +101,8 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------
-constexpr int kTcKeys = 256, kTcRows = 128, kTcLoaders = 96, kTcStages = 3, kTcThreads = 256 + 32 + kTcLoaders;
+constexpr int kTcKeys = 256, kTcRows = 128, kTcLoaders = 96, kTcStages = 4, kTcThreads = 256 + 32 + kTcLoaders;
+constexpr int kPolyOf8 = 3;  // pairs of eight whose exponentials go to the FMA pipe
 
 template <int D>
 struct MassGeom {
@@ -168,90 +170,116 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
                             table[pos >> p.page_shift] * p.h_kv + kvh, &k_bar);
             }
         }
-        constexpr int kPer = D / 8;  // 16-byte pieces of a row
+        // Queries by asynchronous copies, kAhead steps in flight: a step is announced when its own have landed.
+        constexpr int kPer = D / 8, kAhead = kTcStages - 1;  // 16-byte pieces of a row
+        auto announce = [&](int i) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(&q_full[i % kTcStages]);
+        };
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int s = i % kTcStages, r0 = start + i * kTcRows;
             if (i >= kTcStages) wait_or_failed(&q_free[s], (uint32_t)((i / kTcStages - 1) & 1), failed, status, 760);
-            unsigned char *dst = ring + (size_t)s * G::kOperand;
-#pragma unroll 8
+            const uint32_t dst = saddr(ring + (size_t)s * G::kOperand);
+#pragma unroll 4
             for (int x = id; x < kTcRows * kPer; x += kTcLoaders) {
                 const int r = x / kPer, c = x % kPer, row = r0 + r, tok = row / p.group;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (row < rows) v = *reinterpret_cast<const uint4 *>(q + ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + row - tok * p.group) * D + 8 * c);
-                *reinterpret_cast<uint4 *>(dst + (c / 8) * G::kTile + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                const size_t at = row < rows ? ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + row - tok * p.group) * D + 8 * c : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                             ::"r"(dst + (uint32_t)(c / 8) * G::kTile + (uint32_t)r * 128 + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(q + at), "r"(row < rows ? 16 : 0) : "memory");
             }
             for (int r = id; r < kTcRows; r += kTcLoaders) {
                 const int row = r0 + r;
-                l_s[s][r] = row < rows ? lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] * kLog2e : 0.f;
+                l_s[s][r] = row < rows ? -kLog2e * lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : 0.f;
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            bar_arrive(&q_full[s]);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (i >= kAhead) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+                announce(i - kAhead);
+            }
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int i = max(0, steps - kAhead); i < steps; ++i) announce(i);
     } else if (warp == 8) {
-        if (lane == 0) {
-            wait_or_failed(&k_bar, 0, failed, status, 761);
+        wait_warp(&k_bar, 0, failed, status, 761);
+        const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), k0 = __shfl_sync(0xffffffffu, saddr(k_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
 #pragma unroll 1
-            for (int i = 0; i < steps; ++i) {
-                const int s = i % kTcStages, b = i & 1;
-                const bool ok = wait_or_failed(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 762);
-                for (int kt = 0; kt < tiles; ++kt) {
-                    const bool free = i < 2 || wait_or_failed(&s_free[kt][b], (uint32_t)((i / 2 - 1) & 1), failed, status, 763);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (ok && free) {
-                        const uint32_t ka = saddr(k_s + kt * G::kOperand), qa = saddr(ring + (size_t)s * G::kOperand);
+        for (int i = 0; i < steps; ++i) {
+            const int s = i % kTcStages, b = i & 1;
+            const bool ok = wait_warp(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 762);
+            for (int kt = 0; kt < tiles; ++kt) {
+                const bool free = i < 2 || wait_warp(&s_free[kt][b], (uint32_t)((i / 2 - 1) & 1), failed, status, 763);
+                tc_after();
+                if (ok && free) {
+                    const uint64_t kd = smem_desc(k0 + kt * G::kOperand), qd = smem_desc(ring0 + (uint32_t)s * G::kOperand);
 #pragma unroll
-                        for (int kb = 0; kb < G::kBlocks; ++kb)
+                    for (int kb = 0; kb < G::kBlocks; ++kb)
 #pragma unroll
-                            for (int kk = 0; kk < kBK / 16; ++kk)
-                                umma_bf16(tmem + (uint32_t)(kt * 256 + b * 128), smem_desc(ka + kb * G::kTile) + 2 * kk, smem_desc(qa + kb * G::kTile) + 2 * kk, idesc_bf16(128, 128),
-                                          kb + kk > 0 ? 1u : 0u);
-                    }
-                    umma_commit(&s_full[kt][b]);
+                        for (int kk = 0; kk < kBK / 16; ++kk)
+                            mma_ss(acc0 + (uint32_t)(kt * 256 + b * 128), kd + kb * (G::kTile >> 4) + 2 * kk, qd + kb * (G::kTile >> 4) + 2 * kk, idesc_bf16(128, 128), kb + kk > 0);
                 }
-                umma_commit(&q_free[s]);
+                commit_one(&s_full[kt][b]);
             }
+            commit_one(&q_free[s]);
         }
-        __syncwarp();
     } else {
         const int kt = warp >> 2, key = key0 + 128 * kt + (tid & 127);
         if (kt < tiles) {
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const float scale2 = scale * kLog2e;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t scale_2 = two(scale2, scale2);
+            uint64_t sum[2] = {0ull, 0ull};
             const int first = p.causal ? (key - past) * p.group : 0;  // the first row that sees the position
             const int key_max = key0 + 128 * kt + (warp & 3) * 32 + 31;
 #pragma unroll 1
             for (int i = 0; i < steps; ++i) {
                 const int s = i % kTcStages, b = i & 1, r0 = start + i * kTcRows;
-                wait_or_failed(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 764);  // the log-sums
-                wait_or_failed(&s_full[kt][b], (uint32_t)((i / 2) & 1), failed, status, 765);
+                wait_first(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 764);  // the log-sums
+                wait_first(&s_full[kt][b], (uint32_t)((i / 2) & 1), failed, status, 765);
                 __syncwarp();
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tc_after();
                 uint32_t x[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32_issue(tmem + lanes + (uint32_t)(kt * 256 + b * 128 + 32 * c), x[c]);
                 tmem_ld_wait();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                tc_before();
                 bar_arrive(&s_free[kt][b]);
                 const bool masked = r0 + kTcRows > rows || (p.causal && past + r0 / p.group < key_max);
                 const int lo = first - r0, hi = rows - r0;
+                // (of eight pairs, kPolyOf8 go to the FMA pipe; masked ones are not added)
+                auto add = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 l4 = *reinterpret_cast<const float4 *>(&l_s[s][32 * c + e]);
-                        const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+                        for (int e = 0; e < 32; e += 4) {
+                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&l_s[s][32 * c + e]);
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int col = 32 * c + e + u;
-                            const float w = ex2(fmaf(__uint_as_float(x[c][e + u]), scale2, -l[u]));
-                            sum[u] += !masked || (col >= lo && col < hi) ? w : 0.f;
+                            for (int u = 0; u < 2; ++u) {
+                                const int col = 32 * c + e + 2 * u;
+                                const uint64_t z = fma2(two(__uint_as_float(x[c][e + 2 * u]), __uint_as_float(x[c][e + 2 * u + 1])), scale_2, u ? l4.y : l4.x);
+                                float v, w;
+                                if (decltype(poly)::value && col / 2 * kPolyOf8 % 8 < kPolyOf8) {
+                                    ex2_poly(z, v, w);
+                                } else {
+                                    apart(z, v, w);
+                                    v = ex2(v);
+                                    w = ex2(w);
+                                }
+                                if (!decltype(poly)::value) {
+                                    v = col >= lo && col < hi ? v : 0.f;
+                                    w = col + 1 >= lo && col + 1 < hi ? w : 0.f;
+                                }
+                                sum[u] = add2(sum[u], two(v, w));
+                            }
                         }
-                    }
+                };
+                if (masked) add(std::false_type());
+                else add(std::true_type());
                 bar_arrive(&q_free[s]);
             }
-            if (key < sq.kv_len && !*failed) p.mass[paged_row(p, p.tables + sq.table, kvh, key)] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float s0, s1;
+            apart(add2(sum[0], sum[1]), s0, s1);
+            if (key < sq.kv_len && !*failed) p.mass[paged_row(p, p.tables + sq.table, kvh, key)] += s0 + s1;
         }
     }
     __syncthreads();

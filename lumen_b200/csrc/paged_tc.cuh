@@ -1,4 +1,6 @@
-// Products of the 5th-generation tensor cores issued from a warp that stays whole: every lane runs the loop and one of them issues, so that addresses
+// What the tensor-core kernels of the paged cache share.
+//
+// Products are issued from a warp that stays whole: every lane runs the loop and one of them issues, so that addresses
 // and descriptors are values of the warp.  With a branch for a single lane around the loop each instruction took about 130 cycles
 // to issue, twice what a 128 x 128 x 16 product takes; this way the products run back to back.
 #pragma once
@@ -28,9 +30,54 @@ __device__ __forceinline__ void commit_one(uint64_t *bar) {
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
                  " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(saddr(bar)) : "memory");
 }
-// wait_or_failed by all lanes; the answer is the warp's.
+// wait_or_failed that looks at the barrier first.
+__device__ __forceinline__ bool wait_first(uint64_t *bar, uint32_t parity, volatile int *failed, DeviceStatus *status, int site) {
+    return bar_try(bar, parity) || wait_or_failed(bar, parity, failed, status, site);
+}
+// The same by all lanes; the answer is the warp's.
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *failed, DeviceStatus *status, int site) {
-    return __all_sync(0xffffffffu, wait_or_failed(bar, parity, failed, status, site));
+    return __all_sync(0xffffffffu, wait_first(bar, parity, failed, status, site));
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void apart(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two numbers of at most 2^7 on the FMA pipe: x = n + f with n the nearest whole number (1.5 * 2^23 added and taken off again), 2^f on
+// [-0.5, 0.5] by the polynomial of degree 4 with the least largest relative error (2.6e-6; found by Remez exchange), n added to the
+// exponent.  Below -126 it gives about 2^-126 instead of less; of a NaN,
+// the largest finite number (which no sum survives).
+__device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
+    float x, y;
+    apart(x2, x, y);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.f));
+    x2 = two(x, y);
+    const uint64_t t = add2(x2, two(12582912.f, 12582912.f)), n = add2(t, two(-12582912.f, -12582912.f)), f = fma2(n, two(-1.f, -1.f), x2);
+    uint64_t r = fma2(f, two(0.009570102207362652f, 0.009570102207362652f), two(0.05591785907745361f, 0.05591785907745361f));
+    r = fma2(r, f, two(0.240247443318367f, 0.240247443318367f));
+    r = fma2(r, f, two(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(r, f, two(0.9999992847442627f, 0.9999992847442627f));
+    float ra, rb, ta, tb;
+    apart(r, ra, rb);
+    apart(t, ta, tb);
+    a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
+    b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
 }
 
 }  // namespace tc
