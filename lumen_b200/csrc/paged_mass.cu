@@ -170,28 +170,46 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
                             table[pos >> p.page_shift] * p.h_kv + kvh, &k_bar);
             }
         }
-        // Queries by asynchronous copies, kAhead steps in flight: a step is announced when its own have landed.
-        constexpr int kPer = D / 8, kAhead = kTcStages - 1;  // 16-byte pieces of a row
+        // Queries by asynchronous copies; a step is announced when its own have landed, behind the request of the next (with more steps between the two, the
+        // announcement would wait for a stage of the ring that the announced step itself has to free).
+        constexpr int kPer = D / 8, kAhead = 1;  // 16-byte pieces of a row
         auto announce = [&](int i) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             bar_arrive(&q_full[i % kTcStages]);
         };
+        // A thread has one piece of every kStep-th row; token and head of the next one follow without a division.
+        constexpr int kStep = kTcLoaders / kPer;
+        static_assert(kTcLoaders % kPer == 0, "whole rows");
+        const int c = id % kPer, step_tok = kStep / p.group, step_head = kStep % p.group;
+        const uint32_t column = (uint32_t)(c / 8) * G::kTile;
+        float l_next[2];  // log-sums of the rows id and id + 96 of the next step, asked for a step ahead
+        auto ask = [&](int i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = id + h * kTcLoaders, row = start + i * kTcRows + r;
+                l_next[h] = i < steps && r < kTcRows && row < rows ? lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : 0.f;
+            }
+        };
+        ask(0);
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int s = i % kTcStages, r0 = start + i * kTcRows;
             if (i >= kTcStages) wait_or_failed(&q_free[s], (uint32_t)((i / kTcStages - 1) & 1), failed, status, 760);
-            const uint32_t dst = saddr(ring + (size_t)s * G::kOperand);
-#pragma unroll 4
-            for (int x = id; x < kTcRows * kPer; x += kTcLoaders) {
-                const int r = x / kPer, c = x % kPer, row = r0 + r, tok = row / p.group;
-                const size_t at = row < rows ? ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + row - tok * p.group) * D + 8 * c : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                             ::"r"(dst + (uint32_t)(c / 8) * G::kTile + (uint32_t)r * 128 + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(q + at), "r"(row < rows ? 16 : 0) : "memory");
+            const uint32_t dst = saddr(ring + (size_t)s * G::kOperand) + column;
+            int tok = (r0 + id / kPer) / p.group, head = (r0 + id / kPer) - tok * p.group;
+#pragma unroll 8
+            for (int r = id / kPer; r < kTcRows; r += kStep) {
+                const bool live = r0 + r < rows;
+                const size_t at = live ? ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + head) * D + 8 * c : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (uint32_t)r * 128 + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(q + at), "r"(live ? 16 : 0) : "memory");
+                tok += step_tok;
+                head += step_head;
+                if (head >= p.group) head -= p.group, ++tok;
             }
-            for (int r = id; r < kTcRows; r += kTcLoaders) {
-                const int row = r0 + r;
-                l_s[s][r] = row < rows ? -kLog2e * lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : 0.f;
-            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (id + h * kTcLoaders < kTcRows) l_s[s][id + h * kTcLoaders] = -kLog2e * l_next[h];
+            ask(i + 1);
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (i >= kAhead) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
