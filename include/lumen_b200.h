@@ -375,7 +375,7 @@ int lumen_model_free(lumen_model *m);
  * new token (NULL: its place in the cache, kv_lens[s] - q_lens[s]; another number after an eviction).  causal != 0: a
  * new token sees the cached positions up to its own; 0: all kv_lens[s].  The arrays are HOST arrays and are read
  * during the call, which checks every page number and copies the plan to the device; it may not be made while the
- * context's stream is being captured.  Refused: q_lens[s] > kv_lens[s] with causal (LUMEN_ERR_SHAPE), more positions
+ * context's stream is being captured.  Refused: more than 128 query heads to a key head (LUMEN_ERR_UNSUPPORTED), q_lens[s] > kv_lens[s] with causal (LUMEN_ERR_SHAPE), more positions
  * than the table's pages hold (LUMEN_ERR_KV_OVERFLOW), a page outside the pool or twice in a sequence
  * (LUMEN_ERR_INVALID).  Sequences may share pages that they only read.
  * The calls below allocate nothing and may be captured into graphs; a batch owns the workspace of its attention, so

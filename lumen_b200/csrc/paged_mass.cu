@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------
-constexpr int kTcKeys = 256, kTcRows = 128, kTcLoaders = 96, kTcStages = 4, kTcThreads = 256 + 32 + kTcLoaders;
+constexpr int kTcKeys = 256, kTcRows = 128, kTcLoaders = 64, kTcStages = 4, kTcExps = 512, kTcThreads = kTcExps + 64 + kTcLoaders;
 constexpr int kPolyOf8 = 3;  // pairs of eight whose exponentials go to the FMA pipe
 
 template <int D>
@@ -112,19 +112,21 @@ struct MassGeom {
     static constexpr size_t kSmem = (2 + kTcStages) * (size_t)kOperand + 1024;
 };
 
-// A CTA owns 256 positions of a key head (their keys stay in shared memory) and walks the rows that see any of them, 128 at a time: scores
-// transposed, S^T = K.Q^T, so that a thread holds one position and sums over the columns.  Warps 0-7: exponentials and sums (a
-// warpgroup per 128 positions, two score buffers each); warp 8: products; warps 9-11: queries and log-sums into a ring.
+// A CTA owns 256 positions of a key head (their keys stay in shared memory) and walks the rows that see any of them, up to 128 at a time (as many
+// whole tokens as fit): scores transposed, S^T = K.Q^T, so that a thread holds one position and sums over half of the columns.  Warps 0-15:
+// exponentials and sums (two warpgroups per 128 positions, two score buffers each); warps 16 and 17: products, of 128 positions each;
+// warps 18 and 19: queries (a TMA box of tokens x the heads of the group x 64 numbers) and log-sums into a ring.
 // grid (blocks of 256 positions of the longest sequence, key heads, sequences)
 template <int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
-paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView p, const __nv_bfloat16 *__restrict__ q, float scale, const float *__restrict__ lse,
+paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q, const PagedView p, float scale, const float *__restrict__ lse,
                      DeviceStatus *status) {
     using G = MassGeom<D>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *k_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *ring = k_s + 2 * G::kOperand;
-    __shared__ uint64_t k_bar, q_full[kTcStages], q_free[kTcStages], s_full[2][2], s_free[2][2], quiet;
+    __shared__ uint64_t k_bar, q_full[kTcStages], q_free[kTcStages], s_full[2][2], s_free[2][2], quiet[2];
     __shared__ __align__(16) float l_s[kTcStages][kTcRows];
+    __shared__ float part_s[2][kTcKeys];
     __shared__ uint32_t tmem_base_s;
     __shared__ int failed_s;
     volatile int *failed = &failed_s;
@@ -132,23 +134,31 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * kTcKeys, past = sq.kv_len - sq.q_len;
     if (key0 >= sq.kv_len || rows <= kFewRows) return;
-    const int start = p.causal ? max(0, key0 - past) * p.group : 0, steps = (rows - start + kTcRows - 1) / kTcRows;  // (start < rows: key0 < kv_len)
+    const int per = kTcRows / p.group, n_rows = per * p.group;  // tokens and rows of a step
+    const int start_tok = p.causal ? max(0, key0 - past) : 0, start = start_tok * p.group, steps = (sq.q_len - start_tok + per - 1) / per;  // (start < rows: key0 < kv_len)
     const int tiles = min(2, (sq.kv_len - key0 + 127) / 128);  // of 128 positions
     if (tid == 0) {
         bar_init(&k_bar, 1);
         for (int s = 0; s < kTcStages; ++s) {
-            bar_init(&q_full[s], kTcLoaders);
-            bar_init(&q_free[s], 1 + 32 * 4 * (uint32_t)tiles);
+            bar_init(&q_full[s], kTcLoaders + 1);
+            bar_init(&q_free[s], (1 + kTcExps / 2) * (uint32_t)tiles);
         }
         for (int i = 0; i < 4; ++i) {
             bar_init(&s_full[i >> 1][i & 1], 1);
-            bar_init(&s_free[i >> 1][i & 1], 128);
+            bar_init(&s_free[i >> 1][i & 1], kTcExps / 2);
         }
-        bar_init(&quiet, 1);
+        bar_init(&quiet[0], 1);
+        bar_init(&quiet[1], 1);
         failed_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    // rows of the ring that no query reaches (their columns weigh nothing, but have to be numbers)
+    for (int i = tid; i < kTcStages * (kTcRows - n_rows) * (D / 8); i += kTcThreads) {
+        const int c = i % (D / 8), r = n_rows + i / (D / 8) % (kTcRows - n_rows), s = i / (D / 8) / (kTcRows - n_rows);
+        *reinterpret_cast<uint4 *>(ring + (size_t)s * G::kOperand + (c / 8) * G::kTile + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (warp == kTcExps / 32) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_base_s)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -157,9 +167,10 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_s;  // scores: tile 0 even, odd steps, tile 1 even, odd steps
 
-    if (warp >= 9) {
-        const int id = tid - 288;
-        if (warp == 9) {  // the keys, page by page
+    int q_issued = 0;
+    if (warp >= kTcExps / 32 + 2) {
+        const int id = tid - kTcExps - 64;
+        if (id < 32) {  // the keys, page by page
             const int box = min(1 << p.page_shift, 128), live = min(kTcKeys, sq.kv_len - key0), boxes = (live + box - 1) / box * G::kBlocks;
             const int *table = p.tables + sq.table;
             if (lane == 0) bar_expect(&k_bar, (uint32_t)(boxes * box * kBK * 2));
@@ -170,78 +181,56 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
                             table[pos >> p.page_shift] * p.h_kv + kvh, &k_bar);
             }
         }
-        // Queries by asynchronous copies; a step is announced when its own have landed, behind the request of the next (with more steps between the two, the
-        // announcement would wait for a stage of the ring that the announced step itself has to free).
-        constexpr int kPer = D / 8, kAhead = 1;  // 16-byte pieces of a row
-        auto announce = [&](int i) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            bar_arrive(&q_full[i % kTcStages]);
-        };
-        // A thread has one piece of every kStep-th row; token and head of the next one follow without a division.
-        constexpr int kStep = kTcLoaders / kPer;
-        static_assert(kTcLoaders % kPer == 0, "whole rows");
-        const int c = id % kPer, step_tok = kStep / p.group, step_head = kStep % p.group;
-        const uint32_t column = (uint32_t)(c / 8) * G::kTile;
-        float l_next[2];  // log-sums of the rows id and id + 96 of the next step, asked for a step ahead
+        float l_next[2];  // log-sums of the rows id and id + 64 of the next step, asked for a step ahead (no weight in columns without a row)
         auto ask = [&](int i) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int r = id + h * kTcLoaders, row = start + i * kTcRows + r;
-                l_next[h] = i < steps && r < kTcRows && row < rows ? lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : 0.f;
+                const int r = id + h * kTcLoaders, row = start + i * n_rows + r;
+                l_next[h] = i < steps && r < n_rows && row < rows ? -kLog2e * lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : -INFINITY;
             }
         };
         ask(0);
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
-            const int s = i % kTcStages, r0 = start + i * kTcRows;
-            if (i >= kTcStages) wait_or_failed(&q_free[s], (uint32_t)((i / kTcStages - 1) & 1), failed, status, 760);
-            const uint32_t dst = saddr(ring + (size_t)s * G::kOperand) + column;
-            int tok = (r0 + id / kPer) / p.group, head = (r0 + id / kPer) - tok * p.group;
-#pragma unroll 8
-            for (int r = id / kPer; r < kTcRows; r += kStep) {
-                const bool live = r0 + r < rows;
-                const size_t at = live ? ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + head) * D + 8 * c : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (uint32_t)r * 128 + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(q + at), "r"(live ? 16 : 0) : "memory");
-                tok += step_tok;
-                head += step_head;
-                if (head >= p.group) head -= p.group, ++tok;
+            const int s = i % kTcStages;
+            const bool ok = i < kTcStages || wait_or_failed(&q_free[s], (uint32_t)((i / kTcStages - 1) & 1), failed, status, 760);
+            if (id == 0 && ok) {
+                bar_expect(&q_full[s], (uint32_t)n_rows * kBK * 2 * G::kBlocks);
+#pragma unroll
+                for (int c = 0; c < G::kBlocks; ++c) tma_load_3d(ring + (size_t)s * G::kOperand + c * G::kTile, &map_q, c * kBK, kvh * p.group, sq.tok0 + start_tok + i * per, &q_full[s]);
+                ++q_issued;
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (id + h * kTcLoaders < kTcRows) l_s[s][id + h * kTcLoaders] = -kLog2e * l_next[h];
+            for (int h = 0; h < 2; ++h) l_s[s][id + h * kTcLoaders] = l_next[h];
+            bar_arrive(&q_full[s]);
             ask(i + 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (i >= kAhead) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-                announce(i - kAhead);
-            }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (int i = max(0, steps - kAhead); i < steps; ++i) announce(i);
-    } else if (warp == 8) {
-        wait_warp(&k_bar, 0, failed, status, 761);
-        const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), k0 = __shfl_sync(0xffffffffu, saddr(k_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
+    } else if (warp >= kTcExps / 32) {
+        const int kt = warp - kTcExps / 32;
+        if (kt < tiles) {
+            wait_warp(&k_bar, 0, failed, status, 761);
+            const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0) + (uint32_t)kt * 256, k0 = __shfl_sync(0xffffffffu, saddr(k_s), 0) + kt * G::kOperand,
+                           ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
 #pragma unroll 1
-        for (int i = 0; i < steps; ++i) {
-            const int s = i % kTcStages, b = i & 1;
-            const bool ok = wait_warp(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 762);
-            for (int kt = 0; kt < tiles; ++kt) {
-                const bool free = i < 2 || wait_warp(&s_free[kt][b], (uint32_t)((i / 2 - 1) & 1), failed, status, 763);
+            for (int i = 0; i < steps; ++i) {
+                const int s = i % kTcStages, b = i & 1;
+                const bool ok = wait_warp(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 762) &&
+                                (i < 2 || wait_warp(&s_free[kt][b], (uint32_t)((i / 2 - 1) & 1), failed, status, 763));
                 tc_after();
-                if (ok && free) {
-                    const uint64_t kd = smem_desc(k0 + kt * G::kOperand), qd = smem_desc(ring0 + (uint32_t)s * G::kOperand);
+                if (ok) {
+                    const uint64_t kd = smem_desc(k0), qd = smem_desc(ring0 + (uint32_t)s * G::kOperand);
 #pragma unroll
                     for (int kb = 0; kb < G::kBlocks; ++kb)
 #pragma unroll
                         for (int kk = 0; kk < kBK / 16; ++kk)
-                            mma_ss(acc0 + (uint32_t)(kt * 256 + b * 128), kd + kb * (G::kTile >> 4) + 2 * kk, qd + kb * (G::kTile >> 4) + 2 * kk, idesc_bf16(128, 128), kb + kk > 0);
+                            mma_ss(acc0 + (uint32_t)(b * 128), kd + kb * (G::kTile >> 4) + 2 * kk, qd + kb * (G::kTile >> 4) + 2 * kk, idesc_bf16(128, 128), kb + kk > 0);
                 }
                 commit_one(&s_full[kt][b]);
+                commit_one(&q_free[s]);
             }
-            commit_one(&q_free[s]);
         }
     } else {
-        const int kt = warp >> 2, key = key0 + 128 * kt + (tid & 127);
+        const int kt = (warp >> 2) & 1, half = warp >> 3, key = key0 + 128 * kt + (tid & 127);
         if (kt < tiles) {
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const float scale2 = scale * kLog2e;
@@ -251,26 +240,26 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
             const int key_max = key0 + 128 * kt + (warp & 3) * 32 + 31;
 #pragma unroll 1
             for (int i = 0; i < steps; ++i) {
-                const int s = i % kTcStages, b = i & 1, r0 = start + i * kTcRows;
+                const int s = i % kTcStages, b = i & 1, r0 = start + i * n_rows;
                 wait_first(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 764);  // the log-sums
                 wait_first(&s_full[kt][b], (uint32_t)((i / 2) & 1), failed, status, 765);
                 __syncwarp();
                 tc_after();
-                uint32_t x[4][32];
+                uint32_t x[2][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_issue(tmem + lanes + (uint32_t)(kt * 256 + b * 128 + 32 * c), x[c]);
+                for (int c = 0; c < 2; ++c) tmem_ld32_issue(tmem + lanes + (uint32_t)(kt * 256 + b * 128 + 64 * half + 32 * c), x[c]);
                 tmem_ld_wait();
                 tc_before();
                 bar_arrive(&s_free[kt][b]);
-                const bool masked = r0 + kTcRows > rows || (p.causal && past + r0 / p.group < key_max);
-                const int lo = first - r0, hi = rows - r0;
+                const bool masked = r0 + n_rows > rows || (p.causal && past + r0 / p.group < key_max);
+                const int lo = first - r0 - 64 * half, hi = rows - r0 - 64 * half;
                 // (of eight pairs, kPolyOf8 go to the FMA pipe; masked ones are not added)
                 auto add = [&](auto poly) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
-                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&l_s[s][32 * c + e]);
+                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&l_s[s][64 * half + 32 * c + e]);
 #pragma unroll
                             for (int u = 0; u < 2; ++u) {
                                 const int col = 32 * c + e + 2 * u;
@@ -297,17 +286,22 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedView 
             }
             float s0, s1;
             apart(add2(sum[0], sum[1]), s0, s1);
-            if (key < sq.kv_len && !*failed) p.mass[paged_row(p, p.tables + sq.table, kvh, key)] += s0 + s1;
+            part_s[half][128 * kt + (tid & 127)] = s0 + s1;
         }
     }
     __syncthreads();
+    if (tid < kTcKeys && key0 + tid < sq.kv_len && !*failed) p.mass[paged_row(p, p.tables + sq.table, kvh, key0 + tid)] += part_s[0][tid] + part_s[1][tid];
     if (*failed) {
-        if (tid == 288) drain_ring(&k_bar, 1, 1);  // a wait gave up
-        else if (tid == 256) drain_mmas(&quiet);
+        if (tid == kTcExps + 64) {  // a wait gave up
+            drain_ring(&k_bar, 1, 1);
+            drain_ring(q_full, kTcStages, q_issued);
+        } else if (tid == kTcExps || tid == kTcExps + 32) {
+            drain_mmas(&quiet[(tid - kTcExps) / 32]);
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == kTcExps / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ---- 32 bits --------------------------------------------------------------------------------------------------------------
@@ -392,8 +386,11 @@ int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUten
             LUMEN_LAUNCHED(ctx);
         }
         if (a.max_rows > kFewRows) {
+            CUtensorMap q_map;
+            const size_t row = (size_t)all.n_head * D;
+            LUMEN_TRY(make_map_3d(ctx, &q_map, q, D, (size_t)all.n_head, D, (size_t)all.tokens, row, all.group, kTcRows / all.group));
             LUMEN_TRY(allow_smem(ctx, paged_mass_tc_kernel<D>, MassGeom<D>::kSmem));
-            paged_mass_tc_kernel<D><<<grid_of(a, v, kTcKeys, n), kTcThreads, MassGeom<D>::kSmem, s>>>(k_map, v, q, a.scale, a.lse, ctx->d_status);
+            paged_mass_tc_kernel<D><<<grid_of(a, v, kTcKeys, n), kTcThreads, MassGeom<D>::kSmem, s>>>(k_map, q_map, v, a.scale, a.lse, ctx->d_status);
             LUMEN_LAUNCHED(ctx);
         }
     }
