@@ -126,10 +126,14 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
             return set_error(ctx, rc, "page_batch: %s", why.c_str());
         }
         PagedPlan &p = b->plan;
-        std::vector<int> live;
-        for (int s = 0; s < p.n_seq; ++s)
-            if (p.seqs[(size_t)s].q_len) live.push_back(s);
-        paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, ctx->num_sms) : paged_rows_shape(b->g, ctx->num_sms), live);
+        std::vector<int> few, many;
+        for (int s = 0; s < p.n_seq; ++s) {
+            const int rows = p.seqs[(size_t)s].q_len * p.group;
+            if (rows) (b->g.dtype == LUMEN_F32 && rows <= kPagedFewRows ? few : many).push_back(s);
+        }
+        paged_cut(p, b->g, paged_rows_shape(b->g, ctx->num_sms), few);
+        b->n_few = (int)p.items.size();
+        paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, ctx->num_sms) : paged_f32_shape(ctx->num_sms), many);
         // everything the kernels read goes up in one copy, in front of the workspace
         std::vector<char> up;
         auto put = [&](const void *data, size_t bytes) {
@@ -225,13 +229,20 @@ int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *b
     OnDevice on(ctx);
     PagedAttnArgs a = {};
     a.q = q_dev; a.scale = scale; a.out = out_dev; a.out_dtype = out_dtype; a.lse = lse_dev;
-    a.items = batch->items; a.n_items = (int)p.items.size();
-    for (const PagedItem &it : p.items) a.max_rows = std::max(a.max_rows, it.rows);
     a.part = batch->part; a.part_rows = p.part_rows; a.joins = batch->joins; a.n_joins = (int)p.joins.size();
     for (const PagedJoin &j : p.joins) a.join_rows = std::max(a.join_rows, j.rows);
     const PagedView v = view_of(pool, batch);
-    LUMEN_TRY(pool->g.dtype == LUMEN_BF16 ? launch_paged_attn_tc(ctx, pool->g, v, pool->k_map, pool->v_map, a, ctx->stream)
-                                          : launch_paged_rows(ctx, pool->g, v, a, ctx->stream));
+    for (int many = 0; many < 2; ++many) {
+        const int first = many ? batch->n_few : 0, last = many ? (int)p.items.size() : batch->n_few;
+        if (first == last) continue;
+        a.items = batch->items + first;
+        a.n_items = last - first;
+        a.max_rows = 0;
+        for (int i = first; i < last; ++i) a.max_rows = std::max(a.max_rows, p.items[(size_t)i].rows);
+        LUMEN_TRY(!many ? launch_paged_rows(ctx, pool->g, v, a, ctx->stream)
+                  : pool->g.dtype == LUMEN_F32 ? launch_paged_attn_f32(ctx, pool->g, v, a, ctx->stream)
+                                               : launch_paged_attn_tc(ctx, pool->g, v, pool->k_map, pool->v_map, a, ctx->stream));
+    }
     return a.n_joins ? launch_paged_join(ctx, pool->g, v, a, ctx->stream) : LUMEN_OK;
 }
 

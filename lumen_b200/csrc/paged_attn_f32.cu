@@ -1,0 +1,351 @@
+// Attention of many rows over a paged cache of 32 bits on the 5th-generation tensor cores, with all 24 bits.
+//
+// A 32-bit number is the sum of three bf16 numbers, x = hi + mid + lo (each the rounded rest of the ones before; the rest behind the third is
+// below 2^-24 |x|).  Of the nine products of two such sums the six largest are computed; what is left out is below 2^-24 as well.  They are
+// accumulated smallest first, so that a tile's sums are rounded at full size only in the last of them, and the results of a
+// tile are added to the running sums in registers, not in tensor memory.
+//
+// A CTA takes an item: up to 128 rows of one key head (a row is one new token and one of the query heads that read this key head) against a range
+// of positions in tiles of 64.  Warpgroups 0 and 1: weights, two threads a row (32 scores and half of the numbers each); warpgroup 2:
+// keys and values from the pages into registers (a tile ahead), split, into shared memory in the layout of the tensor cores; warpgroup 3: one warp
+// issues S = Q.K^T (the next tile's while this one's weights are computed) and O = P.V, P from tensor memory, V as it lies in the
+// cache.  Bound by the six products.
+//
+// Every wait is bounded; a wait that gives up records LUMEN_ERR_TIMEOUT, the roles run on without acting, products in flight are waited for,
+// tensor memory is freed and the CTA returns.
+#include "paged.cuh"
+#include "paged_tc.cuh"
+
+namespace lumen {
+namespace {
+
+using namespace tc;
+
+constexpr int kRowsTile = 128, kKeys = 64, kTerms = 3, kThreads = 512;
+// (launched with 128 registers a thread; the warpgroup that holds a tile in flight takes more from the one that issues the products: 2 x 128 + 184 + 72)
+constexpr int kRegsLoad = 184, kRegsIssue = 72;
+
+template <int D>
+struct SplitGeom {
+    static constexpr int kBlocks = D / kBK;
+    static constexpr uint32_t kQTile = kRowsTile * kBK * 2, kQTerm = kBlocks * kQTile;
+    static constexpr uint32_t kTile = kKeys * kBK * 2, kTerm = kBlocks * kTile;  // of keys or values
+    static constexpr uint32_t kStage = 2 * kTerms * kTerm;
+    static constexpr int kStages = D == 128 ? 1 : 2;
+    static constexpr size_t kSmem = kTerms * (size_t)kQTerm + kStages * (size_t)kStage + 1024;
+    // tensor memory: scores of even and odd tiles, weights (hi, mid, lo: 32 columns each), O of even and odd tiles
+    static constexpr uint32_t kP = 2 * kKeys, kO = kP + kTerms * kKeys / 2 + 32;
+    static constexpr uint32_t kIdescS = idesc_bf16(kRowsTile, kKeys), kIdescO = idesc_bf16(kRowsTile, D) | (1u << 16);
+    static constexpr int kPieces = kKeys * D / 8 / 128;  // 8 numbers each, of a loading thread and tile
+};
+
+// Products (first term, second term), smallest first.
+__device__ constexpr int kFirst[6] = {2, 0, 1, 1, 0, 0}, kSecond[6] = {0, 2, 1, 0, 1, 0};
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next_block) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next_block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Two numbers as three pairs of bf16.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&t)[kTerms]) {
+    t[0] = pack_bf16(a, b);
+    a -= __uint_as_float(t[0] << 16);
+    b -= __uint_as_float(t[0] & 0xffff0000u);
+    t[1] = pack_bf16(a, b);
+    t[2] = pack_bf16(a - __uint_as_float(t[1] << 16), b - __uint_as_float(t[1] & 0xffff0000u));
+}
+// Eight numbers of a row into the three terms' tiles: `at` is the place of the 16-byte piece in the first.
+__device__ __forceinline__ void split_store(const float4 &x, const float4 &y, unsigned char *at, uint32_t term) {
+    uint32_t t[4][kTerms];
+    split3(x.x, x.y, t[0]);
+    split3(x.z, x.w, t[1]);
+    split3(y.x, y.y, t[2]);
+    split3(y.z, y.w, t[3]);
+#pragma unroll
+    for (int i = 0; i < kTerms; ++i) *reinterpret_cast<uint4 *>(at + i * term) = make_uint4(t[0][i], t[1][i], t[2][i], t[3][i]);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const PagedView p, const PagedAttnArgs a, DeviceStatus *status) {
+    using G = SplitGeom<D>;
+    constexpr int kStages = G::kStages, kDH = D / 2;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *ring = q_s + kTerms * G::kQTerm;
+    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[2], p_bar, o_bar, quiet;
+    __shared__ float xch[2][kRowsTile];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int failed_s;
+    volatile int *failed = &failed_s;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const PagedItem it = a.items[blockIdx.x];
+    const PagedSeq sq = p.seqs[it.seq];
+    const int past = sq.kv_len - sq.q_len, nt = (it.key1 - it.key0 + kKeys - 1) / kKeys;
+    if (tid == 0) {
+        bar_init(&q_bar, 384);
+        for (int s = 0; s < kStages; ++s) {
+            bar_init(&k_full[s], 128);
+            bar_init(&v_full[s], 128);
+            bar_init(&k_free[s], 1);
+            bar_init(&v_free[s], 1);
+        }
+        bar_init(&s_bar[0], 1);
+        bar_init(&s_bar[1], 1);
+        bar_init(&p_bar, 256);
+        bar_init(&o_bar, 1);
+        bar_init(&quiet, 1);
+        failed_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_base_s)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_base_s;
+    auto load_queries = [&](int id, int n) {  // split, in the swizzled layout; rows behind the item's: zeros
+        for (int i = id; i < kRowsTile * (D / 8); i += n) {
+            const int r = i / (D / 8), c = i % (D / 8);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (r < it.rows) {
+                const int g = it.row0 + r;
+                const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) +
+                                                                     ((size_t)(sq.tok0 + g / p.group) * p.n_head + it.kvh * p.group + g % p.group) * D + 8 * c);
+                x = src[0];
+                y = src[1];
+            }
+            split_store(x, y, q_s + (c / 8) * G::kQTile + r * 128 + (((c & 7) ^ (r & 7)) << 4), G::kQTerm);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        bar_arrive(&q_bar);
+    };
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (warp == 12 && nt > 0) {
+            wait_warp(&q_bar, 0, failed, status, 800);
+            tc_after();
+            const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, saddr(q_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
+            auto scores = [&](int j) {
+                const int s = j % kStages;
+                if (wait_warp(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 801)) {
+                    tc_after();
+                    const uint64_t qd = smem_desc(q0), kd = smem_desc(ring0 + (uint32_t)s * G::kStage);
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int kb = 0; kb < G::kBlocks; ++kb)
+#pragma unroll
+                            for (int kk = 0; kk < kBK / 16; ++kk)
+                                mma_ss(acc0 + (uint32_t)((j & 1) * kKeys), qd + ((kFirst[x] * G::kQTerm + kb * G::kQTile) >> 4) + 2 * kk,
+                                       kd + ((kSecond[x] * G::kTerm + kb * G::kTile) >> 4) + 2 * kk, G::kIdescS, x + kb + kk > 0);
+                }
+                commit_one(&s_bar[j & 1]);
+                commit_one(&k_free[s]);
+            };
+            scores(0);
+#pragma unroll 1
+            for (int j = 0; j < nt; ++j) {
+                // (its buffer was read for tile j - 1, whose weights were announced before that tile's product)
+                if (j + 1 < nt) scores(j + 1);
+                const int s = j % kStages;
+                bool ok = wait_warp(&p_bar, (uint32_t)(j & 1), failed, status, 802);
+                if (ok) ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 803);
+                tc_after();
+                if (ok) {
+                    const uint64_t vd = desc_mn(ring0 + (uint32_t)s * G::kStage + kTerms * G::kTerm, G::kTile);
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int kk = 0; kk < kKeys / 16; ++kk)
+                            mma_ts(acc0 + G::kO + (uint32_t)((j & 1) * D), acc0 + G::kP + (uint32_t)(kFirst[x] * (kKeys / 2) + 8 * kk),
+                                   vd + ((kSecond[x] * G::kTerm + kk * 2048) >> 4), G::kIdescO, x + kk > 0);
+                }
+                commit_one(&o_bar);
+                commit_one(&v_free[s]);
+            }
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+        // ---- keys and values: a thread has one piece of 8 numbers of every kStep-th position ----
+        constexpr int kStep = 128 / (D / 8);
+        const int id = tid - 256, c = id % (D / 8), r0 = id / (D / 8);
+        const int *table = p.tables + sq.table;
+        float4 k[G::kPieces][2], v[G::kPieces][2];
+        auto fetch = [&](const void *pool, int j, float4 (&x)[G::kPieces][2]) {
+#pragma unroll
+            for (int i = 0; i < G::kPieces; ++i) {
+                const int pos = it.key0 + j * kKeys + r0 + i * kStep;
+                x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);  // (behind the end: zeros, which meet weights of zero)
+                if (pos < it.key1) {
+                    const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(pool) + paged_row(p, table, it.kvh, pos) * D + 8 * c);
+                    x[i][0] = __ldg(src);
+                    x[i][1] = __ldg(src + 1);
+                }
+            }
+        };
+        auto put = [&](const float4 (&x)[G::kPieces][2], unsigned char *dst) {
+#pragma unroll
+            for (int i = 0; i < G::kPieces; ++i) {
+                const int r = r0 + i * kStep;
+                split_store(x[i][0], x[i][1], dst + (c / 8) * G::kTile + r * 128 + (((c & 7) ^ (r & 7)) << 4), G::kTerm);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        if (nt > 0) {
+            fetch(p.k, 0, k);
+            fetch(p.v, 0, v);
+        }
+        load_queries(256 + id, 384);
+#pragma unroll 1
+        for (int j = 0; j < nt; ++j) {
+            const int s = j % kStages;
+            unsigned char *st = ring + (size_t)s * G::kStage;
+            const uint32_t par = (uint32_t)((j / kStages - 1) & 1);
+            if (j >= kStages) wait_first(&k_free[s], par, failed, status, 810);
+            put(k, st);
+            bar_arrive(&k_full[s]);
+            if (j + 1 < nt) fetch(p.k, j + 1, k);
+            if (j >= kStages) wait_first(&v_free[s], par, failed, status, 811);
+            put(v, st + kTerms * G::kTerm);
+            bar_arrive(&v_full[s]);
+            if (j + 1 < nt) fetch(p.v, j + 1, v);
+        }
+    } else {
+        load_queries(tid, 384);
+        // ---- weights: thread (row, half) has 32 of the tile's 64 scores and half of the row's numbers ----
+        const int row = tid & 127, half = tid >> 7, quad = warp & 3, r = min(row, it.rows - 1);
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const float scale2 = a.scale * kLog2e;
+        const int t = (it.row0 + r) / p.group, end = p.causal ? min(it.key1, past + t + 1) : it.key1;
+        const int end_min = p.causal ? min(it.key1, past + it.row0 / p.group + 1) : it.key1;
+        float ctx[kDH], m = -INFINITY, l = 0.f, r_prev = 0.f;
+#pragma unroll
+        for (int e = 0; e < kDH; ++e) ctx[e] = 0.f;
+        auto fold = [&](int j, float f) {  // ctx = ctx * f + O of tile j
+#pragma unroll
+            for (int x = 0; x < kDH / 32; ++x) {
+                uint32_t o[32];
+                tmem_ld32(tmem + lanes + G::kO + (uint32_t)((j & 1) * D + half * kDH + 32 * x), o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) ctx[32 * x + e] = fmaf(ctx[32 * x + e], f, __uint_as_float(o[e]));
+            }
+        };
+#pragma unroll 1
+        for (int j = 0; j < nt; ++j) {
+            wait_first(&s_bar[j & 1], (uint32_t)((j >> 1) & 1), failed, status, 820);
+            __syncwarp();
+            tc_after();
+            uint32_t s[32];
+            tmem_ld32(tmem + lanes + (uint32_t)((j & 1) * kKeys + 32 * half), s);
+            const int tile0 = it.key0 + j * kKeys, lim = end - tile0 - 32 * half;
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * scale2);
+            if (tile0 + kKeys > end_min) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (e >= lim) s[e] = 0xff800000u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[e]));
+            // the other half's maximum: warps w and w + 4 (one barrier behind the writes, one behind the reads)
+            xch[half][row] = top;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+            const float next = fmaxf(m, fmaxf(top, xch[half ^ 1][row])), base = next == -INFINITY ? 0.f : next, f = ex2(m - base);
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+            m = next;
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const float w = ex2(__uint_as_float(s[e]) - base);
+                s[e] = __float_as_uint(w);
+                sum[e & 1] += w;
+            }
+            l = fmaf(l, f, sum[0] + sum[1]);
+            if (j > 0) {  // the weights' place is free once the product before is complete
+                wait_first(&o_bar, (uint32_t)((j - 1) & 1), failed, status, 821);
+                __syncwarp();
+                tc_after();
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t w[kTerms][8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    uint32_t t3[kTerms];
+                    split3(__uint_as_float(s[16 * x + 2 * e]), __uint_as_float(s[16 * x + 2 * e + 1]), t3);
+#pragma unroll
+                    for (int i = 0; i < kTerms; ++i) w[i][e] = t3[i];
+                }
+#pragma unroll
+                for (int i = 0; i < kTerms; ++i) tmem_st8(tmem + lanes + G::kP + (uint32_t)(i * (kKeys / 2) + 16 * half + 8 * x), w[i]);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_before();
+            bar_arrive(&p_bar);
+            if (j > 0) {  // while this tile's product runs (its O is the other one)
+                fold(j - 1, r_prev);
+                tc_before();
+            }
+            r_prev = f;
+        }
+        if (nt > 0) {
+            wait_first(&o_bar, (uint32_t)((nt - 1) & 1), failed, status, 822);
+            __syncwarp();
+            tc_after();
+            fold(nt - 1, r_prev);
+            tc_before();
+        }
+        xch[half][row] = l;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+        l += xch[half ^ 1][row];
+        if (row < it.rows && !*failed) {
+            const bool part = it.part >= 0;
+            const float inv = part ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+            const size_t o = part ? (size_t)it.part + row : (size_t)(sq.tok0 + t) * p.n_head + it.kvh * p.group + (it.row0 + row) % p.group;
+            float *dst = (part ? a.part : static_cast<float *>(a.out)) + o * D + half * kDH;
+#pragma unroll
+            for (int e = 0; e < kDH; e += 4) *reinterpret_cast<float4 *>(dst + e) = make_float4(ctx[e] * inv, ctx[e + 1] * inv, ctx[e + 2] * inv, ctx[e + 3] * inv);
+            if (half == 0) {
+                if (part) *reinterpret_cast<float2 *>(a.part + (size_t)a.part_rows * D + 2 * o) = make_float2(m, l);
+                else if (a.lse) a.lse[o] = m * 0.6931471805599453f + logf(l);
+            }
+        }
+    }
+    __syncthreads();
+    if (*failed && tid == 384) drain_mmas(&quiet);  // a wait gave up
+    tc_before();
+    __syncthreads();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <int D>
+int launch(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
+    using G = SplitGeom<D>;
+    static_assert(G::kSmem <= 226 * 1024 && G::kO + 2 * D <= 512, "fits shared and tensor memory");
+    static const int regs = [] {  // (what the warpgroups trade has to be there)
+        cudaFuncAttributes attr;
+        return cudaFuncGetAttributes(&attr, paged_attn_f32_kernel<D>) == cudaSuccess ? attr.numRegs : 0;
+    }();
+    if (regs * kThreads < (2 * 128 + kRegsLoad + kRegsIssue) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention: kernel built with %d registers", regs);
+    LUMEN_TRY(allow_smem(ctx, paged_attn_f32_kernel<D>, G::kSmem));
+    paged_attn_f32_kernel<D><<<(unsigned)a.n_items, kThreads, G::kSmem, s>>>(v, a, ctx->d_status);
+    LUMEN_LAUNCHED(ctx);
+    return LUMEN_OK;
+}
+
+}  // namespace
+
+PagedShape paged_f32_shape(int num_sms) { return {kRowsTile, kKeys, num_sms}; }
+
+int launch_paged_attn_f32(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
+    return g.d == 64 ? launch<64>(ctx, v, a, s) : launch<128>(ctx, v, a, s);
+}
+
+}  // namespace lumen

@@ -1,4 +1,4 @@
-// Attention of few rows over a paged cache, in 32-bit arithmetic, and the join of partial results.
+// Attention of few rows over a paged cache of 32 bits, in 32-bit arithmetic, and the join of partial results.
 //
 // o = sum_j 2^(s_j - m) v_j / l with s_j = scale * log2(e) * q . k_j, the running maximum m and sum l = sum_j 2^(s_j - m) of every row (a row
 // is one new token and one of the query heads of a key head).  A CTA takes an item: up to RT rows of one key head against a range of
@@ -33,15 +33,9 @@ __device__ __forceinline__ void four(const float *p, float (&v)[4]) {
     const float4 x = *reinterpret_cast<const float4 *>(p);
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
 }
-__device__ __forceinline__ void four(const __nv_bfloat16 *p, float (&v)[4]) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(p);
-    v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
-    v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
-}
-
-template <typename T, int D, int RT>
+template <int D, int RT>
 struct RowsSmem {
-    static constexpr int kRow = D * (int)sizeof(T) + 16;  // bytes between rows of a tile: 8 rows at one column lie in 8 different groups of banks
+    static constexpr int kRow = D * 4 + 16;  // bytes between rows of a tile: 8 rows at one column lie in 8 different groups of banks
     static constexpr int kTile = kKeys * kRow;
     static constexpr int kQ = 4 * kTile;                       // f32 queries [RT][D]
     static constexpr int kS = kQ + RT * D * 4;                 // scores [RT][kKeys + 1]
@@ -51,10 +45,10 @@ struct RowsSmem {
     static constexpr int kBytes = kRowOff + 2 * kKeys * 8;
 };
 
-template <typename T, int D, int RT>
+template <int D, int RT>
 __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedView p, const PagedAttnArgs a) {
-    using G = RowsSmem<T, D, RT>;
-    constexpr int kParts = D * (int)sizeof(T) / 16;  // 16-byte pieces of a row
+    using G = RowsSmem<D, RT>;
+    constexpr int kParts = D * 4 / 16;  // 16-byte pieces of a row
     extern __shared__ __align__(16) unsigned char smem[];
     float *q_s = reinterpret_cast<float *>(smem + G::kQ), *s_s = reinterpret_cast<float *>(smem + G::kS), *p_s = reinterpret_cast<float *>(smem + G::kP);
     float *fac = reinterpret_cast<float *>(smem + G::kF), *mx = fac + RT, *sum = mx + RT;
@@ -72,7 +66,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedView p,
     for (int i = tid; i < RT * (D / 4); i += kThreads) {
         const int r = i / (D / 4), e = i % (D / 4) * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < it.rows) four(static_cast<const T *>(a.q) + ((size_t)token(r) * p.n_head + head(r)) * D + e, v);
+        if (r < it.rows) four(static_cast<const float *>(a.q) + ((size_t)token(r) * p.n_head + head(r)) * D + e, v);
         *reinterpret_cast<float4 *>(q_s + r * D + e) = make_float4(v[0], v[1], v[2], v[3]);
     }
     if (tid < RT) mx[tid] = -INFINITY, sum[tid] = 0.f;
@@ -87,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedView p,
         for (int i = tid; i < kKeys * kParts; i += kThreads) {
             const int r = i / kParts, c = i % kParts * 16;
             const long long at = at_s[(j & 1) * kKeys + r];
-            const size_t off = at < 0 ? 0 : (size_t)at * D * sizeof(T) + c;
+            const size_t off = at < 0 ? 0 : (size_t)at * D * 4 + c;
             cp16(kt + r * G::kRow + c, static_cast<const char *>(p.k) + off, at >= 0);  // (behind the end: zeros)
             cp16(vt + r * G::kRow + c, static_cast<const char *>(p.v) + off, at >= 0);
         }
@@ -123,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedView p,
             float s[RH];
 #pragma unroll
             for (int r = 0; r < RH; ++r) s[r] = 0.f;
-            const T *kr = reinterpret_cast<const T *>(kt + key * G::kRow);
+            const float *kr = reinterpret_cast<const float *>(kt + key * G::kRow);
 #pragma unroll 4
             for (int e = 0; e < D; e += 4) {
                 float k4[4];
@@ -176,16 +170,13 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedView p,
 #pragma unroll 4
                 for (int i = 0; i < kKeys / 4; ++i) {
                     const int key = warp * (kKeys / 4) + i;
-                    const T *vr = reinterpret_cast<const T *>(vt + key * G::kRow) + lane * E;
+                    const float *vr = reinterpret_cast<const float *>(vt + key * G::kRow) + lane * E;
                     float v[E];
                     if constexpr (E == 4) {
                         four(vr, v);
-                    } else if constexpr (sizeof(T) == 4) {
+                    } else {
                         const float2 x = *reinterpret_cast<const float2 *>(vr);
                         v[0] = x.x; v[1] = x.y;
-                    } else {
-                        const uint32_t x = *reinterpret_cast<const uint32_t *>(vr);
-                        v[0] = __uint_as_float(x << 16); v[1] = __uint_as_float(x & 0xffff0000u);
                     }
 #pragma unroll
                     for (int r = 0; r < RT; r += 4) {
@@ -230,12 +221,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedView p,
         }
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const size_t o = (size_t)token(r) * p.n_head + head(r);
-        if (a.out_dtype == LUMEN_F32) {
-            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + o * D + e) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-        } else {
-            __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v[0] * inv, v[1] * inv), __floats2bfloat162_rn(v[2] * inv, v[3] * inv)};
-            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(a.out) + o * D + e) = *reinterpret_cast<uint2 *>(b);
-        }
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + o * D + e) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
         if (e == 0 && a.lse) a.lse[o] = m * 0.6931471805599453f + logf(l);
     }
 }
@@ -276,29 +262,28 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedView p, cons
     if (lane == 0 && a.lse) a.lse[o] = top * 0.6931471805599453f + logf(l);
 }
 
-template <typename T, int D, int RT>
+template <int D, int RT>
 int launch(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
-    constexpr size_t bytes = RowsSmem<T, D, RT>::kBytes;
-    LUMEN_TRY(allow_smem(ctx, paged_rows_kernel<T, D, RT>, bytes));
-    paged_rows_kernel<T, D, RT><<<(unsigned)a.n_items, kThreads, bytes, s>>>(v, a);
+    constexpr size_t bytes = RowsSmem<D, RT>::kBytes;
+    LUMEN_TRY(allow_smem(ctx, paged_rows_kernel<D, RT>, bytes));
+    paged_rows_kernel<D, RT><<<(unsigned)a.n_items, kThreads, bytes, s>>>(v, a);
     LUMEN_LAUNCHED(ctx);
     return LUMEN_OK;
 }
-template <typename T, int D>
+template <int D>
 int pick(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
-    return a.max_rows <= 4 ? launch<T, D, 4>(ctx, v, a, s) : a.max_rows <= 8 ? launch<T, D, 8>(ctx, v, a, s) : launch<T, D, 16>(ctx, v, a, s);
+    return a.max_rows <= 4 ? launch<D, 4>(ctx, v, a, s) : a.max_rows <= 8 ? launch<D, 8>(ctx, v, a, s) : launch<D, 16>(ctx, v, a, s);
 }
 
 }  // namespace
 
 PagedShape paged_rows_shape(const PagedGeom &g, int num_sms) {
-    const int bytes = g.d * (g.dtype == LUMEN_F32 ? 4 : 2) * kKeys * 4;  // the tiles: what limits the CTAs of an SM
-    return {16, kKeys, num_sms * (bytes > 100 * 1024 ? 1 : bytes > 50 * 1024 ? 2 : 4)};
+    const int bytes = g.d * 4 * kKeys * 4;  // the tiles: what limits the CTAs of an SM
+    return {16, kKeys, num_sms * (bytes > 100 * 1024 ? 1 : 2)};
 }
 
 int launch_paged_rows(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
-    if (g.dtype == LUMEN_F32) return g.d == 64 ? pick<float, 64>(ctx, v, a, s) : pick<float, 128>(ctx, v, a, s);
-    return g.d == 64 ? pick<__nv_bfloat16, 64>(ctx, v, a, s) : pick<__nv_bfloat16, 128>(ctx, v, a, s);
+    return g.d == 64 ? pick<64>(ctx, v, a, s) : pick<128>(ctx, v, a, s);
 }
 
 int launch_paged_join(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
