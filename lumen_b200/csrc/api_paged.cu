@@ -129,9 +129,9 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         std::vector<int> few, many;
         for (int s = 0; s < p.n_seq; ++s) {
             const int rows = p.seqs[(size_t)s].q_len * p.group;
-            if (rows) (b->g.dtype == LUMEN_F32 && rows <= kPagedFewRows ? few : many).push_back(s);
+            if (rows) (rows <= kPagedFewRows ? few : many).push_back(s);
         }
-        paged_cut(p, b->g, paged_rows_shape(b->g, ctx->num_sms), few);
+        paged_cut(p, b->g, paged_few_shape(ctx->num_sms), few);
         b->n_few = (int)p.items.size();
         paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, ctx->num_sms) : paged_f32_shape(ctx->num_sms), many);
         // everything the kernels read goes up in one copy, in front of the workspace
@@ -239,7 +239,7 @@ int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *b
         a.n_items = last - first;
         a.max_rows = 0;
         for (int i = first; i < last; ++i) a.max_rows = std::max(a.max_rows, p.items[(size_t)i].rows);
-        LUMEN_TRY(!many ? launch_paged_rows(ctx, pool->g, v, a, ctx->stream)
+        LUMEN_TRY(!many ? launch_paged_few(ctx, pool->g, v, a, ctx->stream)
                   : pool->g.dtype == LUMEN_F32 ? launch_paged_attn_f32(ctx, pool->g, v, a, ctx->stream)
                                                : launch_paged_attn_tc(ctx, pool->g, v, pool->k_map, pool->v_map, a, ctx->stream));
     }

@@ -23,7 +23,7 @@ struct lumen_page_batch {
     int *tables = nullptr, *tok_slot = nullptr, *tok_pos = nullptr;
     lumen::PagedItem *items = nullptr;
     lumen::PagedJoin *joins = nullptr;
-    int n_few = 0;          // items that the kernel for few rows takes (f32); the others follow
+    int n_few = 0;          // items that the kernel for few rows takes; the others follow
     float *part = nullptr;  // partial sums [part_rows, d], then their maxima and sums [part_rows, 2]
 };
 
@@ -65,13 +65,12 @@ struct PagedAttnArgs {
     const PagedJoin *joins;
     int n_joins, join_rows;
 };
-// f32 pools: few rows of a key head (paged_rows.cu), and more (paged_attn_f32.cu)
-constexpr int kPagedFewRows = 32;
-PagedShape paged_rows_shape(const PagedGeom &g, int num_sms);
+// Few rows of a key head (paged_few.cu); more from f32 pools (paged_attn_f32.cu), and from bf16 pools (paged_attn_tc.cu)
+constexpr int kPagedFewRows = 16;
+PagedShape paged_few_shape(int num_sms);
+int launch_paged_few(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
 PagedShape paged_f32_shape(int num_sms);
 int launch_paged_attn_f32(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
-int launch_paged_rows(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
-// bf16 pools (paged_attn_tc.cu)
 PagedShape paged_tc_shape(int max_rows, int num_sms);
 int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *mem, int most, CUtensorMap *map);
 int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap (&k_map)[2], const CUtensorMap (&v_map)[2], const PagedAttnArgs &a,
