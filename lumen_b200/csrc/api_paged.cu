@@ -230,7 +230,7 @@ int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *b
     PagedAttnArgs a = {};
     a.q = q_dev; a.scale = scale; a.out = out_dev; a.out_dtype = out_dtype; a.lse = lse_dev;
     a.part = batch->part; a.part_rows = p.part_rows; a.joins = batch->joins; a.n_joins = (int)p.joins.size();
-    for (const PagedJoin &j : p.joins) a.join_rows = std::max(a.join_rows, j.rows);
+    for (const PagedJoin &j : p.joins) a.join_rows = std::max(a.join_rows, j.rows), a.join_splits = std::max(a.join_splits, j.splits);
     const PagedView v = view_of(pool, batch);
     for (int many = 0; many < 2; ++many) {
         const int first = many ? batch->n_few : 0, last = many ? (int)p.items.size() : batch->n_few;

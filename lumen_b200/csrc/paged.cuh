@@ -44,6 +44,17 @@ __device__ __forceinline__ size_t paged_row(const PagedView &v, const int *table
     return (((size_t)page * v.h_kv + kvh) << v.page_shift) + (pos & ((1 << v.page_shift) - 1));
 }
 
+// The kernels of the paged cache are launched while their predecessor still runs (dependent launch): before pdl_wait they read the plan alone, which
+// no kernel writes.  Calls one behind another overlap their launches so.
+template <typename... KA, typename... A>
+int launch_paged(lumen_ctx *ctx, void (*kernel)(KA...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, A... args) {
+    const bool before = ctx->pdl;
+    ctx->pdl = true;
+    const int rc = launch_pdl(ctx, kernel, grid, dim3(threads), smem, s, args...);
+    ctx->pdl = before;
+    return rc;
+}
+
 struct PagedAppendArgs {
     const float *q, *k, *v, *q_norm, *k_norm, *cos_t, *sin_t;
     size_t q_stride, kv_stride;
@@ -63,7 +74,7 @@ struct PagedAttnArgs {
     float *part;
     long long part_rows;
     const PagedJoin *joins;
-    int n_joins, join_rows;
+    int n_joins, join_rows, join_splits;  // (the largest of the joins)
 };
 // Few rows of a key head (paged_few.cu); more from f32 pools (paged_attn_f32.cu), and from bf16 pools (paged_attn_tc.cu)
 constexpr int kPagedFewRows = 16;

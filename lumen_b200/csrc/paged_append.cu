@@ -44,7 +44,10 @@ __global__ void __launch_bounds__(kWarps * 32) paged_append_kernel(const PagedVi
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = lane * E, all = p.n_head + 2 * p.h_kv;
     const int h0 = (int)(blockIdx.x * kWarps + warp) * kHeads;
     const size_t t = blockIdx.y + (size_t)gridDim.y * blockIdx.z;
-    if (t >= (size_t)p.tokens || h0 >= all) return;
+    pdl_launch();
+    if (t >= (size_t)p.tokens || h0 >= all) return pdl_wait();
+    const int slot = p.tok_slot[t], pos = p.tok_pos[t];
+    pdl_wait();
     float v[kHeads][E];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
@@ -55,11 +58,10 @@ __global__ void __launch_bounds__(kWarps * 32) paged_append_kernel(const PagedVi
             load_row<E>(v[i], src + e0, vec);
         }
     }
-    const int slot = p.tok_slot[t];
     float co[E], sn[E];
     const bool rot = a.cos_t != nullptr && h0 < p.n_head + p.h_kv;
     if (rot) {
-        const size_t at = (size_t)p.tok_pos[t] * (D / 2) + (size_t)(e0 & (D / 2 - 1));
+        const size_t at = (size_t)pos * (D / 2) + (size_t)(e0 & (D / 2 - 1));
 #pragma unroll
         for (int i = 0; i < E; ++i) co[i] = a.cos_t[at + i], sn[i] = a.sin_t[at + i];
     }
@@ -104,9 +106,7 @@ int launch(lumen_ctx *ctx, const PagedView &v, const PagedAppendArgs &a, cudaStr
     const bool vec = whole(a.q, a.q_stride) && whole(a.k, a.kv_stride) && whole(a.v, a.kv_stride);
     const unsigned y = (unsigned)std::min(v.tokens, 32768), z = ((unsigned)v.tokens + y - 1) / y;
     const dim3 grid(((unsigned)v.n_head + 2u * (unsigned)v.h_kv + kWarps * kHeads - 1) / (kWarps * kHeads), y, z);
-    paged_append_kernel<T, D><<<grid, kWarps * 32, 0, s>>>(v, a, vec);
-    LUMEN_LAUNCHED(ctx);
-    return LUMEN_OK;
+    return launch_paged(ctx, paged_append_kernel<T, D>, grid, kWarps * 32, 0, s, v, a, vec);
 }
 
 }  // namespace

@@ -108,6 +108,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_base_s;
+    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    pdl_wait();
     auto load_queries = [&](int id, int n) {  // split, in the swizzled layout; rows behind the item's: zeros
         for (int i = id; i < kRowsTile * (D / 8); i += n) {
             const int r = i / (D / 8), c = i % (D / 8);
@@ -335,9 +337,7 @@ int launch(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStrea
     }();
     if (regs * kThreads < (2 * 128 + kRegsLoad + kRegsIssue) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention: kernel built with %d registers", regs);
     LUMEN_TRY(allow_smem(ctx, paged_attn_f32_kernel<D>, G::kSmem));
-    paged_attn_f32_kernel<D><<<(unsigned)a.n_items, kThreads, G::kSmem, s>>>(v, a, ctx->d_status);
-    LUMEN_LAUNCHED(ctx);
-    return LUMEN_OK;
+    return launch_paged(ctx, paged_attn_f32_kernel<D>, dim3((unsigned)a.n_items), kThreads, G::kSmem, s, v, a, ctx->d_status);
 }
 
 }  // namespace

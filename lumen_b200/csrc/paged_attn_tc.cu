@@ -133,6 +133,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_s;
+    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    pdl_wait();
     int k_issued = 0, v_issued = 0;  // tiles whose copies are on their way (producer warp)
 
     if (warp >= QT * 4) {
@@ -434,9 +436,7 @@ int launch(lumen_ctx *ctx, const PagedView &v, const CUtensorMap &k_map, const C
         if (regs * G::kThreads < (2 * G::kRegsMore + G::kRegsLess) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention: kernel built with %d registers", regs);
     }
     LUMEN_TRY(allow_smem(ctx, paged_attn_tc_kernel<D, QT>, G::kSmem));
-    paged_attn_tc_kernel<D, QT><<<(unsigned)a.n_items, G::kThreads, G::kSmem, s>>>(k_map, v_map, v, a, ctx->d_status);
-    LUMEN_LAUNCHED(ctx);
-    return LUMEN_OK;
+    return launch_paged(ctx, paged_attn_tc_kernel<D, QT>, dim3((unsigned)a.n_items), G::kThreads, G::kSmem, s, k_map, v_map, v, a, ctx->d_status);
 }
 
 }  // namespace

@@ -27,6 +27,8 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView 
     const int len = sq.kv_len, keep = to_seqs[s].kv_len, last = min(recent, keep), old = len - last, pick = keep - last;
     const int *table = from.tables + sq.table;
     int *out = kept + ((size_t)s * from.h_kv + kvh) * kept_stride;
+    pdl_launch();
+    pdl_wait();
     for (int i = tid; i < last; i += kThreads) out[pick + i] = old + i;
     if (pick == 0) return;
     auto value = [&](int pos) { return order_of(from.mass[paged_row(from, table, kvh, pos)]); };
@@ -94,6 +96,8 @@ __global__ void __launch_bounds__(256) paged_move_kernel(const PagedView from, c
     constexpr int kLanes = B / 16, kRowsPer = 256 / kLanes;
     const int kvh = blockIdx.y, s = blockIdx.z, lane = threadIdx.x % kLanes, i = (int)blockIdx.x * kRowsPer + threadIdx.x / kLanes;
     const PagedSeq a = from.seqs[s], b = to.seqs[s];
+    pdl_launch();
+    pdl_wait();
     if (i >= b.kv_len) return;
     const int pos = kept[((size_t)s * from.h_kv + kvh) * kept_stride + i];
     const size_t src = paged_row(from, from.tables + a.table, kvh, pos), dst = paged_row(to, to.tables + b.table, kvh, i);
@@ -109,9 +113,7 @@ template <int B>
 int move(lumen_ctx *ctx, const PagedView &from, const PagedView &to, int n, int max_keep, const int *kept, size_t kept_stride, cudaStream_t s) {
     constexpr int kRowsPer = 256 / (B / 16);
     const dim3 grid((unsigned)((max_keep + kRowsPer - 1) / kRowsPer), (unsigned)from.h_kv, (unsigned)n);
-    paged_move_kernel<B><<<grid, 256, 0, s>>>(from, to, kept, kept_stride);
-    LUMEN_LAUNCHED(ctx);
-    return LUMEN_OK;
+    return launch_paged(ctx, paged_move_kernel<B>, grid, 256, 0, s, from, to, kept, kept_stride);
 }
 
 }  // namespace
@@ -125,8 +127,7 @@ int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from
         f.seqs += s0;
         t.seqs += s0;
         int *k = kept + (size_t)s0 * from.h_kv * kept_stride;
-        paged_select_kernel<<<dim3((unsigned)from.h_kv, (unsigned)n), kThreads, 0, s>>>(f, t.seqs, recent, k, kept_stride);
-        LUMEN_LAUNCHED(ctx);
+        LUMEN_TRY(launch_paged(ctx, paged_select_kernel, dim3((unsigned)from.h_kv, (unsigned)n), kThreads, 0, s, f, t.seqs, recent, k, kept_stride));
         LUMEN_TRY(bytes == 128 ? move<128>(ctx, f, t, n, max_keep, k, kept_stride, s)
                   : bytes == 256 ? move<256>(ctx, f, t, n, max_keep, k, kept_stride, s) : move<512>(ctx, f, t, n, max_keep, k, kept_stride, s));
     }

@@ -101,6 +101,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_few_kernel(co
     };
     int page[2 * kG];
     pages(warp, page);
+    pdl_launch();
+    pdl_wait();
     load_k(warp, page);
     load_v(warp, page);
 
@@ -332,14 +334,20 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_few_kernel(co
     }
 }
 
-// Joins the parts of a row: a warp per row, the parts in their order.
-template <int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedView p, const PagedAttnArgs a) {
+// Joins the parts of a row, in their order: a warp a row, or (WIDE) eight warps a row whose sums meet in shared memory.
+// grid (joins, rows or groups of eight rows)
+constexpr int kJoinWarps = 8;
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedView p, const PagedAttnArgs a) {
     constexpr int E = D / 32;
+    using V = typename std::conditional<E == 4, float4, float2>::type;
+    __shared__ float o_s[WIDE ? kJoinWarps : 1][D], l_s[kJoinWarps];
     const PagedJoin j = a.joins[blockIdx.x];
-    const int r = (int)(blockIdx.y * 4 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    if (r >= j.rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = WIDE ? (int)blockIdx.y : (int)(blockIdx.y * kJoinWarps) + warp;
     const PagedSeq sq = p.seqs[j.seq];
+    pdl_launch();
+    pdl_wait();
+    if (r >= j.rows) return;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + (size_t)a.part_rows * D);
     float top = -INFINITY;
     for (int i = lane; i < j.splits; i += 32) top = fmaxf(top, ml[(size_t)j.part + (size_t)i * j.rows + r].x);
@@ -349,21 +357,38 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedView p, cons
     float v[E], l = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < j.splits; ++i) {
+#pragma unroll 8
+    for (int i = WIDE ? warp : 0; i < j.splits; i += WIDE ? kJoinWarps : 1) {
         const size_t row = (size_t)j.part + (size_t)i * j.rows + r;
         const float2 x = ml[row];
+        float y[E];
+        *reinterpret_cast<V *>(y) = *reinterpret_cast<const V *>(a.part + row * D + lane * E);
         const float f = ex2(x.x - base);
         l = fmaf(x.y, f, l);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = fmaf(a.part[row * D + lane * E + e], f, v[e]);
+        for (int e = 0; e < E; ++e) v[e] = fmaf(y[e], f, v[e]);
+    }
+    if (WIDE) {
+        *reinterpret_cast<V *>(&o_s[warp][lane * E]) = *reinterpret_cast<const V *>(v);
+        if (lane == 0) l_s[warp] = l;
+        __syncthreads();
+        if (warp > 0) return;
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) {
+            l += l_s[w];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] += o_s[w][lane * E + e];
+        }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const size_t o = (size_t)(sq.tok0 + (j.row0 + r) / p.group) * p.n_head + j.kvh * p.group + (j.row0 + r) % p.group;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (a.out_dtype == LUMEN_F32) static_cast<float *>(a.out)[o * D + lane * E + e] = v[e] * inv;
-        else static_cast<__nv_bfloat16 *>(a.out)[o * D + lane * E + e] = __float2bfloat16_rn(v[e] * inv);
+    for (int e = 0; e < E; ++e) v[e] *= inv;
+    if (a.out_dtype == LUMEN_F32) {
+        *reinterpret_cast<V *>(static_cast<float *>(a.out) + o * D + lane * E) = *reinterpret_cast<const V *>(v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.out) + o * D + lane * E + e) = pack_bf16(v[e], v[e + 1]);
     }
     if (lane == 0 && a.lse) a.lse[o] = top * 0.6931471805599453f + logf(l);
 }
@@ -372,9 +397,7 @@ template <typename T, int D, int NB>
 int launch(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
     constexpr size_t bytes = FewGeom<T, D, NB>::kSmem;
     LUMEN_TRY(allow_smem(ctx, paged_few_kernel<T, D, NB>, bytes));
-    paged_few_kernel<T, D, NB><<<(unsigned)a.n_items, kWarps * 32, bytes, s>>>(v, a);
-    LUMEN_LAUNCHED(ctx);
-    return LUMEN_OK;
+    return launch_paged(ctx, paged_few_kernel<T, D, NB>, dim3((unsigned)a.n_items), kWarps * 32, bytes, s, v, a);
 }
 template <typename T, int D>
 int pick(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
@@ -391,11 +414,11 @@ int launch_paged_few(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, con
 }
 
 int launch_paged_join(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
-    const dim3 grid((unsigned)a.n_joins, ((unsigned)a.join_rows + 3) / 4);
-    if (g.d == 64) paged_join_kernel<64><<<grid, 128, 0, s>>>(v, a);
-    else paged_join_kernel<128><<<grid, 128, 0, s>>>(v, a);
-    LUMEN_LAUNCHED(ctx);
-    return LUMEN_OK;
+    // Many parts of few rows: a row's are read by eight warps (one after another they would wait for each other's latency).
+    const bool wide = a.join_splits > 8;
+    const dim3 grid((unsigned)a.n_joins, wide ? (unsigned)a.join_rows : ((unsigned)a.join_rows + kJoinWarps - 1) / kJoinWarps);
+    auto *kernel = g.d == 64 ? (wide ? paged_join_kernel<64, true> : paged_join_kernel<64, false>) : (wide ? paged_join_kernel<128, true> : paged_join_kernel<128, false>);
+    return launch_paged(ctx, kernel, grid, kJoinWarps * 32, 0, s, v, a);
 }
 
 }  // namespace lumen

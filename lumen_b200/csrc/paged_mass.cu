@@ -33,6 +33,8 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * kFewKeys, past = sq.kv_len - sq.q_len;
+    pdl_launch();
+    pdl_wait();
     if (key0 >= sq.kv_len || rows == 0 || rows > kFewRows) return;
     const int *table = p.tables + sq.table;
     const int blocks = (rows + 7) / 8;
@@ -133,7 +135,10 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * kTcKeys, past = sq.kv_len - sq.q_len;
-    if (key0 >= sq.kv_len || rows <= kFewRows) return;
+    if (key0 >= sq.kv_len || rows <= kFewRows) {
+        pdl_launch();
+        return pdl_wait();
+    }
     const int per = kTcRows / p.group, n_rows = per * p.group;  // tokens and rows of a step
     const int start_tok = p.causal ? max(0, key0 - past) : 0, start = start_tok * p.group, steps = (sq.q_len - start_tok + per - 1) / per;  // (start < rows: key0 < kv_len)
     const int tiles = min(2, (sq.kv_len - key0 + 127) / 128);  // of 128 positions
@@ -166,6 +171,8 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_s;  // scores: tile 0 even, odd steps, tile 1 even, odd steps
+    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    pdl_wait();
 
     int q_issued = 0;
     if (warp >= kTcExps / 32 + 2) {
@@ -321,6 +328,8 @@ __global__ void __launch_bounds__(kThreads) paged_mass_kernel(const PagedView p,
     const int tid = threadIdx.x, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int key0 = blockIdx.x * kKeys, past = sq.kv_len - sq.q_len;
+    pdl_launch();
+    pdl_wait();
     if (key0 >= sq.kv_len || sq.q_len == 0) return;
     const int *table = p.tables + sq.table;
     for (int i = tid; i < kKeys * (D / 4); i += kThreads) {
@@ -375,23 +384,20 @@ int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUten
         PagedView v = all;
         v.seqs += s0;
         if (g.dtype == LUMEN_F32) {
-            paged_mass_kernel<D><<<grid_of(a, v, kKeys, n), kThreads, 0, s>>>(v, static_cast<const float *>(a.q), a.scale, a.lse);
-            LUMEN_LAUNCHED(ctx);
+            LUMEN_TRY(launch_paged(ctx, paged_mass_kernel<D>, grid_of(a, v, kKeys, n), kThreads, 0, s, v, static_cast<const float *>(a.q), a.scale, a.lse));
             continue;
         }
         const auto *q = static_cast<const __nv_bfloat16 *>(a.q);
         if (a.min_rows <= kFewRows) {
             const size_t bytes = (size_t)(std::min(kFewRows, a.max_rows) + 7) / 8 * 8 * D * 2;
-            paged_mass_few_kernel<D><<<grid_of(a, v, kFewKeys, n), kFewThreads, bytes, s>>>(v, q, a.scale, a.lse);
-            LUMEN_LAUNCHED(ctx);
+            LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<D>, grid_of(a, v, kFewKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
         }
         if (a.max_rows > kFewRows) {
             CUtensorMap q_map;
             const size_t row = (size_t)all.n_head * D;
             LUMEN_TRY(make_map_3d(ctx, &q_map, q, D, (size_t)all.n_head, D, (size_t)all.tokens, row, all.group, kTcRows / all.group));
             LUMEN_TRY(allow_smem(ctx, paged_mass_tc_kernel<D>, MassGeom<D>::kSmem));
-            paged_mass_tc_kernel<D><<<grid_of(a, v, kTcKeys, n), kTcThreads, MassGeom<D>::kSmem, s>>>(k_map, q_map, v, a.scale, a.lse, ctx->d_status);
-            LUMEN_LAUNCHED(ctx);
+            LUMEN_TRY(launch_paged(ctx, paged_mass_tc_kernel<D>, grid_of(a, v, kTcKeys, n), kTcThreads, MassGeom<D>::kSmem, s, k_map, q_map, v, a.scale, a.lse, ctx->d_status));
         }
     }
     return LUMEN_OK;
