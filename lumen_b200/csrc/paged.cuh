@@ -77,7 +77,7 @@ struct PagedAttnArgs {
     int n_joins, join_rows, join_splits;  // (the largest of the joins)
 };
 // Few rows of a key head (paged_few.cu); more from f32 pools (paged_attn_f32.cu), and from bf16 pools (paged_attn_tc.cu)
-constexpr int kPagedFewRows = 16;
+int paged_few_rows(const PagedGeom &g);
 PagedShape paged_few_shape(int num_sms);
 int launch_paged_few(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
 PagedShape paged_f32_shape(int num_sms);

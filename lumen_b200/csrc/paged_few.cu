@@ -1,6 +1,6 @@
 // Attention of few rows over a paged cache, and the join of partial results.
 //
-// o = sum_j 2^(s_j - m) v_j / l, s_j = scale * log2(e) * q . k_j, for up to 16 rows of a key head (a row is one new token and one of the query heads
+// o = sum_j 2^(s_j - m) v_j / l, s_j = scale * log2(e) * q . k_j, for few rows of a key head (a row is one new token and one of the query heads
 // that read this key head): single tokens and drafts.  Bound by reading the cache once.  A warp takes 16 positions at a time, on its own:
 //   S^T = K.Q^T by m16n8k16 products.  The sum over a head's numbers may run in any order, so the lanes load 16-byte pieces of the keys straight
 //   into the operand's registers, and the queries lie in shared memory in the order that this gives.
@@ -39,8 +39,7 @@ struct FewGeom {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kTerms = kSplit ? 3 : 1;
     static constexpr int kPieces = D * (int)sizeof(T) / 64;       // 16-byte pieces of a key, per lane
-    static constexpr int kGroups = 512 / (D * (int)sizeof(T));    // of 16 positions in a step: 256 bytes of keys and of values a lane in flight
-    static constexpr int kG = kGroups < 1 ? 1 : kGroups;
+    static constexpr int kG = 512 / (D * (int)sizeof(T));         // groups of 16 positions in a step: 256 bytes of keys and of values a lane in flight
     static constexpr int kStep = 16 * kG;
     static constexpr int kTiles = D / 16;                         // of 16 numbers
     static constexpr int kQ = NB * kTiles * 32 * 8 * kTerms;      // bytes: queries in the order of the operand, 8 a lane, tile and term
@@ -406,7 +405,12 @@ int pick(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_
 
 }  // namespace
 
-PagedShape paged_few_shape(int num_sms) { return {kPagedFewRows, 64, num_sms * kBlocksPerSm}; }
+// Rows of a sequence and key head up to which this kernel is taken.  8 sequences of 2000 positions: 16 bits, 32 heads of 128 by themselves, 16 rows 62 us
+// here and 67 with the tensor-core tiles of 128 rows, 20 rows (in blocks of 32) 101 and 61; 32 bits, 32 rows (16 at a time) 259 and 363 us,
+// 48 rows about 390 and 369.
+int paged_few_rows(const PagedGeom &g) { return g.dtype == LUMEN_F32 ? 32 : 16; }
+
+PagedShape paged_few_shape(int num_sms) { return {16, 64, num_sms * kBlocksPerSm}; }
 
 int launch_paged_few(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s) {
     if (g.dtype == LUMEN_F32) return g.d == 64 ? pick<float, 64>(ctx, v, a, s) : pick<float, 128>(ctx, v, a, s);
