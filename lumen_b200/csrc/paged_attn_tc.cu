@@ -244,20 +244,23 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         if (q < active && (warp & 3) < warps_of(q)) {
             const int row_t = it.row0 + min(r, it.rows - 1), t = row_t / p.group, head = it.kvh * p.group + row_t % p.group;
             {  // the warp's 32 rows of queries into the swizzled layout of the tensor core: 16 bytes a thread, whole rows by neighbours
-                constexpr int kPer = D / 8;  // 16-byte pieces of a row
+                constexpr int kPer = D / 8, kAt = 32 / kPer;  // 16-byte pieces of a row; rows at a time
                 const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;  // (the scale's sign goes into the queries)
-#pragma unroll 8
-                for (int i = lane; i < 32 * kPer; i += 32) {
-                    const int rr = (warp & 3) * 32 + i / kPer, c = i % kPer, rg = q * kMma + rr;
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (rg < it.rows) {
-                        const int g = it.row0 + rg;
-                        x = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) +
-                                                             ((size_t)(sq.tok0 + g / p.group) * p.n_head + it.kvh * p.group + g % p.group) * D + c * 8);
-                        x = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
-                        if (a.scale == 0.f) x = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    *reinterpret_cast<uint4 *>(q_s + q * G::kQBytes + (c / 8) * G::kQTile + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+                // every lane knows where its own row is and tells the others
+                const unsigned long long mine = r < it.rows ? ((unsigned long long)(sq.tok0 + t) * p.n_head + head) * D : ~0ull;
+                const int c = lane % kPer;
+                uint4 x[32 / kAt];
+#pragma unroll
+                for (int i = 0; i < 32 / kAt; ++i) {
+                    const unsigned long long at = __shfl_sync(0xffffffffu, mine, i * kAt + lane / kPer);
+                    x[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (at != ~0ull && a.scale != 0.f) x[i] = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + at + 8 * c);
+                }
+#pragma unroll
+                for (int i = 0; i < 32 / kAt; ++i) {
+                    const int rr = (warp & 3) * 32 + i * kAt + lane / kPer;
+                    *reinterpret_cast<uint4 *>(q_s + q * G::kQBytes + (c / 8) * G::kQTile + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
+                        make_uint4(x[i].x ^ sign, x[i].y ^ sign, x[i].z ^ sign, x[i].w ^ sign);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 bar_arrive(&q_bar);
