@@ -298,7 +298,7 @@ int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const
     }
     if (b.max_kv == 0) return LUMEN_OK;
     OnDevice on(ctx);
-    return launch_paged_evict(ctx, pool->g, view_of(pool, from), view_of(pool, to), (int)std::min<size_t>(recent, INT32_MAX), b.max_kv, kept_dev,
+    return launch_paged_evict(ctx, pool->g, view_of(pool, from), view_of(pool, to), (int)std::min<size_t>(recent, INT32_MAX), a.max_kv, b.max_kv, kept_dev,
                               kept_stride, ctx->stream);
 }
 

@@ -94,7 +94,7 @@ struct PagedMassArgs {
     int max_kv, min_rows, max_rows;  // of the sequences with new tokens: positions, rows of a key head
 };
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s);
-int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_keep, int *kept,
+int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_len, int max_keep, int *kept,
                        size_t kept_stride, cudaStream_t s);
 
 }  // namespace lumen

@@ -42,18 +42,6 @@ struct SplitGeom {
 // Products (first term, second term), smallest first.
 __device__ constexpr int kFirst[6] = {2, 0, 1, 1, 0, 0}, kSecond[6] = {0, 2, 1, 0, 1, 0};
 
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next_block) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next_block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-// Two numbers as three pairs of bf16.
-__device__ __forceinline__ void split3(float a, float b, uint32_t (&t)[kTerms]) {
-    t[0] = pack_bf16(a, b);
-    a -= __uint_as_float(t[0] << 16);
-    b -= __uint_as_float(t[0] & 0xffff0000u);
-    t[1] = pack_bf16(a, b);
-    t[2] = pack_bf16(a - __uint_as_float(t[1] << 16), b - __uint_as_float(t[1] & 0xffff0000u));
-}
 // Eight numbers of a row into the three terms' tiles: `at` is the place of the 16-byte piece in the first.
 __device__ __forceinline__ void split_store(const float4 &x, const float4 &y, unsigned char *at, uint32_t term) {
     uint32_t t[4][kTerms];

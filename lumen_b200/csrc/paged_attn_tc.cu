@@ -54,10 +54,6 @@ struct TcGeom {
     static constexpr uint32_t kIdescO = idesc_bf16(kMma, D) | (1u << 16);  // second operand MN-major
 };
 
-// The second operand as it lies in the cache: rows of 64 numbers (128 bytes, swizzled), 8 positions every 1024 bytes, the next 64 numbers a tile further.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next_block) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next_block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "

@@ -23,16 +23,9 @@ namespace {
 using tc::ex2;
 using tc::kLog2e;
 using tc::pack_bf16;
+using tc::split3;
 
 constexpr int kWarps = 4, kBlocksPerSm = 2;
-
-__device__ __forceinline__ void split3(float a, float b, uint32_t (&t)[3]) {
-    t[0] = pack_bf16(a, b);
-    a -= __uint_as_float(t[0] << 16);
-    b -= __uint_as_float(t[0] & 0xffff0000u);
-    t[1] = pack_bf16(a, b);
-    t[2] = pack_bf16(a - __uint_as_float(t[1] << 16), b - __uint_as_float(t[1] & 0xffff0000u));
-}
 
 template <typename T, int D, int NB>
 struct FewGeom {

@@ -2,9 +2,8 @@
 // of the query heads that read the key head.)
 //
 // Every position belongs to one thread or one group of lanes, which walks the rows in their order: no atomics, the same sum every time.
-//   few rows, 16 bits: paged_mass_few_kernel, bound by reading the keys once
-//   many rows, 16 bits: paged_mass_tc_kernel, scores on the 5th-generation tensor cores, bound by the exponentials (16 a cycle and SM)
-//   32 bits: paged_mass_kernel, FMA pipe
+//   up to 64 rows: paged_mass_few_kernel, bound by reading the keys once; 32-bit caches take it for any number of rows
+//   more rows, 16 bits: paged_mass_tc_kernel, scores on the 5th-generation tensor cores, bound by the exponentials (16 a cycle and SM)
 #include <type_traits>
 
 #include "paged.cuh"
@@ -16,41 +15,67 @@ namespace {
 
 using namespace tc;
 
-constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken
+constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken (16 bits)
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-constexpr int kFewThreads = 128, kFewKeys = 256;  // of a CTA: a warp takes 4 groups of 16 positions
+constexpr int kFewThreads = 128;
+
+template <typename T, int D>
+struct FewMass {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kTerms = kSplit ? 3 : 1;
+    static constexpr int kTiles = D / 16;                     // of 16 numbers
+    static constexpr int kPieces = D * (int)sizeof(T) / 64;   // of 16 bytes, per lane and key
+    static constexpr int kGroups = kSplit ? 1 : 2;            // of 16 positions that a warp takes at once
+    static constexpr int kRounds = kSplit ? 1 : 2;
+    static constexpr int kKeys = kFewThreads / 32 * 16 * kGroups * kRounds;  // of a CTA
+    static constexpr int kChunk = kSplit ? 32 : kFewRows;     // rows in shared memory at a time
+};
 
 // Scores of 16 positions x 8 rows from m16n8k16 products.  The sum over the numbers of a head may run in any order, so lane (g, t) loads pieces of
 // 16 bytes of the keys g and g + 8 straight into the operand's registers - no shared memory on the way - and the queries are put in
-// shared memory in the order that this gives: the i-th pair of products uses numbers 32 i + 8 t .. 32 i + 8 t + 7.
-// grid (blocks of 256 positions of the longest sequence, key heads, sequences)
-template <int D>
-__global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const PagedView p, const __nv_bfloat16 *__restrict__ q, float scale, const float *__restrict__ lse) {
-    constexpr int kPieces = D / 32;  // of 16 bytes, per lane and key
-    extern __shared__ uint4 q_s[];   // [blocks of 8 rows][kPieces][32 lanes]: row g of the block, numbers 32 i + 8 t ..
-    __shared__ float l_s[kFewRows];
+// shared memory in the order that this gives.  32 bits: three bf16 terms a number and the six largest of nine products, as in paged_few.cu.
+// grid (blocks of positions of the longest sequence, key heads, sequences)
+template <typename T, int D>
+__global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const PagedView p, const T *__restrict__ q, float scale, const float *__restrict__ lse) {
+    using G = FewMass<T, D>;
+    constexpr int kTiles = G::kTiles, kTerms = G::kTerms, kGroups = G::kGroups, kPieces = G::kPieces;
+    extern __shared__ uint2 q_s[];   // [blocks of 8 rows][tiles][32 lanes][terms]
+    __shared__ float l_s[G::kChunk];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
-    const int rows = sq.q_len * p.group, key0 = blockIdx.x * kFewKeys, past = sq.kv_len - sq.q_len;
+    const int rows = sq.q_len * p.group, key0 = blockIdx.x * G::kKeys, past = sq.kv_len - sq.q_len;
     pdl_launch();
     pdl_wait();
-    if (key0 >= sq.kv_len || rows == 0 || rows > kFewRows) return;
+    if (key0 >= sq.kv_len || rows == 0 || (!G::kSplit && rows > kFewRows)) return;
     const int *table = p.tables + sq.table;
-    const int blocks = (rows + 7) / 8;
     const float scale2 = scale * kLog2e;
-    for (int i = tid; i < blocks * kPieces * 32; i += kFewThreads) {
-        const int ln = i & 31, pc = i / 32 % kPieces, row = i / (32 * kPieces) * 8 + (ln >> 2);
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows)
-            x = *reinterpret_cast<const uint4 *>(q + ((size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group) * D + 32 * pc + 8 * (ln & 3));
-        q_s[i] = x;
-    }
-    if (tid < kFewRows) l_s[tid] = tid < rows ? lse[(size_t)(sq.tok0 + tid / p.group) * p.n_head + kvh * p.group + tid % p.group] * kLog2e : 0.f;
-    constexpr int kGroups = 2;  // of 16 positions at once
+    const int start = p.causal ? max(0, key0 - past) * p.group : 0;  // the first row that sees any of the CTA's positions
+    auto stage = [&](int r0, int n) {  // rows r0 .. r0 + n - 1
+        for (int i = tid; i < (n + 7) / 8 * kTiles * 32; i += kFewThreads) {
+            const int ln = i & 31, tile = i / 32 % kTiles, row = r0 + i / (32 * kTiles) * 8 + (ln >> 2);
+            // 32 bits: tile c takes piece c, numbers 16 c + 4 t ..; 16 bits: tiles 2 c and 2 c + 1 the halves of piece c, numbers 32 c + 8 t ..
+            const int at = G::kSplit ? 16 * tile + 4 * (ln & 3) : 32 * (tile / 2) + 8 * (ln & 3) + 4 * (tile & 1);
+            const bool live = row < r0 + n;
+            const T *src = q + ((size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group) * D + at;
+            if constexpr (G::kSplit) {
+                const float4 x = live ? *reinterpret_cast<const float4 *>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+                uint32_t lo[3], hi[3];
+                split3(x.x, x.y, lo);
+                split3(x.z, x.w, hi);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) q_s[(size_t)i * 3 + k] = make_uint2(lo[k], hi[k]);
+            } else {
+                q_s[i] = live ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
+            }
+        }
+        for (int i = tid; i < n; i += kFewThreads) l_s[i] = lse[(size_t)(sq.tok0 + (r0 + i) / p.group) * p.n_head + kvh * p.group + (r0 + i) % p.group] * kLog2e;
+    };
+    const bool once = rows - start <= G::kChunk;
+    if (once) stage(start, rows - start);
     const uint4 *keys = static_cast<const uint4 *>(p.k);
 #pragma unroll 1
-    for (int round = 0; round < kFewKeys / (kFewThreads / 32 * 16 * kGroups); ++round) {
+    for (int round = 0; round < G::kRounds; ++round) {
         uint4 k[kGroups][2][kPieces];
         size_t at[kGroups][2];
         const int base = key0 + (round * (kFewThreads / 32) + warp) * 16 * kGroups;
@@ -63,31 +88,67 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int c = 0; c < kPieces; ++c) k[i][h][c] = __ldcs(keys + at[i][h] * (D / 8) + 4 * c + t);
-        if (round == 0) __syncthreads();  // the queries are there
-        if (base >= sq.kv_len) continue;
-        float sum[kGroups][2] = {};
-        for (int b = 0; b < blocks; ++b) {
-            float s[kGroups][4] = {};
+                for (int c = 0; c < kPieces; ++c) k[i][h][c] = __ldcs(keys + at[i][h] * (D * sizeof(T) / 16) + 4 * c + t);
+        uint32_t a[kGroups][kTiles][kTerms][4];  // the keys as the first operand
 #pragma unroll
-            for (int c = 0; c < kPieces; ++c) {
-                const uint4 x = q_s[(b * kPieces + c) * 32 + lane];
+        for (int i = 0; i < kGroups; ++i)
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    const uint32_t a0[4] = {k[i][0][c].x, k[i][1][c].x, k[i][0][c].y, k[i][1][c].y}, a1[4] = {k[i][0][c].z, k[i][1][c].z, k[i][0][c].w, k[i][1][c].w};
-                    mma16816(s[i], a0, x.x, x.y);
-                    mma16816(s[i], a1, x.z, x.w);
+            for (int c = 0; c < kTiles; ++c) {
+                if constexpr (G::kSplit) {
+                    const uint4 x = k[i][0][c], y = k[i][1][c];
+                    uint32_t t0[3], t1[3], t2[3], t3[3];
+                    split3(__uint_as_float(x.x), __uint_as_float(x.y), t0);
+                    split3(__uint_as_float(y.x), __uint_as_float(y.y), t1);
+                    split3(__uint_as_float(x.z), __uint_as_float(x.w), t2);
+                    split3(__uint_as_float(y.z), __uint_as_float(y.w), t3);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) a[i][c][n][0] = t0[n], a[i][c][n][1] = t1[n], a[i][c][n][2] = t2[n], a[i][c][n][3] = t3[n];
+                } else {
+                    const uint4 x = k[i][0][c / 2], y = k[i][1][c / 2];
+                    a[i][c][0][0] = c & 1 ? x.z : x.x;
+                    a[i][c][0][1] = c & 1 ? y.z : y.x;
+                    a[i][c][0][2] = c & 1 ? x.w : x.y;
+                    a[i][c][0][3] = c & 1 ? y.w : y.y;
                 }
             }
+        float sum[kGroups][2] = {};
+#pragma unroll 1
+        for (int r0 = start; r0 < rows; r0 += G::kChunk) {
+            const int n = min(G::kChunk, rows - r0);
+            if (!once) {
+                __syncthreads();  // everyone is done with the rows before
+                stage(r0, n);
+            }
+            if (!once || round == 0) __syncthreads();
+            for (int b = 0; 8 * b < n; ++b) {
+                float big[kGroups][4] = {}, small[kGroups][4] = {};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = 8 * b + 2 * t + e;
-                const float l = l_s[row];
-                const int last = row >= rows ? -1 : p.causal ? past + row / p.group : sq.kv_len - 1;
+                for (int c = 0; c < kTiles; ++c) {
+                    const uint2 *x = q_s + (size_t)((b * kTiles + c) * 32 + lane) * kTerms;
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    sum[i][0] += base + 16 * i + g <= last ? ex2(fmaf(s[i][e], scale2, -l)) : 0.f;
-                    sum[i][1] += base + 16 * i + 8 + g <= last ? ex2(fmaf(s[i][2 + e], scale2, -l)) : 0.f;
+                    for (int i = 0; i < kGroups; ++i) {
+                        if constexpr (G::kSplit) {
+                            mma16816(small[i], a[i][c][2], x[0].x, x[0].y);
+                            mma16816(small[i], a[i][c][0], x[2].x, x[2].y);
+                            mma16816(small[i], a[i][c][1], x[1].x, x[1].y);
+                            mma16816(small[i], a[i][c][1], x[0].x, x[0].y);
+                            mma16816(small[i], a[i][c][0], x[1].x, x[1].y);
+                        }
+                        mma16816(big[i], a[i][c][0], x[0].x, x[0].y);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 8 * b + 2 * t + e, r = r0 + row;
+                    const float l = row < n ? l_s[row] : 0.f;
+                    const int last = row >= n ? -1 : p.causal ? past + r / p.group : sq.kv_len - 1;
+#pragma unroll
+                    for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float s = G::kSplit ? big[i][2 * h + e] + small[i][2 * h + e] : big[i][2 * h + e];
+                            sum[i][h] += base + 16 * i + 8 * h + g <= last ? ex2(fmaf(s, scale2, -l)) : 0.f;
+                        }
                 }
             }
         }
@@ -311,70 +372,6 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (warp == kTcExps / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// ---- 32 bits --------------------------------------------------------------------------------------------------------------
-constexpr int kKeys = 64, kRows = 16, kThreads = 128;
-
-__device__ __forceinline__ void four(const float *p, float (&v)[4]) {
-    const float4 x = *reinterpret_cast<const float4 *>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-}
-
-// grid (tiles of the longest sequence, key heads, sequences)
-template <int D>
-__global__ void __launch_bounds__(kThreads) paged_mass_kernel(const PagedView p, const float *__restrict__ q, float scale, const float *__restrict__ lse) {
-    __shared__ __align__(16) float k_s[kKeys][D + 4];
-    __shared__ __align__(16) float q_s[kRows][D];
-    __shared__ float l_s[kRows], half_s[kKeys];
-    const int tid = threadIdx.x, kvh = blockIdx.y;
-    const PagedSeq sq = p.seqs[blockIdx.z];
-    const int key0 = blockIdx.x * kKeys, past = sq.kv_len - sq.q_len;
-    pdl_launch();
-    pdl_wait();
-    if (key0 >= sq.kv_len || sq.q_len == 0) return;
-    const int *table = p.tables + sq.table;
-    for (int i = tid; i < kKeys * (D / 4); i += kThreads) {
-        const int r = i / (D / 4), e = i % (D / 4) * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (key0 + r < sq.kv_len) four(static_cast<const float *>(p.k) + paged_row(p, table, kvh, key0 + r) * D + e, v);
-        *reinterpret_cast<float4 *>(&k_s[r][e]) = make_float4(v[0], v[1], v[2], v[3]);
-    }
-    const int key = tid % kKeys, half = tid / kKeys, rows = sq.q_len * p.group;
-    const int start = p.causal ? max(0, key0 - past) * p.group : 0;  // the first row that sees any of the tile
-    float gained = 0.f;
-    for (int r0 = start; r0 < rows; r0 += kRows) {
-        __syncthreads();
-        for (int i = tid; i < kRows * (D / 4); i += kThreads) {
-            const int r = i / (D / 4), e = i % (D / 4) * 4, row = r0 + r;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (row < rows) four(q + ((size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group) * D + e, v);
-            *reinterpret_cast<float4 *>(&q_s[r][e]) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-        if (tid < kRows && r0 + tid < rows) l_s[tid] = lse[(size_t)(sq.tok0 + (r0 + tid) / p.group) * p.n_head + kvh * p.group + (r0 + tid) % p.group];
-        __syncthreads();
-        constexpr int RH = kRows / 2;
-        float s[RH];
-#pragma unroll
-        for (int r = 0; r < RH; ++r) s[r] = 0.f;
-#pragma unroll 4
-        for (int e = 0; e < D; e += 4) {
-            const float4 k4 = *reinterpret_cast<const float4 *>(&k_s[key][e]);
-#pragma unroll
-            for (int r = 0; r < RH; ++r) {
-                const float4 q4 = *reinterpret_cast<const float4 *>(&q_s[half * RH + r][e]);
-                s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < RH; ++r) {
-            const int row = r0 + half * RH + r;
-            if (row < rows && (!p.causal || key0 + key <= past + row / p.group)) gained += expf(s[r] * scale - l_s[half * RH + r]);
-        }
-    }
-    if (half) half_s[key] = gained;
-    __syncthreads();
-    if (!half && key0 + key < sq.kv_len) p.mass[paged_row(p, table, kvh, key0 + key)] += gained + half_s[key];
-}
-
 dim3 grid_of(const PagedMassArgs &a, const PagedView &v, int keys, int n) { return dim3((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)v.h_kv, (unsigned)n); }
 
 template <int D>
@@ -384,13 +381,14 @@ int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUten
         PagedView v = all;
         v.seqs += s0;
         if (g.dtype == LUMEN_F32) {
-            LUMEN_TRY(launch_paged(ctx, paged_mass_kernel<D>, grid_of(a, v, kKeys, n), kThreads, 0, s, v, static_cast<const float *>(a.q), a.scale, a.lse));
+            const size_t bytes = (size_t)(std::min(FewMass<float, D>::kChunk, a.max_rows) + 7) / 8 * 8 * D * 6;
+            LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<float, D>, grid_of(a, v, FewMass<float, D>::kKeys, n), kFewThreads, bytes, s, v, static_cast<const float *>(a.q), a.scale, a.lse));
             continue;
         }
         const auto *q = static_cast<const __nv_bfloat16 *>(a.q);
         if (a.min_rows <= kFewRows) {
             const size_t bytes = (size_t)(std::min(kFewRows, a.max_rows) + 7) / 8 * 8 * D * 2;
-            LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<D>, grid_of(a, v, kFewKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
+            LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<__nv_bfloat16, D>, grid_of(a, v, FewMass<__nv_bfloat16, D>::kKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
         }
         if (a.max_rows > kFewRows) {
             CUtensorMap q_map;

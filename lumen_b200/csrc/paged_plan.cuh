@@ -61,7 +61,7 @@ inline int paged_refuse(std::string &err, int code, const char *fmt, long long a
 // Checks the arguments of lumen_page_batch_new and lays out sequences, tables and tokens.
 inline int paged_layout(const PagedGeom &g, size_t n_head, size_t n_seq, const int32_t *q_lens, const int32_t *kv_lens, const int32_t *first_pos,
                         const int32_t *tables, size_t table_stride, int causal, PagedPlan &p, std::string &err) {
-    if (n_head == 0 || n_head > (1u << 20) || n_head % (size_t)g.h_kv) return paged_refuse(err, LUMEN_ERR_SHAPE, "%lld query heads over %lld key heads", (long long)n_head, g.h_kv);
+    if (n_head == 0 || n_head > 65536 || n_head % (size_t)g.h_kv) return paged_refuse(err, LUMEN_ERR_SHAPE, "%lld query heads over %lld key heads", (long long)n_head, g.h_kv);
     if (n_head / (size_t)g.h_kv > 128) return paged_refuse(err, LUMEN_ERR_UNSUPPORTED, "%lld query heads to a key head", (long long)n_head / g.h_kv);
     if (n_seq > (1u << 24)) return paged_refuse(err, LUMEN_ERR_INVALID, "%lld sequences", (long long)n_seq);
     if (n_seq && (!q_lens || !kv_lens || (table_stride && !tables))) return paged_refuse(err, LUMEN_ERR_INVALID, "null argument");

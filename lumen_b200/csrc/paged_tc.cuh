@@ -41,6 +41,21 @@ __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volati
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The second operand as it lies in the cache: rows of 64 numbers (128 bytes, swizzled), 8 positions every 1024 bytes, the next 64 numbers `next_block`
+// bytes further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next_block) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next_block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Two 32-bit numbers as three pairs of bf16: each the rounded rest of the ones before; what is left behind the third is below 2^-24 of the number.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&t)[3]) {
+    t[0] = pack_bf16(a, b);
+    a -= __uint_as_float(t[0] << 16);
+    b -= __uint_as_float(t[0] & 0xffff0000u);
+    t[1] = pack_bf16(a, b);
+    t[2] = pack_bf16(a - __uint_as_float(t[1] << 16), b - __uint_as_float(t[1] & 0xffff0000u));
+}
+
 // Two f32 operations in one instruction.
 __device__ __forceinline__ uint64_t two(float a, float b) {
     uint64_t r;
@@ -58,10 +73,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // 2^x of two numbers of at most 2^7 on the FMA pipe: x = n + f with n the nearest whole number (1.5 * 2^23 added and taken off again), 2^f on
-// [-0.5, 0.5] by the polynomial of degree 4 with the least largest relative error (2.6e-6; found by Remez exchange), n added to the
-// exponent.  Below -126 it gives about 2^-126 instead of less; of a NaN,
-// the largest finite number (which no sum survives).
+// [-0.5, 0.5] by the polynomial of degree 4 with the least largest relative error (2.6e-6; found by Remez exchange), times 2^n.  Below
+// -126 it gives about 2^-126 instead of less.
 __device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
     float x, y;
     apart(x2, x, y);
@@ -73,11 +92,10 @@ __device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
     r = fma2(r, f, two(0.240247443318367f, 0.240247443318367f));
     r = fma2(r, f, two(0.6931217908859253f, 0.6931217908859253f));
     r = fma2(r, f, two(0.9999992847442627f, 0.9999992847442627f));
-    float ra, rb, ta, tb;
-    apart(r, ra, rb);
+    float ta, tb;
     apart(t, ta, tb);
-    a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
-    b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
+    const uint64_t scale = two(__uint_as_float((__float_as_uint(ta) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(tb) << 23) + 0x3f800000u));
+    apart(mul2(r, scale), a, b);  // (a product, so that a NaN stays one)
 }
 
 }  // namespace tc

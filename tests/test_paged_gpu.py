@@ -68,20 +68,20 @@ class World:
 
 
 def reference(w, q, scale, causal=True, q_lens=None, kv_lens=None, tables=None, out_bits=True):
-    """Outputs, log-sums, weights received per sequence and the bounds of the first two, in 64 bits on the CPU."""
+    """Outputs, log-sums, weights received per sequence and the bounds of the first two, in 64 bits."""
     q_lens, kv_lens, tables = q_lens or w.q_lens, kv_lens or w.kv_lens, tables or w.tables
     G, t = w.Hq // w.Hkv, 0
     outs, lses, tols, ltols, mass = [], [], [], [], []
     for b, n in enumerate(q_lens):
-        k, v = (w.rows(x, tables[b], kv_lens[b]).double().cpu() for x in (w.k, w.v))
-        x = q[t: t + n].double().cpu()
+        k, v = (w.rows(x, tables[b], kv_lens[b]).double() for x in (w.k, w.v))
+        x = q[t: t + n].double()
         t += n
         kk, vv = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)  # [kv, Hq, D]
         s = torch.einsum("thd,jhd->htj", x, kk) * scale
         big = torch.einsum("thd,jhd->htj", x.abs(), kk.abs()) * abs(scale)
-        seen = torch.ones(n, kv_lens[b], dtype=torch.bool)
+        seen = torch.ones(n, kv_lens[b], dtype=torch.bool, device=DEV)
         if causal:
-            seen = torch.arange(kv_lens[b])[None] <= kv_lens[b] - n + torch.arange(n)[:, None]
+            seen = torch.arange(kv_lens[b], device=DEV)[None] <= kv_lens[b] - n + torch.arange(n, device=DEV)[:, None]
         s = s.masked_fill(~seen, -np.inf)
         if kv_lens[b] == 0:
             outs.append(torch.zeros(n, w.Hq, w.D, dtype=torch.float64))
@@ -97,12 +97,12 @@ def reference(w, q, scale, causal=True, q_lens=None, kv_lens=None, tables=None, 
         rel_t = rel.squeeze(-1).T[:, :, None]
         o = torch.einsum("htj,jhd->thd", p, vv)
         tol = av * (2 * rel_t + (2.0 ** -8 if w.dtype == "bf16" else 0)) + (o.abs() * 2.0 ** -8 if w.dtype == "bf16" and out_bits else 0) + 1e-30
-        outs.append(o)
-        tols.append(tol)
+        outs.append(o.cpu())
+        tols.append(tol.cpu())
         lse = torch.logsumexp(s, -1)
-        lses.append(lse.T)
-        ltols.append((rel.squeeze(-1) + lse.abs() * 2.0 ** -21).T)
-        mass.append((p.view(w.Hkv, G, n, kv_lens[b]).sum((1, 2)).T, (p * 2 * (rel + ds)).view(w.Hkv, G, n, kv_lens[b]).sum((1, 2)).T + n * G * 1e-7))
+        lses.append(lse.T.cpu())
+        ltols.append((rel.squeeze(-1) + lse.abs() * 2.0 ** -21).T.cpu())
+        mass.append((p.view(w.Hkv, G, n, kv_lens[b]).sum((1, 2)).T.cpu(), (p * 2 * (rel + ds)).view(w.Hkv, G, n, kv_lens[b]).sum((1, 2)).T.cpu() + n * G * 1e-7))
     return torch.cat(outs), torch.cat(lses), torch.cat(tols), torch.cat(ltols), mass
 
 
@@ -166,6 +166,87 @@ def test_long_contexts_are_cut_and_joined(L, dtype, heads, q_len):
     o, l, to, tl, _ = reference(w, q, w.D ** -0.5)
     close(out, o, to)
     close(lse, l, tl)
+
+
+@pytest.mark.parametrize("dtype,heads,q_len,kv_len", [("bf16", (8, 8, 64), 5000, 5000), ("bf16", (32, 8, 128), 1400, 3100), ("f32", (8, 8, 64), 2500, 2700)])
+def test_more_items_than_run_at_once(L, dtype, heads, q_len, kv_len):
+    """The items of the last round are cut, and joined."""
+    w = World(L, dtype, heads, 64, [q_len, 1], [kv_len, 70])
+    q = w.randn(q_len + 1, w.Hq, w.D).mul_(2).to(w.t)
+    out, lse, _ = attend(w, q, w.D ** -0.5)
+    o, l, to, tl, _ = reference(w, q, w.D ** -0.5)
+    close(out, o, to)
+    close(lse, l, tl)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("singles", [3, 24])
+def test_single_tokens_beside_a_chunk(L, dtype, singles):
+    """With the chunk's rows, or, where there is more to read, in a launch of their own."""
+    q_lens, kv_lens = [1] * singles + [100] + [2], [390 + i for i in range(singles)] + [500, 410]
+    w = World(L, dtype, (32, 8, 128), 64, q_lens, kv_lens)
+    q = w.randn(sum(q_lens), w.Hq, w.D).to(w.t)
+    out, lse, _ = attend(w, q, w.D ** -0.5)
+    o, l, to, tl, _ = reference(w, q, w.D ** -0.5)
+    close(out, o, to)
+    close(lse, l, tl)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q_len,kv_len", [(1, 500), (20, 500), (200, 700)])
+@pytest.mark.parametrize("at", [3, 64, 130, 499])
+def test_a_key_that_is_no_number(L, dtype, q_len, kv_len, at):
+    """Tokens that see it have no finite result, the others what they had."""
+    w = World(L, dtype, (8, 2, 64), 16, [q_len], [kv_len])
+    q = w.randn(q_len, w.Hq, w.D).to(w.t)
+    before, _, _ = attend(w, q, 0.125)
+    page, slot = w.at(w.tables[0], kv_len)
+    w.k[page[at], :, slot[at]] = float("nan")
+    after, lse, _ = attend(w, q, 0.125)
+    sees = torch.arange(q_len) + kv_len - q_len >= at
+    assert torch.equal(after[~sees], before[~sees])
+    assert not torch.isfinite(after[sees]).any() and not torch.isfinite(lse[sees]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_pool_beyond_32_bits(L, dtype):
+    """More than 2^32 bytes and 2^31 numbers of keys; the sequences' pages lie all over it."""
+    heads, page = (8, 4, 128), 64
+    q_lens, kv_lens = [1, 90, 2], [700, 300, 64]
+    w = World(L, dtype, heads, page, q_lens, kv_lens, spare=3 * 2 ** 30 // (4 * 128 * 64), extra=[100, 64, 1])
+    assert max(map(max, w.tables)) * 4 * 128 * 64 > 2 ** 31
+    q = w.randn(sum(q_lens), w.Hq, w.D).to(w.t)
+    qkv = w.randn(sum(q_lens), 16 * 128)
+    batch = w.batch()
+    q_out = torch.empty(sum(q_lens), 8, 128, dtype=w.t, device=DEV)
+    torch.cuda.synchronize()
+    at = qkv.data_ptr()
+    L.paged_append(w.pool, batch, at, at + 4 * 8 * 128, at + 4 * 12 * 128, 16 * 128, 16 * 128, q_out.data_ptr())
+    w.pool.ctx.synchronize()
+    t = 0
+    for b, n in enumerate(q_lens):
+        assert torch.equal(w.rows(w.k, w.tables[b], kv_lens[b])[kv_lens[b] - n:], qkv[t: t + n, 8 * 128: 12 * 128].view(n, 4, 128).to(w.t))
+        t += n
+    before = [w.rows(w.mass, w.tables[b], n).double().cpu() for b, n in enumerate(kv_lens)]
+    out, lse, _ = attend(w, q, w.D ** -0.5)
+    o, l, to, tl, mass = reference(w, q, w.D ** -0.5)
+    close(out, o, to)
+    close(lse, l, tl)
+    dev_lse = lse.float().to(DEV)
+    torch.cuda.synchronize()
+    L.paged_attention_mass(w.pool, batch, q.data_ptr(), w.D ** -0.5, dev_lse.data_ptr())
+    w.pool.ctx.synchronize()
+    for b, n in enumerate(kv_lens):
+        close(w.rows(w.mass, w.tables[b], n).double().cpu(), before[b] + mass[b][0], mass[b][1] + (before[b] + mass[b][0]) * 2.0 ** -22)
+    kept = torch.zeros(3, 4, 100, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    L.paged_evict(w.pool, batch, w.batch(q_lens=[0] * 3, kv_lens=[100, 64, 1], tables=w.extra_tables), 5, kept.data_ptr(), 100)
+    w.pool.ctx.synchronize()
+    for b, n in enumerate([100, 64, 1]):
+        for pool in (w.k, w.v):
+            was, now = w.rows(pool, w.tables[b], kv_lens[b]), w.rows(pool, w.extra_tables[b], n)
+            for h in range(4):
+                assert torch.equal(now[:, h], was[kept[b, h, :n].long(), h])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -394,6 +475,20 @@ def test_evict(L, dtype, heads, kv, keep, recent, kind):
         assert torch.equal(got.nan_to_num(5.0, 6.0, 7.0), t.nan_to_num(5.0, 6.0, 7.0))
 
 
+def test_evict_from_a_cache_too_long_for_shared_memory(L):
+    w = World(L, "f32", (4, 2, 64), 256, [0, 0], [45000, 100], extra=[900, 100])
+    w.put(w.mass, 0, (torch.rand(45000, 2, generator=w.g, device=DEV) * 5000).floor())
+    kept = torch.full((2, 2, 900), -7, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    L.paged_evict(w.pool, w.batch(), w.batch(kv_lens=[900, 100], tables=w.extra_tables), 100, kept.data_ptr(), 900)
+    w.pool.ctx.synchronize()
+    m = w.rows(w.mass, w.tables[0], 45000).cpu().numpy()
+    for h in range(2):
+        stay = _chosen(m[:, h], 900, 100)
+        assert kept[0, h].tolist() == stay.tolist() and kept[1, h, :100].tolist() == list(range(100))
+        assert torch.equal(w.rows(w.v, w.extra_tables[0], 900)[:, h], w.rows(w.v, w.tables[0], 45000)[torch.as_tensor(stay, device=DEV), h])
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 def test_refusals(L, ctx):
     def refused(code, call, *a, **k):
@@ -411,6 +506,7 @@ def test_refusals(L, ctx):
                                 ([1.5], [2], [[0]], "ERR_INVALID"), ([1], [2 ** 31], [[0]], "ERR_INVALID")]:
         refused(code, L.PageBatch, pool, 4, q, kv, tables)
     refused("ERR_SHAPE", L.PageBatch, pool, 3, [1], [1], [[0]])
+    refused("ERR_UNSUPPORTED", L.PageBatch, pool, 2 * 129, [1], [1], [[0]])
     refused("ERR_INVALID", L.PageBatch, pool, 4, [1], [1], [[0]], first_pos=[-1])
 
     batch = L.PageBatch(pool, 4, [1], [17], [[0, 1]])
