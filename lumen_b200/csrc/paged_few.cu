@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_few_kernel(co
         for (int x = 0; x < kG; ++x)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float big[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
+                float sums[4][4] = {};  // (of their own, so that products do not wait for each other; the last the largest)
 #pragma unroll
                 for (int c = 0; c < kTiles; ++c) {
                     const uint2 *qf = q_s + (size_t)((b * kTiles + c) * 32 + lane) * kTerms;
@@ -159,20 +159,20 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_few_kernel(co
                         split3(__uint_as_float(k1.z), __uint_as_float(k1.w), a3);
                         const uint2 q0 = qf[0], q1 = qf[1], q2 = qf[2];
                         const uint32_t h[4] = {a0[0], a1[0], a2[0], a3[0]}, md[4] = {a0[1], a1[1], a2[1], a3[1]}, lw[4] = {a0[2], a1[2], a2[2], a3[2]};
-                        mma16816(small, lw, q0.x, q0.y);
-                        mma16816(small, h, q2.x, q2.y);
-                        mma16816(small, md, q1.x, q1.y);
-                        mma16816(small, md, q0.x, q0.y);
-                        mma16816(small, h, q1.x, q1.y);
-                        mma16816(big, h, q0.x, q0.y);
+                        mma16816(sums[0], lw, q0.x, q0.y);
+                        mma16816(sums[1], md, q1.x, q1.y);
+                        mma16816(sums[2], h, q1.x, q1.y);
+                        mma16816(sums[3], h, q0.x, q0.y);
+                        mma16816(sums[0], h, q2.x, q2.y);
+                        mma16816(sums[1], md, q0.x, q0.y);
                     } else {
                         const uint4 k0 = k[x][0][c / 2], k1 = k[x][1][c / 2];
                         const uint32_t h[4] = {c & 1 ? k0.z : k0.x, c & 1 ? k1.z : k1.x, c & 1 ? k0.w : k0.y, c & 1 ? k1.w : k1.y};
-                        mma16816(big, h, qf->x, qf->y);
+                        mma16816(sums[c & 3], h, qf->x, qf->y);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[x][b][e] = kSplit ? big[e] + small[e] : big[e];
+                for (int e = 0; e < 4; ++e) s[x][b][e] = sums[3][e] + (sums[2][e] + (sums[1][e] + sums[0][e]));
             }
         load_k(i + kWarps, next);
         // weights: lane (g, t) has positions g, g + 8 of the rows 2t, 2t + 1

@@ -2,8 +2,9 @@
 // of the query heads that read the key head.)
 //
 // Every position belongs to one thread or one group of lanes, which walks the rows in their order: no atomics, the same sum every time.
-//   up to 64 rows: paged_mass_few_kernel, bound by reading the keys once; 32-bit caches take it for any number of rows
-//   more rows, 16 bits: paged_mass_tc_kernel, scores on the 5th-generation tensor cores, bound by the exponentials (16 a cycle and SM)
+//   up to 64 rows: paged_mass_few_kernel, bound by reading the keys once
+//   more: scores on the 5th-generation tensor cores: paged_mass_tc_kernel (16 bits), bound by the exponentials (16 a cycle and SM), and
+//   paged_mass_f32_kernel, bound by the six products of three bf16 terms
 #include <type_traits>
 
 #include "paged.cuh"
@@ -15,7 +16,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken (16 bits)
+constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
 constexpr int kFewThreads = 128;
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * G::kKeys, past = sq.kv_len - sq.q_len;
     pdl_launch();
     pdl_wait();
-    if (key0 >= sq.kv_len || rows == 0 || (!G::kSplit && rows > kFewRows)) return;
+    if (key0 >= sq.kv_len || rows == 0 || rows > kFewRows) return;
     const int *table = p.tables + sq.table;
     const float scale2 = scale * kLog2e;
     const int start = p.causal ? max(0, key0 - past) * p.group : 0;  // the first row that sees any of the CTA's positions
@@ -121,20 +122,22 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
             }
             if (!once || round == 0) __syncthreads();
             for (int b = 0; 8 * b < n; ++b) {
-                float big[kGroups][4] = {}, small[kGroups][4] = {};
+                float sums[4][kGroups][4] = {};  // (of their own, so that products do not wait for each other; the last the largest)
 #pragma unroll
                 for (int c = 0; c < kTiles; ++c) {
                     const uint2 *x = q_s + (size_t)((b * kTiles + c) * 32 + lane) * kTerms;
 #pragma unroll
                     for (int i = 0; i < kGroups; ++i) {
                         if constexpr (G::kSplit) {
-                            mma16816(small[i], a[i][c][2], x[0].x, x[0].y);
-                            mma16816(small[i], a[i][c][0], x[2].x, x[2].y);
-                            mma16816(small[i], a[i][c][1], x[1].x, x[1].y);
-                            mma16816(small[i], a[i][c][1], x[0].x, x[0].y);
-                            mma16816(small[i], a[i][c][0], x[1].x, x[1].y);
+                            mma16816(sums[0][i], a[i][c][2], x[0].x, x[0].y);
+                            mma16816(sums[1][i], a[i][c][1], x[1].x, x[1].y);
+                            mma16816(sums[2][i], a[i][c][0], x[1].x, x[1].y);
+                            mma16816(sums[3][i], a[i][c][0], x[0].x, x[0].y);
+                            mma16816(sums[0][i], a[i][c][0], x[2].x, x[2].y);
+                            mma16816(sums[1][i], a[i][c][1], x[0].x, x[0].y);
+                        } else {
+                            mma16816(sums[c & 3][i], a[i][c][0], x[0].x, x[0].y);
                         }
-                        mma16816(big[i], a[i][c][0], x[0].x, x[0].y);
                     }
                 }
 #pragma unroll
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const Paged
                     for (int i = 0; i < kGroups; ++i)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float s = G::kSplit ? big[i][2 * h + e] + small[i][2 * h + e] : big[i][2 * h + e];
+                            const float s = sums[3][i][2 * h + e] + (sums[2][i][2 * h + e] + (sums[1][i][2 * h + e] + sums[0][i][2 * h + e]));
                             sum[i][h] += base + 16 * i + 8 * h + g <= last ? ex2(fmaf(s, scale2, -l)) : 0.f;
                         }
                 }
@@ -372,6 +375,205 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (warp == kTcExps / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
+// ---- many rows, 32 bits ---------------------------------------------------------------------------------------------------
+constexpr int kSplitKeys = 128, kSplitThreads = 512;
+// (the warpgroup that holds a step's queries in flight takes registers from the one that issues the products: 128 at launch, 2 x 128 + 184 + 72)
+constexpr int kRegsLoad = 184, kRegsIssue = 72;
+// Products (first term, second term), smallest first.
+__device__ constexpr int kFirst[6] = {2, 0, 1, 1, 0, 0}, kSecond[6] = {0, 2, 1, 0, 1, 0};
+
+template <int D>
+struct SplitMass {
+    static constexpr int kBlocks = D / kBK;
+    static constexpr uint32_t kTile = 128 * kBK * 2, kTerm = kBlocks * kTile, kOperand = 3 * kTerm;  // 128 keys or rows
+    static constexpr int kStages = D == 128 ? 1 : 2;
+    static constexpr size_t kSmem = (1 + kStages) * (size_t)kOperand + 1024;
+    static constexpr int kPieces = 128 * D / 8 / 128;  // 8 numbers each, of a loading thread
+};
+
+// Eight numbers of a row as three terms, `at`: the place of the 16-byte piece in the first.
+template <int D>
+__device__ __forceinline__ void put_split(const float4 &x, const float4 &y, unsigned char *base, int r, int c) {
+    unsigned char *at = base + (c / 8) * SplitMass<D>::kTile + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    uint32_t t[4][3];
+    split3(x.x, x.y, t[0]);
+    split3(x.z, x.w, t[1]);
+    split3(y.x, y.y, t[2]);
+    split3(y.z, y.w, t[3]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4 *>(at + i * SplitMass<D>::kTerm) = make_uint4(t[0][i], t[1][i], t[2][i], t[3][i]);
+}
+
+// A CTA owns 128 positions of a key head and walks the rows that see any of them, 128 at a time, as paged_mass_tc_kernel does.  Warpgroups 0 and 1:
+// exponentials and sums (half of the columns each); 2: queries, a step ahead in registers, split into shared memory; 3: products.
+// grid (blocks of 128 positions of the longest sequence, key heads, sequences)
+template <int D>
+__global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const PagedView p, const float *__restrict__ q, float scale, const float *__restrict__ lse, DeviceStatus *status) {
+    using G = SplitMass<D>;
+    constexpr int kStages = G::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *k_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *ring = k_s + G::kOperand;
+    __shared__ uint64_t q_full[kStages], q_free[kStages], l_full[2], s_full[2], s_free[2], quiet;
+    __shared__ __align__(16) float l_s[2][128];
+    __shared__ float part_s[2][kSplitKeys];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int failed_s;
+    volatile int *failed = &failed_s;
+    const int tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.y;
+    const PagedSeq sq = p.seqs[blockIdx.z];
+    const int rows = sq.q_len * p.group, key0 = blockIdx.x * kSplitKeys, past = sq.kv_len - sq.q_len;
+    if (key0 >= sq.kv_len || rows <= kFewRows) {
+        pdl_launch();
+        return pdl_wait();
+    }
+    const int start = p.causal ? max(0, key0 - past) * p.group : 0, steps = (rows - start + 127) / 128;  // (start < rows: key0 < kv_len)
+    const int *table = p.tables + sq.table;
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            bar_init(&q_full[s], 128);
+            bar_init(&q_free[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            bar_init(&l_full[b], 128);
+            bar_init(&s_full[b], 1);
+            bar_init(&s_free[b], 256);
+        }
+        bar_init(&quiet, 1);
+        failed_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_base_s)), "r"(256) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    for (int i = tid; i < kSplitKeys * (D / 8); i += kSplitThreads) {  // the keys (behind the end: zeros)
+        const int r = i / (D / 8), c = i % (D / 8);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (key0 + r < sq.kv_len) {
+            const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.k) + paged_row(p, table, kvh, key0 + r) * D + 8 * c);
+            x = src[0];
+            y = src[1];
+        }
+        put_split<D>(x, y, k_s, r, c);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_before();
+    __syncthreads();
+    tc_after();
+    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    const uint32_t tmem = tmem_base_s;  // scores of even and odd steps
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (warp == 12) {
+            const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), k0 = __shfl_sync(0xffffffffu, saddr(k_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                const int s = i % kStages, b = i & 1;
+                const bool ok = wait_warp(&q_full[s], (uint32_t)((i / kStages) & 1), failed, status, 900) &&
+                                (i < 2 || wait_warp(&s_free[b], (uint32_t)((i / 2 - 1) & 1), failed, status, 901));
+                tc_after();
+                if (ok) {
+                    const uint64_t kd = smem_desc(k0), qd = smem_desc(ring0 + (uint32_t)s * G::kOperand);
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int kb = 0; kb < G::kBlocks; ++kb)
+#pragma unroll
+                            for (int kk = 0; kk < kBK / 16; ++kk)
+                                mma_ss(acc0 + (uint32_t)(b * 128), kd + ((kFirst[x] * G::kTerm + kb * G::kTile) >> 4) + 2 * kk, qd + ((kSecond[x] * G::kTerm + kb * G::kTile) >> 4) + 2 * kk,
+                                       idesc_bf16(128, 128), x + kb + kk > 0);
+                }
+                commit_one(&s_full[b]);
+                commit_one(&q_free[s]);
+            }
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+        // a thread has one piece of 8 numbers of every kStep-th row
+        constexpr int kStep = 128 / (D / 8);
+        const int id = tid - 256, c = id % (D / 8), r0 = id / (D / 8);
+        float4 x[G::kPieces][2];
+        float l = 0.f;
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int n = 0; n < G::kPieces; ++n) {
+                const int row = start + i * 128 + r0 + n * kStep, tok = row / p.group;
+                x[n][0] = x[n][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (row < rows) {
+                    const float4 *src = reinterpret_cast<const float4 *>(q + ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + row - tok * p.group) * D + 8 * c);
+                    x[n][0] = __ldg(src);
+                    x[n][1] = __ldg(src + 1);
+                }
+            }
+            const int row = start + i * 128 + id;
+            l = row < rows ? -kLog2e * lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : -INFINITY;  // (no weight in columns without a row)
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+            const int s = i % kStages;
+            if (i >= kStages) wait_first(&q_free[s], (uint32_t)((i / kStages - 1) & 1), failed, status, 910);
+            unsigned char *dst = ring + (size_t)s * G::kOperand;
+#pragma unroll
+            for (int n = 0; n < G::kPieces; ++n) put_split<D>(x[n][0], x[n][1], dst, r0 + n * kStep, c);
+            if (i >= 2) wait_first(&s_free[i & 1], (uint32_t)((i / 2 - 1) & 1), failed, status, 911);  // (the log-sums before are read)
+            l_s[i & 1][id] = l;
+            bar_arrive(&l_full[i & 1]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(&q_full[s]);
+            if (i + 1 < steps) fetch(i + 1);
+        }
+    } else {
+        const int half = warp >> 2, key = key0 + (tid & 127);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint64_t scale_2 = two(scale * kLog2e, scale * kLog2e);
+        uint64_t sum[2] = {0ull, 0ull};
+        const int first = p.causal ? (key - past) * p.group : 0, key_max = key0 + (warp & 3) * 32 + 31;
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+            const int b = i & 1, r0 = start + i * 128;
+            wait_first(&l_full[b], (uint32_t)((i / 2) & 1), failed, status, 920);
+            wait_first(&s_full[b], (uint32_t)((i / 2) & 1), failed, status, 921);
+            __syncwarp();
+            tc_after();
+            uint32_t x[2][32];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_ld32_issue(tmem + lanes + (uint32_t)(b * 128 + 64 * half + 32 * c), x[c]);
+            tmem_ld_wait();
+            const bool masked = r0 + 128 > rows || (p.causal && past + r0 / p.group < key_max);
+            const int lo = first - r0 - 64 * half, hi = rows - r0 - 64 * half;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float v, w;
+                    apart(fma2(two(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), scale_2, *reinterpret_cast<const uint64_t *>(&l_s[b][64 * half + 32 * c + e])), v, w);
+                    v = ex2(v);
+                    w = ex2(w);
+                    const int col = 32 * c + e;
+                    if (masked) {
+                        v = col >= lo && col < hi ? v : 0.f;
+                        w = col + 1 >= lo && col + 1 < hi ? w : 0.f;
+                    }
+                    sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], two(v, w));
+                }
+            tc_before();
+            bar_arrive(&s_free[b]);  // (the scores and the log-sums)
+        }
+        float s0, s1;
+        apart(add2(sum[0], sum[1]), s0, s1);
+        part_s[half][tid & 127] = s0 + s1;
+    }
+    __syncthreads();
+    if (tid < kSplitKeys && key0 + tid < sq.kv_len && !*failed) p.mass[paged_row(p, table, kvh, key0 + tid)] += part_s[0][tid] + part_s[1][tid];
+    if (*failed && tid == 384) drain_mmas(&quiet);  // a wait gave up
+    tc_before();
+    __syncthreads();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
+}
+
 dim3 grid_of(const PagedMassArgs &a, const PagedView &v, int keys, int n) { return dim3((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)v.h_kv, (unsigned)n); }
 
 template <int D>
@@ -380,17 +582,30 @@ int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUten
         const int n = std::min(all.n_seq - s0, 32768);
         PagedView v = all;
         v.seqs += s0;
+        const bool few = a.min_rows <= kFewRows, many = a.max_rows > kFewRows;
         if (g.dtype == LUMEN_F32) {
-            const size_t bytes = (size_t)(std::min(FewMass<float, D>::kChunk, a.max_rows) + 7) / 8 * 8 * D * 6;
-            LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<float, D>, grid_of(a, v, FewMass<float, D>::kKeys, n), kFewThreads, bytes, s, v, static_cast<const float *>(a.q), a.scale, a.lse));
+            const auto *q = static_cast<const float *>(a.q);
+            if (few) {
+                const size_t bytes = (size_t)(std::min(FewMass<float, D>::kChunk, a.max_rows) + 7) / 8 * 8 * D * 6;
+                LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<float, D>, grid_of(a, v, FewMass<float, D>::kKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
+            }
+            if (many) {
+                static const int regs = [] {  // (what the warpgroups trade has to be there)
+                    cudaFuncAttributes attr;
+                    return cudaFuncGetAttributes(&attr, paged_mass_f32_kernel<D>) == cudaSuccess ? attr.numRegs : 0;
+                }();
+                if (regs * kSplitThreads < (2 * 128 + kRegsLoad + kRegsIssue) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention_mass: kernel built with %d registers", regs);
+                LUMEN_TRY(allow_smem(ctx, paged_mass_f32_kernel<D>, SplitMass<D>::kSmem));
+                LUMEN_TRY(launch_paged(ctx, paged_mass_f32_kernel<D>, grid_of(a, v, kSplitKeys, n), kSplitThreads, SplitMass<D>::kSmem, s, v, q, a.scale, a.lse, ctx->d_status));
+            }
             continue;
         }
         const auto *q = static_cast<const __nv_bfloat16 *>(a.q);
-        if (a.min_rows <= kFewRows) {
+        if (few) {
             const size_t bytes = (size_t)(std::min(kFewRows, a.max_rows) + 7) / 8 * 8 * D * 2;
             LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<__nv_bfloat16, D>, grid_of(a, v, FewMass<__nv_bfloat16, D>::kKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
         }
-        if (a.max_rows > kFewRows) {
+        if (many) {
             CUtensorMap q_map;
             const size_t row = (size_t)all.n_head * D;
             LUMEN_TRY(make_map_3d(ctx, &q_map, q, D, (size_t)all.n_head, D, (size_t)all.tokens, row, all.group, kTcRows / all.group));
