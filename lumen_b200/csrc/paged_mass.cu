@@ -38,7 +38,7 @@ struct FewMass {
 // shared memory in the order that this gives.  32 bits: three bf16 terms a number and the six largest of nine products, as in paged_few.cu.
 // grid (blocks of positions of the longest sequence, key heads, sequences)
 template <typename T, int D>
-__global__ void __launch_bounds__(kFewThreads) paged_mass_few_kernel(const PagedView p, const T *__restrict__ q, float scale, const float *__restrict__ lse) {
+__global__ void __launch_bounds__(kFewThreads, 4) paged_mass_few_kernel(const PagedView p, const T *__restrict__ q, float scale, const float *__restrict__ lse) {
     using G = FewMass<T, D>;
     constexpr int kTiles = G::kTiles, kTerms = G::kTerms, kGroups = G::kGroups, kPieces = G::kPieces;
     extern __shared__ uint2 q_s[];   // [blocks of 8 rows][tiles][32 lanes][terms]
