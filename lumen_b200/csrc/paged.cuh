@@ -55,6 +55,17 @@ int launch_paged(lumen_ctx *ctx, void (*kernel)(KA...), dim3 grid, unsigned thre
     return rc;
 }
 
+// The same for a kernel of clusters of `cluster` CTAs (1: none).
+template <typename... KA, typename... A>
+int launch_paged(lumen_ctx *ctx, void (*kernel)(KA...), unsigned cluster, dim3 grid, unsigned threads, size_t smem, cudaStream_t s, A... args) {
+    if (cluster == 1) return launch_paged(ctx, kernel, grid, threads, smem, s, args...);
+    const bool before = ctx->pdl;
+    ctx->pdl = true;
+    const int rc = launch_pdl_cluster(ctx, kernel, cluster, grid, dim3(threads), smem, s, args...);
+    ctx->pdl = before;
+    return rc;
+}
+
 struct PagedAppendArgs {
     const float *q, *k, *v, *q_norm, *k_norm, *cos_t, *sin_t;
     size_t q_stride, kv_stride;

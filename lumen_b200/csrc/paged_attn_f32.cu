@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
     volatile int *failed = &failed_s;
     const int tid = threadIdx.x, warp = tid >> 5;
     const PagedItem it = a.items[blockIdx.x];
-    const PagedSeq sq = p.seqs[it.seq];
+    const PagedSeq sq = it.sq;
     const int past = sq.kv_len - sq.q_len, nt = (it.key1 - it.key0 + kKeys - 1) / kKeys;
     if (tid == 0) {
         bar_init(&q_bar, 384);

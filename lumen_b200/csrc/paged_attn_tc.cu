@@ -95,7 +95,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     volatile int *failed = &failed_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedItem it = a.items[blockIdx.x];
-    const PagedSeq sq = p.seqs[it.seq];
+    const PagedSeq sq = it.sq;
     const int past = sq.kv_len - sq.q_len, nt = (it.key1 - it.key0 + kKeys - 1) / kKeys;
     const int active = min(QT, (it.rows + kMma - 1) / kMma);  // tiles of rows in use
     auto warps_of = [&](int q) { return min(4, (it.rows - q * kMma + 31) / 32); };  // of a tile, with rows

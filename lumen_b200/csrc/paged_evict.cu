@@ -1,9 +1,9 @@
 // Eviction: the positions of a sequence that received most attention, and its last ones, go to new pages.
 //
-// paged_select_kernel, a CTA per sequence and key head: the weights as ordered 32-bit integers, in shared memory where they fit; four passes over 8
-// bits each narrow the value of the last one that stays, and a last one writes the positions in order, of the equal ones the lowest.  The
-// histograms have a column per lane, so that the many equal weights (nothing at all, say) do not queue for one counter: whole numbers, so the
-// order of the atomics changes nothing.  paged_move_kernel copies the rows: bound by HBM.
+// paged_select_kernel, a CTA or a cluster of CTAs per sequence and key head: the weights as ordered 32-bit integers, in shared memory where they fit;
+// four passes over 8 bits each narrow the value of the last one that stays, and a last one writes the positions in order, of the equal ones the
+// lowest.  The histograms have a column per lane, so that the many equal weights (nothing at all, say) do not queue for one counter: whole
+// numbers, so the order of the atomics changes nothing.  paged_move_kernel copies the rows: bound by HBM.
 #include "paged.cuh"
 
 namespace lumen {
@@ -18,48 +18,86 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kHeld = 40 * 1024;  // weights that shared memory holds
+constexpr int kHeld = 40 * 1024;  // weights that the shared memory of a CTA holds
 
-// grid (key heads, sequences); HELD: the weights of every sequence fit (else they are read again in every pass)
+// The 32-bit number at the place of `mine` in the shared memory of a CTA of the cluster.
+__device__ __forceinline__ unsigned there(const unsigned *mine, unsigned rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// grid (CTAs of a cluster x key heads, sequences); HELD: the weights of every sequence fit (else they are read again in every pass).  Four
+// neighbouring positions a thread: bound by the instructions of its SMs.
 template <bool HELD>
-__global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView from, const PagedSeq *to_seqs, int recent, int *kept, size_t kept_stride) {
-    extern __shared__ uint32_t held[];
-    __shared__ unsigned hist[256][32], sums[256];
-    __shared__ unsigned prefix_s, want_s, above_s[kWarps], equal_s[kWarps];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.x, s = blockIdx.y;
+__global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView from, const PagedSeq *to_seqs, int recent, int *kept, size_t kept_stride, int ctas) {
+    extern __shared__ uint4 held[];
+    __shared__ __align__(16) unsigned hist[256][32];
+    __shared__ unsigned own[2][256], sums[256], prefix_s, want_s, above_s[kWarps], equal_s[kWarps], counts_s[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)blockIdx.x % ctas, kvh = (int)blockIdx.x / ctas, s = blockIdx.y;
     const PagedSeq sq = from.seqs[s];
     const int len = sq.kv_len, keep = to_seqs[s].kv_len, last = min(recent, keep), old = len - last, pick = keep - last;
+    const int all_groups = (old + 3) / 4, share = (all_groups + ctas - 1) / ctas, first = min(all_groups, rank * share), groups = min(all_groups, first + share) - first;
     const int *table = from.tables + sq.table;
     int *out = kept + ((size_t)s * from.h_kv + kvh) * kept_stride;
     pdl_launch();
     pdl_wait();
-    for (int i = tid; i < last; i += kThreads) out[pick + i] = old + i;
-    if (pick == 0) return;
-    auto fetch = [&](int pos) { return order_of(from.mass[paged_row(from, table, kvh, pos)]); };
-    auto value = [&](int pos) { return HELD ? held[pos] : fetch(pos); };
-    if (HELD)
-#pragma unroll 4
-        for (int i = tid; i < old; i += kThreads) held[i] = fetch(i);
+    for (int i = rank * kThreads + tid; i < last; i += ctas * kThreads) out[pick + i] = old + i;
+    if (pick == 0) return;  // (of the whole cluster)
+    auto fetch = [&](int group) {  // (a page holds whole groups; what of the last group lies behind `old` is left out where it is used)
+        const float4 m = *reinterpret_cast<const float4 *>(from.mass + paged_row(from, table, kvh, 4 * (first + group)));
+        return make_uint4(order_of(m.x), order_of(m.y), order_of(m.z), order_of(m.w));
+    };
+    auto value = [&](int group) { return HELD ? held[group] : fetch(group); };
+    auto rest = [&](int group) { return old - 4 * (first + group); };  // positions from the group's first on
     // the pick-th largest value: `prefix` are its leading bits, `want` how many of those that share them are still to be taken
-    if (tid == 0) prefix_s = 0u, want_s = (unsigned)pick;
+    uint32_t prefix = 0u;
+    unsigned want = (unsigned)pick;
     for (int shift = 24; shift >= 0; shift -= 8) {
 #pragma unroll
-        for (int i = 0; i < 256 * 32 / kThreads; ++i) (&hist[0][0])[tid + i * kThreads] = 0u;
+        for (int i = 0; i < 256 * 8 / kThreads; ++i) reinterpret_cast<uint4 *>(&hist[0][0])[tid + i * kThreads] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
-        const unsigned prefix = prefix_s;
-        for (int i = tid; i < old; i += kThreads) {
-            const uint32_t u = value(i);
-            if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u][lane], 1u);
+        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+        auto count = [&](uint32_t u, bool live) {
+            if (live && (u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255u][lane], 1u);
+        };
+        if (HELD && shift == 24) {
+#pragma unroll 4
+            for (int i = tid; i < groups; i += kThreads) held[i] = fetch(i);  // (a thread reads back what it wrote itself)
+        }
+#pragma unroll 2
+        for (int i = tid; i < groups; i += kThreads) {
+            const uint4 u = value(i);
+            const int n = rest(i);
+            count(u.x, true);
+            count(u.y, n > 1);
+            count(u.z, n > 2);
+            count(u.w, n > 3);
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 256 / kWarps; ++i) {
-            const int bin = warp * (256 / kWarps) + i;
-            const unsigned c = __reduce_add_sync(0xffffffffu, hist[bin][lane]);
-            if (lane == 0) sums[bin] = c;
+        unsigned *mine_s = ctas > 1 ? own[(shift >> 3) & 1] : sums;
+        {  // four threads a counter
+            const uint4 *row = reinterpret_cast<const uint4 *>(&hist[tid >> 2][(tid & 3) * 8]);
+            const uint4 x = row[0], y = row[1];
+            unsigned c = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
+            c += __shfl_xor_sync(0xffffffffu, c, 1);
+            c += __shfl_xor_sync(0xffffffffu, c, 2);
+            if ((tid & 3) == 0) mine_s[tid >> 2] = c;
+        }
+        if (ctas > 1) {  // (two sets in turn: the one of the pass before may still be read)
+            cluster_meet();
+            if (tid < 256) {
+                unsigned c = 0u;
+                for (int r = 0; r < ctas; ++r) c += there(&mine_s[tid], (unsigned)r);
+                sums[tid] = c;
+            }
         }
         __syncthreads();
-        if (warp == 0) {  // lane l: bins 255 - 8 l down to 248 - 8 l
+        if (warp == 0) {  // lane l has the bins 255 - 8 l down to 248 - 8 l
             unsigned c[8], mine = 0u;
 #pragma unroll
             for (int i = 0; i < 8; ++i) c[i] = sums[255 - 8 * lane - i], mine += c[i];
@@ -69,44 +107,74 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView 
                 const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += y;
             }
-            const unsigned want = want_s;
             unsigned before = incl - mine;
-            __syncwarp();
-            if (before < want && want <= incl)
+            if (before < want && want <= incl) {  // (of exactly one lane)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (before < want && want <= before + c[i]) {
-                        prefix_s = prefix | ((unsigned)(255 - 8 * lane - i) << shift);
+                        prefix_s = prefix | (unsigned)(255 - 8 * lane - i) << shift;
                         want_s = want - before;
                     }
                     before += c[i];
                 }
+            }
         }
         __syncthreads();
+        prefix = prefix_s;
+        want = want_s;
     }
-    const unsigned edge = prefix_s, ties = want_s;  // all above `edge` stay, and the first `ties` equal to it
-    // every warp has a run of positions: it counts them, learns what the warps before it have, and writes its own
-    const int run = ((old + kWarps - 1) / kWarps + 31) & ~31, lo = min(old, warp * run), hi = min(old, lo + run);
-    unsigned above = 0u, equal = 0u;
+    const uint32_t edge = prefix;  // all above it stay, and the first `want` equal to it
+    // every warp has a run of groups: it counts them, learns what the warps and CTAs before it have, and writes its own
+    const int run = ((groups + kWarps - 1) / kWarps + 31) & ~31, lo = min(groups, warp * run), hi = min(groups, lo + run);
+    auto kinds = [&](int i, unsigned &gt, unsigned &eq) {  // a bit for each of the four positions
+        gt = eq = 0u;
+        if (i >= hi) return;
+        const uint4 u = value(i);
+        const unsigned live = rest(i) >= 4 ? 15u : (1u << rest(i)) - 1u;
+        gt = ((u.x > edge) | (u.y > edge) << 1 | (u.z > edge) << 2 | (u.w > edge) << 3) & live;
+        eq = ((u.x == edge) | (u.y == edge) << 1 | (u.z == edge) << 2 | (u.w == edge) << 3) & live;
+    };
+    unsigned above = 0u, equal = 0u, gt, eq;
     for (int i0 = lo; i0 < hi; i0 += 32) {
-        const uint32_t u = i0 + lane < hi ? value(i0 + lane) : 0u;
-        above += __popc(__ballot_sync(0xffffffffu, i0 + lane < hi && u > edge));
-        equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < hi && u == edge));
+        kinds(i0 + lane, gt, eq);
+        above += __popc(gt);
+        equal += __popc(eq);
     }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) above_s[warp] = above, equal_s[warp] = equal;
     __syncthreads();
-    above = __reduce_add_sync(0xffffffffu, lane < warp ? above_s[lane] : 0u);
-    equal = __reduce_add_sync(0xffffffffu, lane < warp ? equal_s[lane] : 0u);
+    const unsigned before_above = __reduce_add_sync(0xffffffffu, lane < warp ? above_s[lane] : 0u), before_equal = __reduce_add_sync(0xffffffffu, lane < warp ? equal_s[lane] : 0u);
+    if (ctas > 1) {
+        if (warp == kWarps - 1 && lane == 0) counts_s[0] = before_above + above, counts_s[1] = before_equal + equal;
+        cluster_meet();
+    }
+    above = before_above;
+    equal = before_equal;
+    for (int r = 0; r < rank; ++r) above += there(&counts_s[0], (unsigned)r), equal += there(&counts_s[1], (unsigned)r);
     for (int i0 = lo; i0 < hi; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t u = i < hi ? value(i) : 0u;
-        const bool gt = i < hi && u > edge, eq = i < hi && u == edge;
-        const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq), low = (1u << lane) - 1u;
-        const unsigned g = above + (unsigned)__popc(mg & low), e = equal + (unsigned)__popc(me & low);
-        if (gt || (eq && e < ties)) out[g + min(e, ties)] = i;
-        above += (unsigned)__popc(mg);
-        equal += (unsigned)__popc(me);
+        kinds(i, gt, eq);
+        const unsigned mine = (unsigned)__popc(gt) | (unsigned)__popc(eq) << 16;  // (at most 128 of each)
+        unsigned incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        unsigned g = above + ((incl - mine) & 0xffffu), e = equal + ((incl - mine) >> 16);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const bool is_gt = (gt >> x) & 1u, is_eq = (eq >> x) & 1u;
+            if (is_gt || (is_eq && e < want)) out[g + min(e, want)] = 4 * (first + i) + x;
+            g += is_gt;
+            e += is_eq;
+        }
+        const unsigned all = __shfl_sync(0xffffffffu, incl, 31);
+        above += all & 0xffffu;
+        equal += all >> 16;
     }
+    if (ctas > 1) cluster_meet();  // (the counts may still be read by the CTAs behind)
 }
 
 // grid (groups of rows, key heads, sequences): 16 bytes a thread
@@ -146,13 +214,14 @@ int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from
         f.seqs += s0;
         t.seqs += s0;
         int *k = kept + (size_t)s0 * from.h_kv * kept_stride;
-        const dim3 grid((unsigned)from.h_kv, (unsigned)n);
-        if (max_len <= kHeld) {
-            LUMEN_TRY(raise_smem_limit(ctx, reinterpret_cast<const void *>(paged_select_kernel<true>), kHeld * 4));
-            LUMEN_TRY(launch_paged(ctx, paged_select_kernel<true>, grid, kThreads, (size_t)max_len * 4, s, f, t.seqs, recent, k, kept_stride));
-        } else {
-            LUMEN_TRY(launch_paged(ctx, paged_select_kernel<false>, grid, kThreads, 0, s, f, t.seqs, recent, k, kept_stride));
-        }
+        // Long sequences, where there are SMs for it: four each (with the copy, 32 rows of 16384 positions 32 us, with one SM each 35, with eight, two
+        // CTAs an SM, 59); short ones: the cluster's meetings cost what they save.
+        const int ctas = max_len > 4096 && 4LL * from.h_kv * n <= 2LL * ctx->num_sms ? 4 : 1, held = ((max_len + 3) / 4 + ctas - 1) / ctas;
+        const dim3 grid((unsigned)(ctas * from.h_kv), (unsigned)n);
+        auto *kernel = held * 4 <= kHeld ? paged_select_kernel<true> : paged_select_kernel<false>;
+        const size_t smem = held * 4 <= kHeld ? (size_t)held * 16 : 0;
+        if (smem) LUMEN_TRY(raise_smem_limit(ctx, reinterpret_cast<const void *>(kernel), kHeld * 4));
+        LUMEN_TRY(launch_paged(ctx, kernel, (unsigned)ctas, grid, kThreads, smem, s, f, t.seqs, recent, k, kept_stride, ctas));
         LUMEN_TRY(bytes == 128 ? move<128>(ctx, f, t, n, max_keep, k, kept_stride, s)
                   : bytes == 256 ? move<256>(ctx, f, t, n, max_keep, k, kept_stride, s) : move<512>(ctx, f, t, n, max_keep, k, kept_stride, s));
     }

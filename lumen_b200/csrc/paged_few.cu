@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_few_kernel(co
     __shared__ float m_s[kWarps][NB * 8], l_s[kWarps][NB * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const PagedItem it = a.items[blockIdx.x];
-    const PagedSeq sq = p.seqs[it.seq];
+    const PagedSeq sq = it.sq;
     const int *table = p.tables + sq.table;
     const int past = sq.kv_len - sq.q_len;
     const float scale2 = a.scale * kLog2e;
@@ -336,7 +336,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
     __shared__ float o_s[WIDE ? kJoinWarps : 1][D], l_s[kJoinWarps];
     const PagedJoin j = a.joins[blockIdx.x];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = WIDE ? (int)blockIdx.y : (int)(blockIdx.y * kJoinWarps) + warp;
-    const PagedSeq sq = p.seqs[j.seq];
     pdl_launch();
     pdl_wait();
     if (r >= j.rows) return;
@@ -373,7 +372,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
         }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const size_t o = (size_t)(sq.tok0 + (j.row0 + r) / p.group) * p.n_head + j.kvh * p.group + (j.row0 + r) % p.group;
+    const size_t o = (size_t)(j.tok0 + (j.row0 + r) / p.group) * p.n_head + j.kvh * p.group + (j.row0 + r) % p.group;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] *= inv;
     if (a.out_dtype == LUMEN_F32) {

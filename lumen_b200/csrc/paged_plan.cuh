@@ -26,11 +26,13 @@ struct PagedSeq {
 // Rows of one key head of a sequence: row r is new token r / group, query head kvh * group + r % group.  An item is `rows` of them from row0
 // against the cached positions [key0, key1); part < 0: the result is final, else its partial sums are rows part .. part + rows - 1.
 struct PagedItem {
-    int seq, kvh, row0, rows, key0, key1, part, pad;
+    int seq, kvh, row0, rows, key0, key1, part;
+    PagedSeq sq;  // (its own copy: a kernel starts with one read, not two in turn)
+    int pad;
 };
 // Rows whose partial sums are joined: split i's are the rows from part + i * rows.
 struct PagedJoin {
-    int seq, kvh, row0, rows, part, splits;
+    int seq, kvh, row0, rows, part, splits, tok0, pad;
 };
 // What a kernel takes per item: its rows, the granularity in which it walks the positions, items that run at once.
 struct PagedShape {
@@ -137,7 +139,7 @@ inline void paged_cut(PagedPlan &p, const PagedGeom &g, const PagedShape &shape,
         const int rows = q.q_len * p.group;
         for (int r = 0; r < rows; r += shape.rows) {
             const int n = std::min(shape.rows, rows - r), end = paged_visible(p, q, (r + n - 1) / p.group), tiles = (end + shape.keys - 1) / shape.keys;
-            for (int h = 0; h < g.h_kv; ++h) base.push_back({{s, h, r, n, 0, end, -1, 0}, tiles}), work += tiles;
+            for (int h = 0; h < g.h_kv; ++h) base.push_back({{s, h, r, n, 0, end, -1, q, 0}, tiles}), work += tiles;
         }
     }
     if (base.empty()) return;
@@ -171,7 +173,7 @@ inline void paged_cut(PagedPlan &p, const PagedGeom &g, const PagedShape &shape,
             p.items.push_back(b.it);
             continue;
         }
-        p.joins.push_back({b.it.seq, b.it.kvh, b.it.row0, b.it.rows, (int)p.part_rows, splits});
+        p.joins.push_back({b.it.seq, b.it.kvh, b.it.row0, b.it.rows, (int)p.part_rows, splits, b.it.sq.tok0, 0});
         for (int i = 0; i < splits; ++i) {  // part i: tiles [i * tiles / splits, (i + 1) * tiles / splits)
             PagedItem it = b.it;
             it.key0 = (int)((long long)b.tiles * i / splits) * shape.keys;

@@ -442,7 +442,7 @@ def _chosen(m, keep, recent):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128)], ids=str)
 @pytest.mark.parametrize("kv,keep,recent", [([1], [1], 0), ([1], [0], 3), ([64, 0, 3000, 65], [13, 0, 1500, 65], 16), ([5000], [4999], 0), ([2049, 300], [1, 200], 1000),
-                                            ([1500, 40], [700, 39], 1)])
+                                            ([1500, 40], [700, 39], 1), ([6000, 7, 0, 4500], [2000, 7, 0, 4499], 30)])
 @pytest.mark.parametrize("kind", ["smooth", "ties", "wild"])
 def test_evict(L, dtype, heads, kv, keep, recent, kind):
     w = World(L, dtype, heads, 32, [0] * len(kv), kv, extra=keep)
@@ -475,18 +475,21 @@ def test_evict(L, dtype, heads, kv, keep, recent, kind):
         assert torch.equal(got.nan_to_num(5.0, 6.0, 7.0), t.nan_to_num(5.0, 6.0, 7.0))
 
 
-def test_evict_from_a_cache_too_long_for_shared_memory(L):
-    w = World(L, "f32", (4, 2, 64), 256, [0, 0], [45000, 100], extra=[900, 100])
-    w.put(w.mass, 0, (torch.rand(45000, 2, generator=w.g, device=DEV) * 5000).floor())
-    kept = torch.full((2, 2, 900), -7, dtype=torch.int32, device=DEV)
+@pytest.mark.parametrize("n", [4096, 4097, 45000, 333000])
+@pytest.mark.parametrize("keep", [900, 4000])
+def test_evict_from_long_caches(L, n, keep):
+    """By one SM, by several, and too long for their shared memory."""
+    w = World(L, "f32", (4, 2, 64), 256, [0, 0], [n, 100], extra=[keep, 100])
+    w.put(w.mass, 0, (torch.rand(n, 2, generator=w.g, device=DEV) * 5000).floor())
+    kept = torch.full((2, 2, keep), -7, dtype=torch.int32, device=DEV)
     torch.cuda.synchronize()
-    L.paged_evict(w.pool, w.batch(), w.batch(kv_lens=[900, 100], tables=w.extra_tables), 100, kept.data_ptr(), 900)
+    L.paged_evict(w.pool, w.batch(), w.batch(kv_lens=[keep, 100], tables=w.extra_tables), 100, kept.data_ptr(), keep)
     w.pool.ctx.synchronize()
-    m = w.rows(w.mass, w.tables[0], 45000).cpu().numpy()
+    m = w.rows(w.mass, w.tables[0], n).cpu().numpy()
     for h in range(2):
-        stay = _chosen(m[:, h], 900, 100)
+        stay = _chosen(m[:, h], keep, 100)
         assert kept[0, h].tolist() == stay.tolist() and kept[1, h, :100].tolist() == list(range(100))
-        assert torch.equal(w.rows(w.v, w.extra_tables[0], 900)[:, h], w.rows(w.v, w.tables[0], 45000)[torch.as_tensor(stay, device=DEV), h])
+        assert torch.equal(w.rows(w.v, w.extra_tables[0], keep)[:, h], w.rows(w.v, w.tables[0], n)[torch.as_tensor(stay, device=DEV), h])
 
 
 # ---- refusals ------------------------------------------------------------------------------------------------------
