@@ -89,7 +89,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     // the swizzle pattern repeats every 1024 bytes
     unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *ring = q_s + QT * G::kQBytes;  // stage: keys, values
-    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers * G::kHalves], o_bar[QT][G::kBuffers], quiet[QT];
+    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[QT][G::kBuffers], p_bar[QT][G::kBuffers * G::kHalves], o_bar[QT][G::kBuffers], quiet[QT], dead_bar;
     __shared__ uint32_t tmem_base_s;
     __shared__ int failed_s;
     volatile int *failed = &failed_s;
@@ -111,6 +111,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             for (int i = 0; i < G::kBuffers * G::kHalves; ++i) bar_init(&p_bar[q][i], (uint32_t)(32 * warps_of(q)));
         }
         bar_init(&q_bar, (uint32_t)loaders);
+        bar_init(&dead_bar, (uint32_t)(32 * warps_of(0)));  // the last tile's dead rows are zeroes
         for (int s = 0; s < kStages; ++s) {
             bar_init(&k_full[s], 1);
             bar_init(&v_full[s], 1);
@@ -204,7 +205,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 for (int h = 0; h < G::kHalves; ++h) {
                     bool ok = wait_warp(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
                     // (the values' dead rows are zeroed by the first tile's warps)
-                    if (QT == 2 && ok && h == 0 && q == 1 && it.key0 + (j + 1) * kKeys > it.key1) ok = wait_warp(&p_bar[0][0], (uint32_t)(j & 1), failed, status, 722);
+                    if (QT == 2 && ok && h == 0 && q == 1 && it.key0 + (j + 1) * kKeys > it.key1) ok = wait_warp(&dead_bar, 0, failed, status, 722);
                     if (ok && h == 0) ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
                     tc_after();
                     if (ok) {
@@ -354,6 +355,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         *reinterpret_cast<uint4 *>(v + (c / 8) * G::kTile + pos * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    bar_arrive(&dead_bar);
                 }
 #pragma unroll
                 for (int h = 0; h < kKeys / 64; ++h) {
