@@ -210,6 +210,12 @@ public:
         check(lumen_rope_new(ctx.get(), dim, max_seq_len, theta, &r), ctx.get());
         h_.reset(r, [](lumen_rope *p) { lumen_rope_free(p); });
     }
+    // The caller's own tables [max_seq_len, dim / 2]; no counterpart in the reference.
+    static RotaryEmbedding from_tables(const Context &ctx, size_t dim, size_t max_seq_len, const float *cos, const float *sin) {
+        lumen_rope *r = nullptr;
+        check(lumen_rope_from_tables(ctx.get(), dim, max_seq_len, cos, sin, &r), ctx.get());
+        return RotaryEmbedding(ctx, r);
+    }
     Tensor forward(const Tensor &x_bhsd, size_t offset) const {
         lumen_tensor *out = nullptr;
         check(lumen_rope_forward(h_.get(), x_bhsd.get(), offset, &out), ctx_.get());
@@ -218,6 +224,7 @@ public:
     lumen_rope *get() const { return h_.get(); }
 
 private:
+    RotaryEmbedding(const Context &ctx, lumen_rope *owned) : ctx_(ctx), h_(owned, [](lumen_rope *p) { lumen_rope_free(p); }) {}
     Context ctx_;
     std::shared_ptr<lumen_rope> h_;
 };
@@ -241,6 +248,58 @@ private:
     Context ctx_{};
     std::shared_ptr<lumen_kv_cache> h_;
 };
+
+// Pages of one layer of a paged cache, and the sequences of one step (lumen_page_*, lumen_paged_*); no counterpart in the reference.
+class PagePool {
+public:
+    PagePool(const Context &ctx, size_t pages, size_t page_size, size_t h_kv, size_t d, lumen_dtype dtype) : ctx_(ctx) {
+        lumen_page_pool *p = nullptr;
+        check(lumen_page_pool_new(ctx.get(), pages, page_size, h_kv, d, dtype, &p), ctx.get());
+        h_.reset(p, [](lumen_page_pool *x) { lumen_page_pool_free(x); });
+    }
+    void *k() const { return lumen_page_pool_k(get()); }
+    void *v() const { return lumen_page_pool_v(get()); }
+    float *mass() const { return lumen_page_pool_mass(get()); }
+    lumen_page_pool *get() const { return h_.get(); }
+    const Context &context() const { return ctx_; }
+
+private:
+    Context ctx_;
+    std::shared_ptr<lumen_page_pool> h_;
+};
+
+class PageBatch {
+public:
+    // tables: [sequences][table_stride] page numbers; first_pos may be empty
+    PageBatch(const PagePool &pool, size_t n_head, const std::vector<int32_t> &q_lens, const std::vector<int32_t> &kv_lens, const std::vector<int32_t> &tables,
+              size_t table_stride, const std::vector<int32_t> &first_pos = {}, bool causal = true) {
+        if (kv_lens.size() != q_lens.size() || tables.size() != q_lens.size() * table_stride || (!first_pos.empty() && first_pos.size() != q_lens.size()))
+            throw Error(LUMEN_ERR_SHAPE, "PageBatch: lengths and tables of different numbers of sequences");
+        lumen_page_batch *b = nullptr;
+        check(lumen_page_batch_new(pool.get(), n_head, q_lens.size(), q_lens.data(), kv_lens.data(), first_pos.empty() ? nullptr : first_pos.data(), tables.data(),
+                                   table_stride, causal, &b), pool.context().get());
+        h_.reset(b, [](lumen_page_batch *x) { lumen_page_batch_free(x); });
+    }
+    lumen_page_batch *get() const { return h_.get(); }
+
+private:
+    std::shared_ptr<lumen_page_batch> h_;
+};
+
+// Device pointers, as of lumen_paged_append, lumen_paged_attention, lumen_paged_attention_mass and lumen_paged_evict.
+inline void paged_append(const PagePool &pool, const PageBatch &batch, const RotaryEmbedding *rope, const float *q, const float *k, const float *v, size_t q_stride,
+                         size_t kv_stride, void *q_out, const float *q_norm = nullptr, const float *k_norm = nullptr, float eps = 0.f) {
+    check(lumen_paged_append(pool.get(), batch.get(), rope ? rope->get() : nullptr, q, k, v, q_stride, kv_stride, q_norm, k_norm, eps, q_out), pool.context().get());
+}
+inline void paged_attention(const PagePool &pool, const PageBatch &batch, const void *q, float scale, void *out, lumen_dtype out_dtype, float *lse = nullptr) {
+    check(lumen_paged_attention(pool.get(), batch.get(), q, scale, out, out_dtype, lse), pool.context().get());
+}
+inline void paged_attention_mass(const PagePool &pool, const PageBatch &batch, const void *q, float scale, const float *lse) {
+    check(lumen_paged_attention_mass(pool.get(), batch.get(), q, scale, lse), pool.context().get());
+}
+inline void paged_evict(const PagePool &pool, const PageBatch &from, const PageBatch &to, size_t recent, int32_t *kept, size_t kept_stride) {
+    check(lumen_paged_evict(pool.get(), from.get(), to.get(), recent, kept, kept_stride), pool.context().get());
+}
 
 // LlamaKVCache (src/kv_cache.rs:14-59)
 class LlamaKVCache {
