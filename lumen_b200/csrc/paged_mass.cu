@@ -199,10 +199,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * kTcKeys, past = sq.kv_len - sq.q_len;
-    if (key0 >= sq.kv_len || rows <= kFewRows) {
-        pdl_launch();
-        return pdl_wait();
-    }
+    if (key0 >= sq.kv_len || rows <= kFewRows) return pdl_wait();
     const int per = kTcRows / p.group, n_rows = per * p.group;  // tokens and rows of a step
     const int start_tok = p.causal ? max(0, key0 - past) : 0, start = start_tok * p.group, steps = (sq.q_len - start_tok + per - 1) / per;  // (start < rows: key0 < kv_len)
     const int tiles = min(2, (sq.kv_len - key0 + 127) / 128);  // of 128 positions
@@ -422,10 +419,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
     const int tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * kSplitKeys, past = sq.kv_len - sq.q_len;
-    if (key0 >= sq.kv_len || rows <= kFewRows) {
-        pdl_launch();
-        return pdl_wait();
-    }
+    if (key0 >= sq.kv_len || rows <= kFewRows) return pdl_wait();
     const int start = p.causal ? max(0, key0 - past) * p.group : 0, steps = (rows - start + 127) / 128;  // (start < rows: key0 < kv_len)
     const int *table = p.tables + sq.table;
     if (tid == 0) {
