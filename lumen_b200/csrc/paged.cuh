@@ -66,6 +66,11 @@ int launch_paged(lumen_ctx *ctx, void (*kernel)(KA...), unsigned cluster, dim3 g
     return rc;
 }
 
+#ifdef __CUDACC__
+// Lets the next kernel start.  Kernels that take tensor memory call it behind their own allocation (the next one may take some before it waits).
+__device__ __forceinline__ void paged_start_next() { pdl_launch(); }
+#endif
+
 struct PagedAppendArgs {
     const float *q, *k, *v, *q_norm, *k_norm, *cos_t, *sin_t;
     size_t q_stride, kv_stride;

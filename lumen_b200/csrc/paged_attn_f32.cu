@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_base_s;
-    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    paged_start_next();
     pdl_wait();
     auto load_queries = [&](int id, int n) {  // split, in the swizzled layout; rows behind the item's: zeros
         for (int i = id; i < kRowsTile * (D / 8); i += n) {

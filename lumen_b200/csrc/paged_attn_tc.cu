@@ -130,7 +130,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_s;
-    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    paged_start_next();
     pdl_wait();
     int k_issued = 0, v_issued = 0;  // tiles whose copies are on their way (producer warp)
 
@@ -416,7 +416,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             drain_ring(k_full, kStages, k_issued);
             drain_ring(v_full, kStages, v_issued);
         } else if (warp >= QT * 4 && warp < QT * 5 && lane == 0) {
-            drain_mmas(&quiet[warp - QT * 4]);
+            uint64_t &ended = quiet[warp - QT * 4];
+            drain_mmas(&ended);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

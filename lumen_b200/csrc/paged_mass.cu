@@ -232,7 +232,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_s;  // scores: tile 0 even, odd steps, tile 1 even, odd steps
-    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    paged_start_next();
     pdl_wait();
 
     int q_issued = 0;
@@ -364,7 +364,8 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             drain_ring(&k_bar, 1, 1);
             drain_ring(q_full, kTcStages, q_issued);
         } else if (tid == kTcExps || tid == kTcExps + 32) {
-            drain_mmas(&quiet[(tid - kTcExps) / 32]);
+            uint64_t &ended = quiet[(tid - kTcExps) / 32];
+            drain_mmas(&ended);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
     tc_before();
     __syncthreads();
     tc_after();
-    pdl_launch();  // (behind the allocation: the next kernel may take tensor memory before it waits)
+    paged_start_next();
     const uint32_t tmem = tmem_base_s;  // scores of even and odd steps
 
     if (warp >= 12) {

@@ -127,3 +127,19 @@ def test_every_row_meets_every_position_once(plan, seed):
 def test_few_long_sequences_fill_the_slots(plan):
     rc, _, _, items, joins = plan([(1, 16000, list(range(250)))], pages=250, page=64, h_kv=8, n_head=32, slots=148)
     assert rc == OK and 120 <= len(items) <= 148 and len(joins) == 8
+
+
+def test_kernels_let_the_next_start_behind_their_allocation():
+    """As the other kernels that take tensor memory: every CTA has its own by the time it lets the next kernel start, and waits for the kernel before on
+    every way out."""
+    seen = 0
+    for p in sorted((ROOT / "lumen_b200" / "csrc").glob("paged*.cu")):
+        for body in p.read_text().split("__global__")[1:]:
+            assert "pdl_wait();" in body, p.name
+            if "tcgen05.alloc" in body:
+                between = body[body.index("tcgen05.alloc"): body.index("paged_start_next();")]
+                assert "tcgen05.relinquish_alloc_permit" in between and "__syncthreads()" in between, p.name
+                for early in body[: body.index("tcgen05.alloc")].split("return")[1:]:
+                    assert early.startswith(" pdl_wait();") or not early.startswith(";"), p.name
+                seen += 1
+    assert seen == 4
