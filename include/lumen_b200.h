@@ -394,13 +394,13 @@ int lumen_page_batch_free(lumen_page_batch *batch);
  * q_norm / k_norm [d] (NULL: none; rms_norm.rs:49-56), then the rotation of rope (NULL: none; encoding.rs:195-203);
  * q goes to q_out[tokens, n_head, d], k and v to their slots, all of the pool's type, each rounded once; the slots'
  * attention weight becomes 0.  Refused: pages that receive new rows and also belong to another sequence, positions
- * beyond the tables (LUMEN_ERR_ROPE_RANGE).  q_out: 16-byte aligned. */
+ * beyond the tables (LUMEN_ERR_ROPE_RANGE), rows that overlap one another or q_out.  q_out: 16-byte aligned. */
 int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, const lumen_rope *rope, const float *q_dev, const float *k_dev,
                        const float *v_dev, size_t q_stride, size_t kv_stride, const float *q_norm_dev, const float *k_norm_dev, float eps,
                        void *q_out_dev);
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the positions that token t sees, query head h reading key head
- * h / (n_head / h_kv).  q: the pool's type; out: f32, or bf16 from a bf16 pool; [tokens, n_head, d], 16-byte aligned, not
- * overlapping.  lse (NULL: not wanted): f32 [tokens, n_head], log of the sum of exp(scale * q . k).  A token that sees nothing
+ * h / (n_head / h_kv).  q: the pool's type; out: f32, or bf16 from a bf16 pool; [tokens, n_head, d], 16-byte aligned; q, out
+ * and lse may not overlap.  lse (NULL: not wanted): f32 [tokens, n_head], log of the sum of exp(scale * q . k).  A token that sees nothing
  * gives zeros and -infinity.  Sums and softmax in f32; from a bf16 pool the weights are rounded to bf16 before they
  * meet the values; an f32 pool is computed with all 24 bits.  Slots behind a sequence's end may hold anything. A value that is not
  * finite, in a slot of the sequence, can reach every token whose call reads that slot. */

@@ -35,6 +35,12 @@ PagedView view_of(const lumen_page_pool *pool, const lumen_page_batch *b) {
     return v;
 }
 
+// Whether two ranges of device memory have bytes in common.
+bool meet(const void *a, size_t na, const void *b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na && nb && x < y + nb && y < x + na;
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_pair(const lumen_page_pool *pool, const lumen_page_batch *b, const char *what) {
@@ -143,6 +149,18 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         paged_cut(p, b->g, paged_few_shape(ctx->num_sms), few);
         b->n_few = (int)p.items.size();
         paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, ctx->num_sms) : paged_f32_shape(ctx->num_sms), many);
+        for (size_t i = 0; i < p.items.size(); ++i) {
+            int &rows = (int)i < b->n_few ? b->few_rows : b->many_rows;
+            rows = std::max(rows, p.items[i].rows);
+        }
+        for (const PagedJoin &j : p.joins) b->join_rows = std::max(b->join_rows, j.rows), b->join_splits = std::max(b->join_splits, j.splits);
+        for (const PagedSeq &q : p.seqs)
+            if (q.q_len && q.kv_len) {
+                const int rows = q.q_len * p.group;
+                b->seen_kv = std::max(b->seen_kv, q.kv_len);
+                b->min_rows = b->max_rows ? std::min(b->min_rows, rows) : rows;
+                b->max_rows = std::max(b->max_rows, rows);
+            }
         // everything the kernels read goes up in one copy, in front of the workspace
         std::vector<char> up;
         auto put = [&](const void *data, size_t bytes) {
@@ -212,6 +230,10 @@ int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, con
             return set_error(ctx, LUMEN_ERR_ROPE_RANGE, "RoPE index out of range: pos %lld >= max %zu", p.max_pos, rope->max_seq);
     }
     if (p.tokens == 0) return LUMEN_OK;
+    const size_t q_span = ((size_t)(p.tokens - 1) * q_stride + p.n_head * d) * 4, kv_span = ((size_t)(p.tokens - 1) * kv_stride + pool->g.h_kv * d) * 4;
+    const size_t out_bytes = (size_t)p.tokens * p.n_head * d * (pool->g.dtype == LUMEN_F32 ? 4 : 2);
+    if (meet(q_out_dev, out_bytes, q_dev, q_span) || meet(q_out_dev, out_bytes, k_dev, kv_span) || meet(q_out_dev, out_bytes, v_dev, kv_span))
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: q_out overlaps the rows that are read");
     OnDevice on(ctx);
     PagedAppendArgs a = {};
     a.q = q_dev; a.k = k_dev; a.v = v_dev; a.q_norm = q_norm_dev; a.k_norm = k_norm_dev;
@@ -230,24 +252,22 @@ int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *b
         return set_error(ctx, LUMEN_ERR_DTYPE, "paged_attention: output type %d from a pool of type %d", (int)out_dtype, (int)pool->g.dtype);
     if (!aligned16(q_dev) || !aligned16(out_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q or out is not 16-byte aligned");
     if (!(scale - scale == 0.f)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: scale is not finite");
-    const size_t n = (size_t)p.tokens * p.n_head * pool->g.d;
-    const char *q0 = static_cast<const char *>(q_dev), *o0 = static_cast<const char *>(out_dev);
-    if (q0 < o0 + n * (out_dtype == LUMEN_F32 ? 4 : 2) && o0 < q0 + n * (pool->g.dtype == LUMEN_F32 ? 4 : 2))
-        return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q and out overlap");
+    const size_t rows = (size_t)p.tokens * p.n_head, q_bytes = rows * pool->g.d * (pool->g.dtype == LUMEN_F32 ? 4 : 2), out_bytes = rows * pool->g.d * (out_dtype == LUMEN_F32 ? 4 : 2);
+    if (meet(q_dev, q_bytes, out_dev, out_bytes) || (lse_dev && (meet(q_dev, q_bytes, lse_dev, rows * 4) || meet(out_dev, out_bytes, lse_dev, rows * 4))))
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q, out and lse overlap");
     if (p.tokens == 0) return LUMEN_OK;
     OnDevice on(ctx);
     PagedAttnArgs a = {};
     a.q = q_dev; a.scale = scale; a.out = out_dev; a.out_dtype = out_dtype; a.lse = lse_dev;
     a.part = batch->part; a.part_rows = p.part_rows; a.joins = batch->joins; a.n_joins = (int)p.joins.size();
-    for (const PagedJoin &j : p.joins) a.join_rows = std::max(a.join_rows, j.rows), a.join_splits = std::max(a.join_splits, j.splits);
+    a.join_rows = batch->join_rows; a.join_splits = batch->join_splits;
     const PagedView v = view_of(pool, batch);
     for (int many = 0; many < 2; ++many) {
         const int first = many ? batch->n_few : 0, last = many ? (int)p.items.size() : batch->n_few;
         if (first == last) continue;
         a.items = batch->items + first;
         a.n_items = last - first;
-        a.max_rows = 0;
-        for (int i = first; i < last; ++i) a.max_rows = std::max(a.max_rows, p.items[(size_t)i].rows);
+        a.max_rows = many ? batch->many_rows : batch->few_rows;
         LUMEN_TRY(!many ? launch_paged_few(ctx, pool->g, v, a, ctx->stream)
                   : pool->g.dtype == LUMEN_F32 ? launch_paged_attn_f32(ctx, pool->g, v, a, ctx->stream)
                                                : launch_paged_attn_tc(ctx, pool->g, v, pool->k_map, pool->v_map, a, ctx->stream));
@@ -265,13 +285,7 @@ int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *ba
     if (p.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: two sequences share a page");
     if (p.tokens == 0 || p.max_kv == 0) return LUMEN_OK;
     OnDevice on(ctx);
-    PagedMassArgs a = {q_dev, scale, lse_dev, 0, INT32_MAX, 0};
-    for (const PagedSeq &q : p.seqs)
-        if (q.q_len && q.kv_len) {
-            a.max_kv = std::max(a.max_kv, q.kv_len);
-            a.min_rows = std::min(a.min_rows, q.q_len * p.group);
-            a.max_rows = std::max(a.max_rows, q.q_len * p.group);
-        }
+    const PagedMassArgs a = {q_dev, scale, lse_dev, batch->seen_kv, batch->min_rows, batch->max_rows};
     return a.max_rows ? launch_paged_mass(ctx, pool->g, view_of(pool, batch), pool->k_map[1], a, ctx->stream) : (int)LUMEN_OK;
 }
 

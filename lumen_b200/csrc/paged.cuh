@@ -24,6 +24,8 @@ struct lumen_page_batch {
     lumen::PagedItem *items = nullptr;
     lumen::PagedJoin *joins = nullptr;
     int n_few = 0;          // items that the kernel for few rows takes; the others follow
+    int few_rows = 0, many_rows = 0, join_rows = 0, join_splits = 0;  // the largest of either, and of the joins
+    int seen_kv = 0, min_rows = 0, max_rows = 0;                      // of the sequences with new tokens and positions: most positions, rows of a key head
     float *part = nullptr;  // partial sums [part_rows, d], then their maxima and sums [part_rows, 2]
 };
 

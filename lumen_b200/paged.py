@@ -69,9 +69,10 @@ class PageBatch:
         if isinstance(tables, np.ndarray) and tables.ndim == 2:
             rows = _int32(tables.reshape(-1), "tables", tables.size).reshape(tables.shape)
         else:  # (shorter lists are filled up with a page number that is refused if it is ever needed)
-            rows = np.full((n, max((len(t) for t in tables), default=0)), -1, np.int32)
-            for row, t in zip(rows, tables):
-                row[: len(t)] = _int32(t, "tables", len(t))
+            lens = np.asarray([len(t) for t in tables], np.int64)
+            flat = [x for t in tables for x in t]
+            rows = np.full((n, int(lens.max(initial=0))), -1, np.int32)
+            rows[np.arange(rows.shape[1]) < lens[:, None]] = _int32(flat, "tables", len(flat))
         self.tokens, self.q_lens, self.kv_lens = int(q.sum()), q, kv
         self.h = C.c_void_p()
         self.ctx.check(self.ctx._lib.lumen_page_batch_new(pool.h, n_head, n, q.ctypes.data, kv.ctypes.data, None if first is None else first.ctypes.data,

@@ -521,6 +521,8 @@ def test_refusals(L, ctx):
     refused("ERR_SHAPE", app, batch, kv_stride=127)
     refused("ERR_INVALID", app, batch, q_out_ptr=p + 8)
     refused("ERR_INVALID", app, batch, q_ptr=0)
+    refused("ERR_INVALID", app, batch, q_out_ptr=p + 1008)  # (rows of 1024 bytes)
+    refused("ERR_INVALID", app, batch, q_ptr=p + 4096, q_out_ptr=p)
     refused("ERR_ROPE_RANGE", app, batch, rope=rope)  # position 16 of 16
     refused("ERR_SHAPE", app, batch, rope=L.RotaryEmbedding(32, 99, 10000.0))
     refused("ERR_SHAPE", app, L.PageBatch(pool, 4, [3], [1], [[0]], causal=False))
@@ -531,6 +533,8 @@ def test_refusals(L, ctx):
     refused("ERR_INVALID", att, out_ptr=0)
     refused("ERR_INVALID", att, out_ptr=p + 8)
     refused("ERR_INVALID", att, out_ptr=p + 16)  # overlaps
+    refused("ERR_INVALID", att, lse_ptr=p + 8192)
+    refused("ERR_INVALID", att, lse_ptr=p + 508)
     refused("ERR_INVALID", att, scale=float("nan"))
     refused("ERR_INVALID", att, scale=float("inf"))
     refused("ERR_DTYPE", att, out_dtype=7)
@@ -569,6 +573,54 @@ def test_nothing_to_do(L):
         L.paged_evict(pool, batch, L.PageBatch(pool, 4, [0] * len(batch.q_lens), [0] * len(batch.q_lens), [[]] * len(batch.q_lens)), 4, kept.data_ptr(), 0)
     pool.ctx.synchronize()
     assert pool.ctx.launch_count == before and (x == 3).all() and (kept == -1).all()
+
+
+def test_a_batch_fits_the_pools_of_all_layers(L):
+    w, other = World(L, "bf16", (8, 2, 64), 16, [1, 40], [100, 90]), World(L, "bf16", (8, 2, 64), 16, [1, 40], [100, 90], seed=0)
+    other.k.copy_(w.k.flip(0))
+    other.v.copy_(w.v.flip(0))
+    other.tables = [[w.pages - 1 - t for t in table] for table in w.tables]
+    q = w.randn(41, 8, 64).to(w.t)
+    a, b = attend(w, q, 0.125), attend(other, q, 0.125)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    L.paged_attention(other.pool, b[2], q.data_ptr(), 0.125, out.data_ptr())
+    L.paged_attention(w.pool, a[2], q.data_ptr(), 0.125, out.data_ptr())
+    L.paged_attention(other.pool, L.PageBatch(w.pool, 8, [1, 40], [100, 90], other.tables), q.data_ptr(), 0.125, out.data_ptr())
+    w.pool.ctx.synchronize()
+    assert torch.equal(out.double().cpu(), a[0]) and torch.equal(a[0], b[0])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_sequences_than_a_grid_has_rows(L, dtype):
+    """33000 short sequences: one token each to 2 positions, observed, then one of them stays."""
+    n, D = 33000, 64
+    w = World(L, dtype, (2, 1, D), 8, [], [], spare=2 * n)
+    w.k.copy_(w.randn(2 * n, 1, 8, D))
+    w.v.copy_(w.randn(2 * n, 1, 8, D))
+    w.mass.zero_()
+    tables = np.random.default_rng(1).permutation(2 * n)
+    batch, goal = w.batch(q_lens=[1] * n, kv_lens=[2] * n, tables=tables[:n, None]), w.batch(q_lens=[0] * n, kv_lens=[1] * n, tables=tables[n:, None])
+    q = w.randn(n, 2, D).to(w.t)
+    out, lse, kept = torch.empty_like(q), torch.empty(n, 2, device=DEV), torch.full((n, 1), -7, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    L.paged_attention(w.pool, batch, q.data_ptr(), 0.3, out.data_ptr(), lse_ptr=lse.data_ptr())
+    L.paged_attention_mass(w.pool, batch, q.data_ptr(), 0.3, lse.data_ptr())
+    L.paged_evict(w.pool, batch, goal, 0, kept.data_ptr(), 1)
+    w.pool.ctx.synchronize()
+    at = torch.as_tensor(tables, device=DEV)
+    k, v = (x[at[:n], 0, :2].double() for x in (w.k, w.v))
+    p = torch.softmax(torch.einsum("nhd,njd->nhj", q.double(), k) * 0.3, -1)
+    big = torch.einsum("nhd,njd->nhj", q.double().abs(), k.abs()).amax(-1, keepdim=True) * 0.3
+    rel = 2 * (D + 4) * 2.0 ** -23 * big + 2.0 ** -19 + (2 ** -8 if dtype == "bf16" else 0)
+    o = torch.einsum("nhj,njd->nhd", p, v)
+    close(out.double().cpu(), o.cpu(), (2 * rel * torch.einsum("nhj,njd->nhd", p, v.abs()) + o.abs() * (2.0 ** -8 if dtype == "bf16" else 0)).cpu())
+    gain = p.sum(1)
+    got = w.mass[at[:n], 0, :2].double()
+    close(got.cpu(), gain.cpu(), (2 * rel.amax(1) * gain + 1e-6).cpu())
+    want = (got[:, 1] > got[:, 0]).int()
+    assert torch.equal(kept[:, 0], want)
+    assert torch.equal(w.v[at[n:], 0, 0], w.v[at[:n]][torch.arange(n, device=DEV), 0, want.long()])
 
 
 # ---- captured, and together ---------------------------------------------------------------------------------------------
