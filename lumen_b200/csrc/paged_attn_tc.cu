@@ -186,9 +186,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             wait_warp(&q_bar, 0, failed, status, 700);
             tc_after();
             const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, saddr(q_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
-            auto scores = [&](int j) {
+            auto keys_in = [&](int j) { return wait_warp(&k_full[j % kStages], (uint32_t)((j / kStages) & 1), failed, status, 710); };
+            auto values_in = [&](int j) { return wait_warp(&v_full[j % kStages], (uint32_t)((j / kStages) & 1), failed, status, 721); };
+            auto scores = [&](int j, bool ok) {
                 const int s = j % kStages;
-                if (wait_warp(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 710)) {
+                if (ok) {
                     const uint64_t qd = smem_desc(q0 + q * G::kQBytes), kd = smem_desc(ring0 + (uint32_t)s * 2 * G::kKBytes);
                     const uint32_t acc = acc0 + (uint32_t)((q * G::kBuffers + (j & (G::kBuffers - 1))) * kKeys);
 #pragma unroll
@@ -199,14 +201,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
                 commit_one(&s_bar[q][j & (G::kBuffers - 1)]);  // (at once if nothing was issued)
             };
-            auto values = [&](int j) {
+            auto values = [&](int j, bool there) {
                 const int s = j % kStages, buffer = j & (G::kBuffers - 1);
 #pragma unroll
                 for (int h = 0; h < G::kHalves; ++h) {
-                    bool ok = wait_warp(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720);
+                    bool ok = wait_warp(&p_bar[q][buffer * G::kHalves + h], (uint32_t)((j / G::kBuffers) & 1), failed, status, 720) && there;
                     // (the values' dead rows are zeroed by the first tile's warps)
                     if (QT == 2 && ok && h == 0 && q == 1 && it.key0 + (j + 1) * kKeys > it.key1) ok = wait_warp(&dead_bar, 0, failed, status, 722);
-                    if (ok && h == 0) ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 721);
                     tc_after();
                     if (ok) {
                         const uint64_t v = desc_mn(ring0 + (uint32_t)s * 2 * G::kKBytes + G::kKBytes, G::kTile);
@@ -219,16 +220,18 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
             };
             // Products run in the order in which they are issued: scores go over weights whose product stands before them.
-            scores(0);
+            scores(0, keys_in(0));
             commit_one(&k_free[0]);
 #pragma unroll 1
             for (int j = 0; j < nt; ++j) {
+                // (what the copies bring is waited for while the weights are computed, not behind them: each wait takes some 200 cycles even then)
+                const bool keys = j + 1 < nt && keys_in(j + 1);
                 if (QT == 1 && j + 1 < nt) {
-                    scores(j + 1);
+                    scores(j + 1, keys);
                     commit_one(&k_free[(j + 1) % kStages]);
                 }
-                values(j);
-                if (QT == 2 && j + 1 < nt) scores(j + 1);
+                values(j, values_in(j));
+                if (QT == 2 && j + 1 < nt) scores(j + 1, keys);
                 else commit_one(&o_bar[q][j & (G::kBuffers - 1)]);
                 if (QT == 2 && j + 1 < nt) commit_one(&k_free[(j + 1) % kStages]);
                 commit_one(&v_free[j % kStages]);

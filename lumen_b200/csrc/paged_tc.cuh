@@ -34,7 +34,7 @@ __device__ __forceinline__ void commit_one(uint64_t *bar) {
 __device__ __forceinline__ bool wait_first(uint64_t *bar, uint32_t parity, volatile int *failed, DeviceStatus *status, int site) {
     return bar_try(bar, parity) || wait_or_failed(bar, parity, failed, status, site);
 }
-// The same by all lanes; the answer is the warp's.
+// wait_first by all lanes; the answer is the warp's.
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *failed, DeviceStatus *status, int site) {
     return __all_sync(0xffffffffu, wait_first(bar, parity, failed, status, site));
 }
