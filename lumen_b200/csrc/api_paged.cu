@@ -219,8 +219,8 @@ int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, con
     if (!q_dev || !k_dev || !v_dev || !q_out_dev) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: null argument");
     if (!aligned16(q_out_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: q_out is not 16-byte aligned");
     const size_t d = (size_t)pool->g.d;
-    if (q_stride < (size_t)p.n_head * d || kv_stride < (size_t)pool->g.h_kv * d)
-        return set_error(ctx, LUMEN_ERR_SHAPE, "paged_append: rows of %zu and %zu floats overlap", q_stride, kv_stride);
+    if (q_stride < (size_t)p.n_head * d || kv_stride < (size_t)pool->g.h_kv * d || q_stride >> 40 || kv_stride >> 40)
+        return set_error(ctx, LUMEN_ERR_SHAPE, "paged_append: rows %zu and %zu floats apart", q_stride, kv_stride);
     if (!p.can_append) return set_error(ctx, LUMEN_ERR_SHAPE, "paged_append: a sequence has more new tokens than positions");
     if (p.write_shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: a page that receives rows belongs to two sequences");
     if (rope) {
@@ -300,7 +300,7 @@ int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const
     for (int s = 0; s < a.n_seq; ++s)
         if (b.seqs[(size_t)s].kv_len > a.seqs[(size_t)s].kv_len)
             return set_error(ctx, LUMEN_ERR_SHAPE, "paged_evict: sequence %d: %d of %d positions", s, b.seqs[(size_t)s].kv_len, a.seqs[(size_t)s].kv_len);
-    if ((size_t)b.max_kv > kept_stride) return set_error(ctx, LUMEN_ERR_SHAPE, "paged_evict: rows of %zu for %d positions", kept_stride, b.max_kv);
+    if ((size_t)b.max_kv > kept_stride || kept_stride >> 40) return set_error(ctx, LUMEN_ERR_SHAPE, "paged_evict: rows of %zu for %d positions", kept_stride, b.max_kv);
     if (b.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: two sequences share a page of the destination");
     try {
         std::vector<char> used((size_t)pool->g.pages, 0);

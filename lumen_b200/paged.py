@@ -80,24 +80,30 @@ class PageBatch:
         self._finalizer = weakref.finalize(self, self.ctx._lib.lumen_page_batch_free, C.c_void_p(self.h.value))
 
 
+def _done(pool: PagePool, status: int) -> None:
+    if status:
+        pool.ctx.check(status)
+
+
 def paged_append(pool: PagePool, batch: PageBatch, q_ptr: int, k_ptr: int, v_ptr: int, q_stride: int, kv_stride: int, q_out_ptr: int,
                  rope: RotaryEmbedding | None = None, q_norm_ptr: int = 0, k_norm_ptr: int = 0, eps: float = 0.0) -> None:
     """The new tokens' f32 projections: norms and rotation of queries and keys, queries to `q_out`, keys and values to their slots."""
-    pool.ctx.check(pool.ctx._lib.lumen_paged_append(pool.h, batch.h, rope.h if rope else None, q_ptr, k_ptr, v_ptr, q_stride, kv_stride,
-                                                    q_norm_ptr or None, k_norm_ptr or None, C.c_float(eps), q_out_ptr))
+    _done(pool, pool.ctx._lib.lumen_paged_append(pool.h, batch.h, rope.h if rope else None, q_ptr, k_ptr, v_ptr, q_stride, kv_stride, q_norm_ptr or None,
+                                                 k_norm_ptr or None, eps, q_out_ptr))
 
 
 def paged_attention(pool: PagePool, batch: PageBatch, q_ptr: int, scale: float, out_ptr: int, out_dtype: int | None = None, lse_ptr: int = 0) -> None:
     """Attention of the new tokens over their pages; `out` is of the pool's type unless `out_dtype` says otherwise."""
-    pool.ctx.check(pool.ctx._lib.lumen_paged_attention(pool.h, batch.h, q_ptr, C.c_float(scale), out_ptr,
-                                                       pool.dtype if out_dtype is None else out_dtype, lse_ptr or None))
+    _done(pool, pool.ctx._lib.lumen_paged_attention(pool.h, batch.h, q_ptr, scale, out_ptr, pool.dtype if out_dtype is None else out_dtype, lse_ptr or None))
 
 
 def paged_attention_mass(pool: PagePool, batch: PageBatch, q_ptr: int, scale: float, lse_ptr: int) -> None:
     """Adds the weights that the cached positions received from the new tokens to the pool's mass."""
-    pool.ctx.check(pool.ctx._lib.lumen_paged_attention_mass(pool.h, batch.h, q_ptr, C.c_float(scale), lse_ptr))
+    _done(pool, pool.ctx._lib.lumen_paged_attention_mass(pool.h, batch.h, q_ptr, scale, lse_ptr))
 
 
 def paged_evict(pool: PagePool, source: PageBatch, goal: PageBatch, recent: int, kept_ptr: int, kept_stride: int) -> None:
     """Moves the positions of `source` that received most weight, and the last `recent`, to the pages of `goal`."""
-    pool.ctx.check(pool.ctx._lib.lumen_paged_evict(pool.h, source.h, goal.h, recent, kept_ptr, kept_stride))
+    if recent < 0:
+        raise _lib.LumenError(_lib.ERR_INVALID, f"paged_evict: the last {recent} positions")
+    _done(pool, pool.ctx._lib.lumen_paged_evict(pool.h, source.h, goal.h, recent, kept_ptr, kept_stride))
