@@ -8,8 +8,7 @@
 // A CTA takes an item: up to 128 rows of one key head (a row is one new token and one of the query heads that read this key head) against a range
 // of positions in tiles of 64.  Warpgroups 0 and 1: weights, two threads a row (32 scores and half of the numbers each); warpgroup 2:
 // keys and values from the pages into registers (a tile ahead), split, into shared memory in the layout of the tensor cores; warpgroup 3: one warp
-// issues S = Q.K^T (the next tile's while this one's weights are computed) and O = P.V, P from tensor memory, V as it lies in the
-// cache.  Bound by the six products.
+// issues S = Q.K^T (the next tile's while this one's weights are computed), another O = P.V, P from tensor memory, V as it lies in the cache.  Bound by the six products.
 //
 // Every wait is bounded; a wait that gives up records LUMEN_ERR_TIMEOUT, the roles run on without acting, products in flight are waited for,
 // tensor memory is freed and the CTA returns.
@@ -63,7 +62,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
     constexpr int kStages = G::kStages, kDH = D / 2;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *ring = q_s + kTerms * G::kQTerm;
-    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[2], p_bar, o_bar, quiet;
+    __shared__ uint64_t q_bar, k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], s_bar[2], s_free[2], p_bar, o_bar, quiet, quiet_values;
     __shared__ float xch[2][kRowsTile];
     __shared__ uint32_t tmem_base_s;
     __shared__ int failed_s;
@@ -82,9 +81,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
         }
         bar_init(&s_bar[0], 1);
         bar_init(&s_bar[1], 1);
+        bar_init(&s_free[0], 256);
+        bar_init(&s_free[1], 256);
         bar_init(&p_bar, 256);
         bar_init(&o_bar, 1);
         bar_init(&quiet, 1);
+        bar_init(&quiet_values, 1);
         failed_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -117,47 +119,50 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-        if (warp == 12 && nt > 0) {
-            wait_warp(&q_bar, 0, failed, status, 800);
-            tc_after();
+        // One warp issues the scores, another the values: each waits on its own, and the tensor cores take what is ready.
+        if ((warp == 12 || warp == 13) && nt > 0) {
             const uint32_t acc0 = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, saddr(q_s), 0), ring0 = __shfl_sync(0xffffffffu, saddr(ring), 0);
-            auto scores = [&](int j) {
-                const int s = j % kStages;
-                if (wait_warp(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 801)) {
-                    tc_after();
-                    const uint64_t qd = smem_desc(q0), kd = smem_desc(ring0 + (uint32_t)s * G::kStage);
-#pragma unroll
-                    for (int x = 0; x < 6; ++x)
-#pragma unroll
-                        for (int kb = 0; kb < G::kBlocks; ++kb)
-#pragma unroll
-                            for (int kk = 0; kk < kBK / 16; ++kk)
-                                mma_ss(acc0 + (uint32_t)((j & 1) * kKeys), qd + ((kFirst[x] * G::kQTerm + kb * G::kQTile) >> 4) + 2 * kk,
-                                       kd + ((kSecond[x] * G::kTerm + kb * G::kTile) >> 4) + 2 * kk, G::kIdescS, x + kb + kk > 0);
-                }
-                commit_one(&s_bar[j & 1]);
-                commit_one(&k_free[s]);
-            };
-            scores(0);
+            if (warp == 12) {
+                wait_warp(&q_bar, 0, failed, status, 800);
 #pragma unroll 1
-            for (int j = 0; j < nt; ++j) {
-                // (its buffer was read for tile j - 1, whose weights were announced before that tile's product)
-                if (j + 1 < nt) scores(j + 1);
-                const int s = j % kStages;
-                bool ok = wait_warp(&p_bar, (uint32_t)(j & 1), failed, status, 802);
-                if (ok) ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 803);
-                tc_after();
-                if (ok) {
-                    const uint64_t vd = desc_mn(ring0 + (uint32_t)s * G::kStage + kTerms * G::kTerm, G::kTile);
+                for (int j = 0; j < nt; ++j) {
+                    const int s = j % kStages;
+                    bool ok = wait_warp(&k_full[s], (uint32_t)((j / kStages) & 1), failed, status, 801);
+                    if (j >= 2) ok = wait_warp(&s_free[j & 1], (uint32_t)((j / 2 - 1) & 1), failed, status, 802) && ok;
+                    tc_after();
+                    if (ok) {
+                        const uint64_t qd = smem_desc(q0), kd = smem_desc(ring0 + (uint32_t)s * G::kStage);
 #pragma unroll
-                    for (int x = 0; x < 6; ++x)
+                        for (int x = 0; x < 6; ++x)
 #pragma unroll
-                        for (int kk = 0; kk < kKeys / 16; ++kk)
-                            mma_ts(acc0 + G::kO + (uint32_t)((j & 1) * D), acc0 + G::kP + (uint32_t)(kFirst[x] * (kKeys / 2) + 8 * kk),
-                                   vd + ((kSecond[x] * G::kTerm + kk * 2048) >> 4), G::kIdescO, x + kk > 0);
+                            for (int kb = 0; kb < G::kBlocks; ++kb)
+#pragma unroll
+                                for (int kk = 0; kk < kBK / 16; ++kk)
+                                    mma_ss(acc0 + (uint32_t)((j & 1) * kKeys), qd + ((kFirst[x] * G::kQTerm + kb * G::kQTile) >> 4) + 2 * kk,
+                                           kd + ((kSecond[x] * G::kTerm + kb * G::kTile) >> 4) + 2 * kk, G::kIdescS, x + kb + kk > 0);
+                    }
+                    commit_one(&s_bar[j & 1]);
+                    commit_one(&k_free[s]);
                 }
-                commit_one(&o_bar);
-                commit_one(&v_free[s]);
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < nt; ++j) {
+                    const int s = j % kStages;
+                    bool ok = wait_warp(&v_full[s], (uint32_t)((j / kStages) & 1), failed, status, 803);
+                    ok = wait_warp(&p_bar, (uint32_t)(j & 1), failed, status, 804) && ok;
+                    tc_after();
+                    if (ok) {
+                        const uint64_t vd = desc_mn(ring0 + (uint32_t)s * G::kStage + kTerms * G::kTerm, G::kTile);
+#pragma unroll
+                        for (int x = 0; x < 6; ++x)
+#pragma unroll
+                            for (int kk = 0; kk < kKeys / 16; ++kk)
+                                mma_ts(acc0 + G::kO + (uint32_t)((j & 1) * D), acc0 + G::kP + (uint32_t)(kFirst[x] * (kKeys / 2) + 8 * kk),
+                                       vd + ((kSecond[x] * G::kTerm + kk * 2048) >> 4), G::kIdescO, x + kk > 0);
+                    }
+                    commit_one(&o_bar);
+                    commit_one(&v_free[s]);
+                }
             }
         }
     } else if (warp >= 8) {
@@ -233,6 +238,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
             tc_after();
             uint32_t s[32];
             tmem_ld32(tmem + lanes + (uint32_t)((j & 1) * kKeys + 32 * half), s);
+            tc_before();
+            bar_arrive(&s_free[j & 1]);
             const int tile0 = it.key0 + j * kKeys, lim = end - tile0 - 32 * half;
             float top = -INFINITY;
 #pragma unroll
@@ -309,7 +316,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_f32_kernel(const Paged
         }
     }
     __syncthreads();
-    if (*failed && tid == 384) drain_mmas(&quiet);  // a wait gave up
+    if (*failed && (tid == 384 || tid == 416)) {  // a wait gave up
+        uint64_t &ended = tid == 384 ? quiet : quiet_values;
+        drain_mmas(&ended);
+    }
     tc_before();
     __syncthreads();
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
