@@ -272,7 +272,7 @@ class PageBatch {
 public:
     // tables: [sequences][table_stride] page numbers; first_pos may be empty
     PageBatch(const PagePool &pool, size_t n_head, const std::vector<int32_t> &q_lens, const std::vector<int32_t> &kv_lens, const std::vector<int32_t> &tables,
-              size_t table_stride, const std::vector<int32_t> &first_pos = {}, bool causal = true) {
+              size_t table_stride, const std::vector<int32_t> &first_pos = {}, bool causal = true) : ctx_(pool.context()) {
         if (kv_lens.size() != q_lens.size() || tables.size() != q_lens.size() * table_stride || (!first_pos.empty() && first_pos.size() != q_lens.size()))
             throw Error(LUMEN_ERR_SHAPE, "PageBatch: lengths and tables of different numbers of sequences");
         lumen_page_batch *b = nullptr;
@@ -283,6 +283,7 @@ public:
     lumen_page_batch *get() const { return h_.get(); }
 
 private:
+    Context ctx_;  // (outlives the batch)
     std::shared_ptr<lumen_page_batch> h_;
 };
 

@@ -79,6 +79,12 @@ int main(int argc, char **argv) {
             refused = e.code == LUMEN_ERR_KV_OVERFLOW;
         }
         if (!refused) throw std::runtime_error("a table too short was not refused");
+        std::shared_ptr<L::PageBatch> left;
+        {  // a batch keeps the context that it was made in
+            L::Context own(0);
+            left = std::make_shared<L::PageBatch>(L::PagePool(own, 1, 8, 1, D, LUMEN_F32), H, std::vector<int32_t>{1}, std::vector<int32_t>{1}, std::vector<int32_t>{0}, 1);
+        }
+        left.reset();
         std::printf("ok\n");
         return 0;
     } catch (const std::exception &e) {
