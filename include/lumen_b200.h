@@ -374,9 +374,10 @@ int lumen_model_free(lumen_model *m);
  * outputs follow one another, sequence by sequence.  first_pos[s] is the position that the rotation gives the first
  * new token (NULL: its place in the cache, kv_lens[s] - q_lens[s]; another number after an eviction).  causal != 0: a
  * new token sees the cached positions up to its own; 0: all kv_lens[s].  The arrays are HOST arrays and are read
- * during the call, which checks every page number and copies the plan to the device; it may not be made while the
- * context's stream is being captured.  Refused: more than 128 query heads to a key head (LUMEN_ERR_UNSUPPORTED), q_lens[s] > kv_lens[s] with causal (LUMEN_ERR_SHAPE), more positions
- * than the table's pages hold (LUMEN_ERR_KV_OVERFLOW), a page outside the pool or twice in a sequence
+ * during the call, which checks every page number and copies the plan to the device; neither a pool nor a batch may be
+ * made or freed while the context's stream is being captured.  Refused: more than 128 query heads to a key head
+ * (LUMEN_ERR_UNSUPPORTED), q_lens[s] > kv_lens[s] with causal (LUMEN_ERR_SHAPE), more positions than the table's pages
+ * hold (LUMEN_ERR_KV_OVERFLOW), a page outside the pool or twice in a sequence, more than 2^30 rows of queries
  * (LUMEN_ERR_INVALID).  Sequences may share pages that they only read.
  * The calls below allocate nothing and may be captured into graphs; a batch owns the workspace of its attention, so
  * calls with ONE batch must not overlap, as those on one context's stream do not.  A batch or pool that a graph uses
@@ -394,16 +395,19 @@ int lumen_page_batch_free(lumen_page_batch *batch);
  * q_norm / k_norm [d] (NULL: none; rms_norm.rs:49-56), then the rotation of rope (NULL: none; encoding.rs:195-203);
  * q goes to q_out[tokens, n_head, d], k and v to their slots, all of the pool's type, each rounded once; the slots'
  * attention weight becomes 0.  Refused: pages that receive new rows and also belong to another sequence, positions
- * beyond the tables (LUMEN_ERR_ROPE_RANGE), rows that overlap one another or q_out.  q_out: 16-byte aligned. */
+ * beyond the tables (LUMEN_ERR_ROPE_RANGE), rows that overlap one another, q_out or the pool.  q_out: 16-byte
+ * aligned. */
 int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, const lumen_rope *rope, const float *q_dev, const float *k_dev,
                        const float *v_dev, size_t q_stride, size_t kv_stride, const float *q_norm_dev, const float *k_norm_dev, float eps,
                        void *q_out_dev);
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the positions that token t sees, query head h reading key head
  * h / (n_head / h_kv).  q: the pool's type; out: f32, or bf16 from a bf16 pool; [tokens, n_head, d], 16-byte aligned; q, out
- * and lse may not overlap.  lse (NULL: not wanted): f32 [tokens, n_head], log of the sum of exp(scale * q . k).  A token that sees nothing
- * gives zeros and -infinity.  Sums and softmax in f32; from a bf16 pool the weights are rounded to bf16 before they
- * meet the values; an f32 pool is computed with all 24 bits.  Slots behind a sequence's end may hold anything. A value that is not
- * finite, in a slot of the sequence, can reach every token whose call reads that slot. */
+ * and lse may not overlap, nor results the pool.  |scale| is below 2^127.  lse (NULL: not wanted): f32
+ * [tokens, n_head], log of the sum of exp(scale * q . k).  A token that sees nothing gives zeros and -infinity.
+ * Sums and softmax in f32; from a bf16 pool the weights are rounded to bf16 before they meet the values; an f32 pool is
+ * computed with all 24 bits.  Slots behind a sequence's end may hold anything.  A value that is not finite (from an f32
+ * pool: not of a magnitude that rounds to a finite bf16 number), in a slot of the sequence, can reach every token whose
+ * call reads that slot. */
 int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *batch, const void *q_dev, float scale, void *out_dev,
                           lumen_dtype out_dtype, float *lse_dev);
 /* What the cached positions were looked at: mass[slot of j] += sum over the new tokens that see j and the query heads of its key

@@ -1,4 +1,6 @@
 // C ABI of the paged key/value cache: pools of pages, batches of sequences, and the calls that fill, read, observe and shrink them.
+#include <cfloat>
+#include <cmath>
 #include <cstdlib>
 #include <new>
 
@@ -41,7 +43,19 @@ bool meet(const void *a, size_t na, const void *b, size_t nb) {
     return na && nb && x < y + nb && y < x + na;
 }
 
+bool in_pool(const lumen_page_pool *pool, const void *p, size_t bytes) { return meet(p, bytes, pool->k, pool->bytes); }
+
+// A scale that the kernels can take: they multiply by scale * log2(e).
+bool scale_ok(float scale) { return fabsf(scale) <= FLT_MAX / 2.f; }
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Memory is neither taken nor given back while the context's stream is captured: the graph would do it, at every replay.
+int not_captured(lumen_ctx *ctx, const char *what) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    LUMEN_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+    return capture == cudaStreamCaptureStatusNone ? (int)LUMEN_OK : set_error(ctx, LUMEN_ERR_INVALID, "%s: the context's stream is being captured", what);
+}
 
 int check_pair(const lumen_page_pool *pool, const lumen_page_batch *b, const char *what) {
     if (!pool) return LUMEN_ERR_INVALID;
@@ -65,6 +79,7 @@ int lumen_page_pool_new(lumen_ctx *ctx, size_t pages, size_t page_size, size_t h
     if (pages == 0 || h_kv == 0 || h_kv > 65535 || pages > INT32_MAX / page_size)
         return set_error(ctx, LUMEN_ERR_INVALID, "page_pool: %zu pages of %zu positions, %zu key heads", pages, page_size, h_kv);
     OnDevice on(ctx);
+    LUMEN_TRY(not_captured(ctx, "page_pool"));
     auto *p = new (std::nothrow) lumen_page_pool();
     if (!p) return set_error(ctx, LUMEN_ERR_INVALID, "page_pool: out of host memory");
     p->ctx = ctx;
@@ -81,6 +96,7 @@ int lumen_page_pool_new(lumen_ctx *ctx, size_t pages, size_t page_size, size_t h
     p->k = mem;
     p->v = mem + bytes;
     p->mass = reinterpret_cast<float *>(mem + 2 * bytes);
+    p->bytes = 2 * bytes + slots * 4;
     if (dtype == LUMEN_BF16) {
         int rc = LUMEN_OK;
         for (int i = 0; i < 2 && rc == LUMEN_OK; ++i) {
@@ -105,6 +121,7 @@ float *lumen_page_pool_mass(const lumen_page_pool *pool) { return pool ? pool->m
 int lumen_page_pool_free(lumen_page_pool *pool) {
     if (!pool) return LUMEN_ERR_INVALID;
     OnDevice on(pool->ctx);
+    LUMEN_TRY(not_captured(pool->ctx, "page_pool_free"));
     cudaStreamSynchronize(pool->ctx->stream);
     cudaFree(pool->k);
     delete pool;
@@ -117,9 +134,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
     *out = nullptr;
     lumen_ctx *ctx = pool->ctx;
     OnDevice on(ctx);
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    LUMEN_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
-    if (capture != cudaStreamCaptureStatusNone) return set_error(ctx, LUMEN_ERR_INVALID, "page_batch: the context's stream is being captured");
+    LUMEN_TRY(not_captured(ctx, "page_batch"));
     lumen_page_batch *b = nullptr;
     try {
         b = new lumen_page_batch();
@@ -205,6 +220,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
 int lumen_page_batch_free(lumen_page_batch *batch) {
     if (!batch) return LUMEN_ERR_INVALID;
     OnDevice on(batch->ctx);
+    LUMEN_TRY(not_captured(batch->ctx, "page_batch_free"));
     const int rc = dev_free(batch->ctx, batch->dev);
     delete batch;
     return rc;
@@ -234,6 +250,8 @@ int lumen_paged_append(lumen_page_pool *pool, const lumen_page_batch *batch, con
     const size_t out_bytes = (size_t)p.tokens * p.n_head * d * (pool->g.dtype == LUMEN_F32 ? 4 : 2);
     if (meet(q_out_dev, out_bytes, q_dev, q_span) || meet(q_out_dev, out_bytes, k_dev, kv_span) || meet(q_out_dev, out_bytes, v_dev, kv_span))
         return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: q_out overlaps the rows that are read");
+    if (in_pool(pool, q_out_dev, out_bytes) || in_pool(pool, q_dev, q_span) || in_pool(pool, k_dev, kv_span) || in_pool(pool, v_dev, kv_span))
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_append: rows in the pool's own memory");
     OnDevice on(ctx);
     PagedAppendArgs a = {};
     a.q = q_dev; a.k = k_dev; a.v = v_dev; a.q_norm = q_norm_dev; a.k_norm = k_norm_dev;
@@ -251,10 +269,12 @@ int lumen_paged_attention(const lumen_page_pool *pool, const lumen_page_batch *b
     if (out_dtype != LUMEN_F32 && !(out_dtype == LUMEN_BF16 && pool->g.dtype == LUMEN_BF16))
         return set_error(ctx, LUMEN_ERR_DTYPE, "paged_attention: output type %d from a pool of type %d", (int)out_dtype, (int)pool->g.dtype);
     if (!aligned16(q_dev) || !aligned16(out_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q or out is not 16-byte aligned");
-    if (!(scale - scale == 0.f)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: scale is not finite");
+    if (!scale_ok(scale)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: scale is not finite");
     const size_t rows = (size_t)p.tokens * p.n_head, q_bytes = rows * pool->g.d * (pool->g.dtype == LUMEN_F32 ? 4 : 2), out_bytes = rows * pool->g.d * (out_dtype == LUMEN_F32 ? 4 : 2);
     if (meet(q_dev, q_bytes, out_dev, out_bytes) || (lse_dev && (meet(q_dev, q_bytes, lse_dev, rows * 4) || meet(out_dev, out_bytes, lse_dev, rows * 4))))
         return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: q, out and lse overlap");
+    if (in_pool(pool, out_dev, out_bytes) || (lse_dev && in_pool(pool, lse_dev, rows * 4)))
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention: results in the pool's own memory");
     if (p.tokens == 0) return LUMEN_OK;
     OnDevice on(ctx);
     PagedAttnArgs a = {};
@@ -281,7 +301,7 @@ int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *ba
     const PagedPlan &p = batch->plan;
     if (!q_dev || !lse_dev) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: null argument");
     if (!aligned16(q_dev)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: q is not 16-byte aligned");
-    if (!(scale - scale == 0.f)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: scale is not finite");
+    if (!scale_ok(scale)) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: scale is not finite");
     if (p.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: two sequences share a page");
     if (p.tokens == 0 || p.max_kv == 0) return LUMEN_OK;
     OnDevice on(ctx);
@@ -311,6 +331,8 @@ int lumen_paged_evict(lumen_page_pool *pool, const lumen_page_batch *from, const
         return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: out of host memory");
     }
     if (b.max_kv == 0) return LUMEN_OK;
+    if (in_pool(pool, kept_dev, (((size_t)b.n_seq * (size_t)pool->g.h_kv - 1) * kept_stride + (size_t)b.max_kv) * 4))
+        return set_error(ctx, LUMEN_ERR_INVALID, "paged_evict: kept in the pool's own memory");
     OnDevice on(ctx);
     return launch_paged_evict(ctx, pool->g, view_of(pool, from), view_of(pool, to), (int)std::min<size_t>(recent, INT32_MAX), a.max_kv, b.max_kv, kept_dev,
                               kept_stride, ctx->stream);

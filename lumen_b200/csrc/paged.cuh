@@ -11,6 +11,7 @@ struct lumen_page_pool {
     lumen::PagedGeom g;
     void *k = nullptr, *v = nullptr;  // [pages, h_kv, page, d]
     float *mass = nullptr;            // [pages, h_kv, page]
+    size_t bytes = 0;                 // of all three, which follow one another
     CUtensorMap k_map[2], v_map[2];   // bf16: boxes of up to 64 and up to 128 positions of a page x 64 numbers
 };
 

@@ -304,7 +304,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const float scale2 = scale * kLog2e;
             const uint64_t scale_2 = two(scale2, scale2);
             uint64_t sum[2] = {0ull, 0ull};
-            const int first = p.causal ? (key - past) * p.group : 0;  // the first row that sees the position
+            const int first = p.causal ? max(0, key - past) * p.group : 0;  // the first row that sees the position
             const int key_max = key0 + 128 * kt + (warp & 3) * 32 + 31;
 #pragma unroll 1
             for (int i = 0; i < steps; ++i) {
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint64_t scale_2 = two(scale * kLog2e, scale * kLog2e);
         uint64_t sum[2] = {0ull, 0ull};
-        const int first = p.causal ? (key - past) * p.group : 0, key_max = key0 + (warp & 3) * 32 + 31;
+        const int first = p.causal ? max(0, key - past) * p.group : 0, key_max = key0 + (warp & 3) * 32 + 31;
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int b = i & 1, r0 = start + i * 128;

@@ -83,7 +83,8 @@ inline int paged_layout(const PagedGeom &g, size_t n_head, size_t n_seq, const i
         p.seqs[s] = {(int)tokens, (int)q, (int)kv, (int)entries};
         tokens += q;
         entries += need;
-        if (tokens * p.group > INT32_MAX || entries > INT32_MAX) return paged_refuse(err, LUMEN_ERR_INVALID, "too many tokens or pages");
+        if (tokens * (long long)n_head > 1LL << 30 || entries > INT32_MAX)  // (2^30 rows of queries and outputs are more than a GPU holds)
+            return paged_refuse(err, LUMEN_ERR_INVALID, "too many tokens or pages");
         p.max_q = std::max(p.max_q, (int)q);
         p.max_kv = std::max(p.max_kv, (int)kv);
         if (q > kv) p.can_append = false;

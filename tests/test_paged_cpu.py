@@ -55,6 +55,11 @@ def test_refused_heads_and_positions(plan):
     assert plan([(1, 1, [0])], first=[-5])[0] == INVALID
 
 
+def test_refused_more_rows_than_a_gpu_holds(plan):
+    assert plan([(2 ** 30 + 1, 1, [0])], h_kv=1, n_head=1, causal=0)[0] == INVALID
+    assert plan([(2 ** 28, 1, [0]), (1, 1, [1])], h_kv=2, n_head=4, causal=0)[0] == INVALID
+
+
 def test_numbers_behind_the_last_page_are_not_looked_at(plan):
     assert plan([(1, 8, [3, 77, -9])])[0] == OK and plan([(0, 0, [99])])[0] == OK and plan([])[0] == OK
 

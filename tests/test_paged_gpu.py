@@ -558,6 +558,40 @@ def test_refusals(L, ctx):
     ctx.synchronize()
 
 
+def test_refusals_of_the_pool_s_own_memory(L, ctx):
+    """Rows and results may not lie in the pool; scales that overflow with log2(e) are refused; nothing is freed into a graph."""
+    def refused(call, *a, **k):
+        with pytest.raises(L.LumenError) as e:
+            call(*a, **k)
+        assert e.value.code == L._lib.ERR_INVALID, e.value
+
+    pool = L.PagePool(8, 16, 2, 64, L.F32)
+    batch, goal = L.PageBatch(pool, 4, [1], [17], [[0, 1]]), L.PageBatch(pool, 4, [0], [10], [[2]])
+    x = torch.zeros(4096, device=DEV)
+    p, last = x.data_ptr(), pool.mass_ptr + 8 * 2 * 16 * 4 - 16  # (the pool's last 16 bytes)
+    row = dict(pool=pool, batch=batch, q_ptr=p, k_ptr=p, v_ptr=p, q_stride=256, kv_stride=128, q_out_ptr=p + 8192)
+    for at in (pool.k_ptr, pool.v_ptr, pool.mass_ptr, last):
+        for name in ("q_ptr", "k_ptr", "v_ptr", "q_out_ptr"):
+            refused(L.paged_append, **{**row, name: at})
+        refused(L.paged_attention, pool, batch, p, 1.0, at)
+        refused(L.paged_attention, pool, batch, p, 1.0, p + 8192, lse_ptr=at)
+        refused(L.paged_evict, pool, batch, goal, 0, at, 16)
+    for scale in (2.0 ** 127, -(2.0 ** 127)):
+        refused(L.paged_attention, pool, batch, p, scale, p + 8192)
+        refused(L.paged_attention_mass, pool, batch, p, scale, p)
+    L.paged_attention(pool, batch, p, 2.0 ** 126, p + 8192)
+    lib, other, spare = L._lib.load(), L.PageBatch(pool, 4, [1], [1], [[0]]), L.PagePool(1, 16, 1, 64)
+    ctx.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(ctx.stream)):
+        L.paged_attention(pool, batch, p, 1.0, p + 8192)
+        refused(L.PagePool, 1, 16, 1, 64)
+        assert lib.lumen_page_batch_free(other.h) == lib.lumen_page_pool_free(spare.h) == L._lib.ERR_INVALID
+    L.paged_attention(pool, other, p, 1.0, p + 8192)  # (still there)
+    L.paged_append(**{**row, "pool": spare, "batch": L.PageBatch(spare, 1, [1], [1], [[0]])})
+    ctx.synchronize()
+
+
 def test_nothing_to_do(L):
     """No sequences, no new tokens, nothing to keep: accepted, and nothing is written."""
     pool = L.PagePool(8, 16, 2, 64)
