@@ -169,13 +169,22 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
             rows = std::max(rows, p.items[i].rows);
         }
         for (const PagedJoin &j : p.joins) b->join_rows = std::max(b->join_rows, j.rows), b->join_splits = std::max(b->join_splits, j.splits);
-        for (const PagedSeq &q : p.seqs)
-            if (q.q_len && q.kv_len) {
-                const int rows = q.q_len * p.group;
-                b->seen_kv = std::max(b->seen_kv, q.kv_len);
-                b->min_rows = b->max_rows ? std::min(b->min_rows, rows) : rows;
-                b->max_rows = std::max(b->max_rows, rows);
-            }
+        PagedPlan mass;  // (its parts are positions of their own: nothing is joined)
+        const PagedShape mass_shape = paged_mass_shape(ctx->num_sms);
+        mass.seqs = p.seqs;
+        mass.group = p.group;
+        mass.causal = p.causal;
+        few.clear();
+        for (int s = 0; s < p.n_seq; ++s) {
+            const PagedSeq &q = p.seqs[(size_t)s];
+            const int rows = q.q_len * p.group;
+            if (!rows || !q.kv_len) continue;
+            b->seen_kv = std::max(b->seen_kv, q.kv_len);
+            b->max_rows = std::max(b->max_rows, rows);
+            if (rows <= mass_shape.rows) few.push_back(s), b->mass_rows = std::max(b->mass_rows, rows);
+        }
+        paged_cut(mass, b->g, mass_shape, few);
+        b->n_mass = (int)mass.items.size();
         // everything the kernels read goes up in one copy, in front of the workspace
         std::vector<char> up;
         auto put = [&](const void *data, size_t bytes) {
@@ -187,6 +196,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         const size_t o_seqs = put(p.seqs.data(), p.seqs.size() * sizeof(PagedSeq)), o_tab = put(p.tables.data(), p.tables.size() * 4);
         const size_t o_slot = put(p.tok_slot.data(), p.tok_slot.size() * 4), o_pos = put(p.tok_pos.data(), p.tok_pos.size() * 4);
         const size_t o_it = put(p.items.data(), p.items.size() * sizeof(PagedItem)), o_jo = put(p.joins.data(), p.joins.size() * sizeof(PagedJoin));
+        const size_t o_mass = put(mass.items.data(), mass.items.size() * sizeof(PagedItem));
         const size_t o_part = (up.size() + 255) & ~(size_t)255;
         rc = dev_alloc(ctx, o_part + (size_t)p.part_rows * (size_t)(b->g.d + 2) * 4, &b->dev);
         if (rc == LUMEN_OK && !up.empty()) {
@@ -208,6 +218,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         b->tok_pos = reinterpret_cast<int *>(at + o_pos);
         b->items = reinterpret_cast<PagedItem *>(at + o_it);
         b->joins = reinterpret_cast<PagedJoin *>(at + o_jo);
+        b->mass = reinterpret_cast<PagedItem *>(at + o_mass);
         b->part = reinterpret_cast<float *>(at + o_part);
     } catch (const std::exception &) {
         delete b;
@@ -305,7 +316,7 @@ int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *ba
     if (p.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: two sequences share a page");
     if (p.tokens == 0 || p.max_kv == 0) return LUMEN_OK;
     OnDevice on(ctx);
-    const PagedMassArgs a = {q_dev, scale, lse_dev, batch->seen_kv, batch->min_rows, batch->max_rows};
+    const PagedMassArgs a = {q_dev, scale, lse_dev, batch->seen_kv, batch->max_rows, batch->mass, batch->n_mass, batch->mass_rows};
     return a.max_rows ? launch_paged_mass(ctx, pool->g, view_of(pool, batch), pool->k_map[1], a, ctx->stream) : (int)LUMEN_OK;
 }
 

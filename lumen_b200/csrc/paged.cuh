@@ -26,7 +26,9 @@ struct lumen_page_batch {
     lumen::PagedJoin *joins = nullptr;
     int n_few = 0;          // items that the kernel for few rows takes; the others follow
     int few_rows = 0, many_rows = 0, join_rows = 0, join_splits = 0;  // the largest of either, and of the joins
-    int seen_kv = 0, min_rows = 0, max_rows = 0;                      // of the sequences with new tokens and positions: most positions, rows of a key head
+    int seen_kv = 0, max_rows = 0;                                    // of the sequences with new tokens and positions: most positions, rows of a key head
+    lumen::PagedItem *mass = nullptr;  // what the kernel that adds up the weights of few rows takes
+    int n_mass = 0, mass_rows = 0;
     float *part = nullptr;  // partial sums [part_rows, d], then their maxima and sums [part_rows, 2]
 };
 
@@ -110,8 +112,11 @@ struct PagedMassArgs {
     const void *q;
     float scale;
     const float *lse;
-    int max_kv, min_rows, max_rows;  // of the sequences with new tokens: positions, rows of a key head
+    int max_kv, max_rows;    // of the sequences with new tokens: positions, rows of a key head
+    const PagedItem *few;    // the work of the sequences with few rows
+    int n_few, few_rows;
 };
+PagedShape paged_mass_shape(int num_sms);  // (its rows: up to which the items are taken)
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s);
 int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_len, int max_keep, int *kept,
                        size_t kept_stride, cudaStream_t s);

@@ -3,7 +3,8 @@
 // y = x / sqrt(mean(x^2) + eps) * w per head, then (a, b) -> (a c - b s, b c + a s) over the pairs (i, i + d/2); values are copied.  A lane
 // holds eight neighbours, d / 8 lanes a head, so the partner of a pair is the lane d / 16 further, and a warp works on 256 / d heads at once
 // (one head a warp took 173 instructions per head, and twice the time).  Every number is read once and written once: bound by HBM, by the launch for a
-// decode step.
+// decode step.  Measured, 48 heads of 128 with norms and rotation to bf16: 6726 tokens 57 us, 251 MB at 4.4 TB/s (a copy moves 6.5); 64 tokens 4.9 us,
+// one behind another.  Registers hold the loads in flight: 62 a thread, 46 % of the warps an SM can have.
 #include "paged.cuh"
 
 namespace lumen {

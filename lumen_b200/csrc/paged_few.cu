@@ -8,6 +8,10 @@
 //   of neighbouring positions make the operand.  The weights, which come out position by row, are transposed by movmatrix.
 // So nothing of the cache goes through shared memory, and no warp waits for another until the end, where their sums are joined.  Long ranges are
 // cut over the CTAs and joined by paged_join_kernel, in the order of the parts.
+// Measured: single tokens of 64 sequences of 1000 to 8000 positions, 8 key heads of 128, bf16, 188 us with the join: 1.25 GB at 6.6 TB/s, what a copy
+// moves.  One sequence of 16001 positions, 4 key heads of 64, f32: 15 us for 33 MB, where starting, the first loads and the join are most of it.
+// (Two CTAs of four warps an SM with up to 255 registers: the loads of a whole step are in flight while the one before is worked on.  Three or four CTAs with fewer
+// registers: 191 to 417 us.)
 //
 // 32 bits: a number is the sum of three bf16 numbers (each the rounded rest of the ones before; what is left is below 2^-24 of it); the six largest
 // of the nine products are computed, the largest apart from the others, and a step's results are added in f32 registers.

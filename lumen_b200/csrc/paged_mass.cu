@@ -2,9 +2,11 @@
 // of the query heads that read the key head.)
 //
 // Every position belongs to one thread or one group of lanes, which walks the rows in their order: no atomics, the same sum every time.
-//   up to 64 rows: paged_mass_few_kernel, bound by reading the keys once
-//   more: scores on the 5th-generation tensor cores: paged_mass_tc_kernel (16 bits), bound by the exponentials (16 a cycle and SM), and
-//   paged_mass_f32_kernel, bound by the six products of three bf16 terms
+//   up to 64 rows: paged_mass_few_kernel, bound by reading the keys once (16 sequences of 2000 to 8000 positions, 8 key heads of 128, one token: 37 us
+//   behind the attention, 165 MB at 4.5 TB/s; half of the time for the first use of an SM by each CTA)
+//   more: scores on the 5th-generation tensor cores: paged_mass_tc_kernel (16 bits; two chunks of 200 to 512 tokens over up to 6500 positions, 32 over 8 heads of
+//   128: 97 us, exponential unit 41 % and tensor pipe 29 % busy), and paged_mass_f32_kernel, bound by the six products of three bf16 terms (390 us there; 1550 as
+//   m16n8k16 products)
 #include <type_traits>
 
 #include "paged.cuh"
@@ -19,7 +21,7 @@ using namespace tc;
 constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-constexpr int kFewThreads = 128;
+constexpr int kFewWarps = 4, kFewPerSm = 2, kFewKeys = 128;  // (kFewKeys: in what steps an item's positions are cut)
 
 template <typename T, int D>
 struct FewMass {
@@ -28,140 +30,151 @@ struct FewMass {
     static constexpr int kTiles = D / 16;                     // of 16 numbers
     static constexpr int kPieces = D * (int)sizeof(T) / 64;   // of 16 bytes, per lane and key
     static constexpr int kGroups = kSplit ? 1 : 2;            // of 16 positions that a warp takes at once
-    static constexpr int kRounds = kSplit ? 1 : 2;
-    static constexpr int kKeys = kFewThreads / 32 * 16 * kGroups * kRounds;  // of a CTA
-    static constexpr int kChunk = kSplit ? 32 : kFewRows;     // rows in shared memory at a time
+    static constexpr int kStep = 16 * kGroups;
 };
 
 // Scores of 16 positions x 8 rows from m16n8k16 products.  The sum over the numbers of a head may run in any order, so lane (g, t) loads pieces of
 // 16 bytes of the keys g and g + 8 straight into the operand's registers - no shared memory on the way - and the queries are put in
-// shared memory in the order that this gives.  32 bits: three bf16 terms a number and the six largest of nine products, as in paged_few.cu.
-// grid (blocks of positions of the longest sequence, key heads, sequences)
+// shared memory in the order that this gives.  A warp walks steps of 16 or 32 positions of its item on its own, the next step's keys on their way.
 template <typename T, int D>
-__global__ void __launch_bounds__(kFewThreads, 4) paged_mass_few_kernel(const PagedView p, const T *__restrict__ q, float scale, const float *__restrict__ lse) {
+__global__ void __launch_bounds__(kFewWarps * 32, kFewPerSm) paged_mass_few_kernel(const PagedView p, const PagedItem *items, const T *__restrict__ q, float scale, const float *__restrict__ lse) {
     using G = FewMass<T, D>;
     constexpr int kTiles = G::kTiles, kTerms = G::kTerms, kGroups = G::kGroups, kPieces = G::kPieces;
     extern __shared__ uint2 q_s[];   // [blocks of 8 rows][tiles][32 lanes][terms]
-    __shared__ float l_s[G::kChunk];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
-    const PagedSeq sq = p.seqs[blockIdx.z];
-    const int rows = sq.q_len * p.group, key0 = blockIdx.x * G::kKeys, past = sq.kv_len - sq.q_len;
-    pdl_launch();
-    pdl_wait();
-    if (key0 >= sq.kv_len || rows == 0 || rows > kFewRows) return;
+    __shared__ float l_s[kFewRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const PagedItem it = items[blockIdx.x];
+    const PagedSeq sq = it.sq;
+    const int rows = it.rows, kvh = it.kvh, past = sq.kv_len - sq.q_len, steps = (it.key1 - it.key0 + G::kStep - 1) / G::kStep;
     const int *table = p.tables + sq.table;
     const float scale2 = scale * kLog2e;
-    const int start = p.causal ? max(0, key0 - past) * p.group : 0;  // the first row that sees any of the CTA's positions
-    auto stage = [&](int r0, int n) {  // rows r0 .. r0 + n - 1
-        for (int i = tid; i < (n + 7) / 8 * kTiles * 32; i += kFewThreads) {
-            const int ln = i & 31, tile = i / 32 % kTiles, row = r0 + i / (32 * kTiles) * 8 + (ln >> 2);
-            // 32 bits: tile c takes piece c, numbers 16 c + 4 t ..; 16 bits: tiles 2 c and 2 c + 1 the halves of piece c, numbers 32 c + 8 t ..
-            const int at = G::kSplit ? 16 * tile + 4 * (ln & 3) : 32 * (tile / 2) + 8 * (ln & 3) + 4 * (tile & 1);
-            const bool live = row < r0 + n;
-            const T *src = q + ((size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group) * D + at;
-            if constexpr (G::kSplit) {
-                const float4 x = live ? *reinterpret_cast<const float4 *>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
-                uint32_t lo[3], hi[3];
-                split3(x.x, x.y, lo);
-                split3(x.z, x.w, hi);
+    int page[2 * kGroups];  // of every 8 positions of a step, looked up a step before their keys are asked for
+    auto pages = [&](int i) {
 #pragma unroll
-                for (int k = 0; k < 3; ++k) q_s[(size_t)i * 3 + k] = make_uint2(lo[k], hi[k]);
-            } else {
-                q_s[i] = live ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
-            }
+        for (int b = 0; b < 2 * kGroups; ++b) {
+            const int pos = it.key0 + i * G::kStep + 8 * b;
+            page[b] = pos < it.key1 ? table[pos >> p.page_shift] : -1;
         }
-        for (int i = tid; i < n; i += kFewThreads) l_s[i] = lse[(size_t)(sq.tok0 + (r0 + i) / p.group) * p.n_head + kvh * p.group + (r0 + i) % p.group] * kLog2e;
     };
-    const bool once = rows - start <= G::kChunk;
-    if (once) stage(start, rows - start);
     const uint4 *keys = static_cast<const uint4 *>(p.k);
+    auto load = [&](int i, uint4 (&k)[kGroups][2][kPieces], size_t (&at)[kGroups][2]) {
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // (keys behind the end, in the same 8 slots, are loaded and not counted)
+                const int pg = page[2 * x + h], pos = it.key0 + i * G::kStep + 16 * x + 8 * h + g;
+                at[x][h] = (((size_t)max(pg, 0) * p.h_kv + kvh) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+#pragma unroll
+                for (int c = 0; c < kPieces; ++c) k[x][h][c] = pg >= 0 ? __ldcs(keys + at[x][h] * (D * sizeof(T) / 16) + 4 * c + t) : make_uint4(0u, 0u, 0u, 0u);
+            }
+    };
+    pages(warp);
+    pdl_launch();
+    pdl_wait();
+    uint4 k[kGroups][2][kPieces], next[kGroups][2][kPieces];
+    size_t at[kGroups][2], at_next[kGroups][2];
+    load(warp, next, at_next);
+    pages(warp + kFewWarps);
+    for (int i = tid; i < (rows + 7) / 8 * kTiles * 32; i += kFewWarps * 32) {
+        const int ln = i & 31, tile = i / 32 % kTiles, row = i / (32 * kTiles) * 8 + (ln >> 2);
+        // 32 bits: tile c takes piece c, numbers 16 c + 4 t ..; 16 bits: tiles 2 c and 2 c + 1 the halves of piece c, numbers 32 c + 8 t ..
+        const int e = G::kSplit ? 16 * tile + 4 * (ln & 3) : 32 * (tile / 2) + 8 * (ln & 3) + 4 * (tile & 1);
+        const T *src = q + ((size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group) * D + e;
+        if constexpr (G::kSplit) {
+            const float4 x = row < rows ? *reinterpret_cast<const float4 *>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+            uint32_t lo[3], hi[3];
+            split3(x.x, x.y, lo);
+            split3(x.z, x.w, hi);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) q_s[(size_t)i * 3 + n] = make_uint2(lo[n], hi[n]);
+        } else {
+            q_s[i] = row < rows ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
+        }
+    }
+    for (int i = tid; i < rows; i += kFewWarps * 32) l_s[i] = lse[(size_t)(sq.tok0 + i / p.group) * p.n_head + kvh * p.group + i % p.group] * kLog2e;
+    __syncthreads();
 #pragma unroll 1
-    for (int round = 0; round < G::kRounds; ++round) {
-        uint4 k[kGroups][2][kPieces];
-        size_t at[kGroups][2];
-        const int base = key0 + (round * (kFewThreads / 32) + warp) * 16 * kGroups;
+    for (int i = warp; i < steps; i += kFewWarps) {
+        const int base = it.key0 + i * G::kStep;
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i)
+        for (int x = 0; x < kGroups; ++x)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) at[i][h] = paged_row(p, table, kvh, min(base + 16 * i + 8 * h + g, sq.kv_len - 1));
+            for (int h = 0; h < 2; ++h) {
+                at[x][h] = at_next[x][h];
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i)
+                for (int c = 0; c < kPieces; ++c) k[x][h][c] = next[x][h][c];
+            }
+        load(i + kFewWarps, next, at_next);
+        pages(i + 2 * kFewWarps);
+        float had[kGroups][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+        for (int x = 0; x < kGroups; ++x)
 #pragma unroll
-                for (int c = 0; c < kPieces; ++c) k[i][h][c] = __ldcs(keys + at[i][h] * (D * sizeof(T) / 16) + 4 * c + t);
+            for (int h = 0; h < 2; ++h) had[x][h] = t == 0 && base + 16 * x + 8 * h + g < it.key1 ? p.mass[at[x][h]] : 0.f;
         uint32_t a[kGroups][kTiles][kTerms][4];  // the keys as the first operand
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i)
+        for (int x = 0; x < kGroups; ++x)
 #pragma unroll
             for (int c = 0; c < kTiles; ++c) {
                 if constexpr (G::kSplit) {
-                    const uint4 x = k[i][0][c], y = k[i][1][c];
+                    const uint4 y = k[x][0][c], z = k[x][1][c];
                     uint32_t t0[3], t1[3], t2[3], t3[3];
-                    split3(__uint_as_float(x.x), __uint_as_float(x.y), t0);
-                    split3(__uint_as_float(y.x), __uint_as_float(y.y), t1);
-                    split3(__uint_as_float(x.z), __uint_as_float(x.w), t2);
-                    split3(__uint_as_float(y.z), __uint_as_float(y.w), t3);
+                    split3(__uint_as_float(y.x), __uint_as_float(y.y), t0);
+                    split3(__uint_as_float(z.x), __uint_as_float(z.y), t1);
+                    split3(__uint_as_float(y.z), __uint_as_float(y.w), t2);
+                    split3(__uint_as_float(z.z), __uint_as_float(z.w), t3);
 #pragma unroll
-                    for (int n = 0; n < 3; ++n) a[i][c][n][0] = t0[n], a[i][c][n][1] = t1[n], a[i][c][n][2] = t2[n], a[i][c][n][3] = t3[n];
+                    for (int n = 0; n < 3; ++n) a[x][c][n][0] = t0[n], a[x][c][n][1] = t1[n], a[x][c][n][2] = t2[n], a[x][c][n][3] = t3[n];
                 } else {
-                    const uint4 x = k[i][0][c / 2], y = k[i][1][c / 2];
-                    a[i][c][0][0] = c & 1 ? x.z : x.x;
-                    a[i][c][0][1] = c & 1 ? y.z : y.x;
-                    a[i][c][0][2] = c & 1 ? x.w : x.y;
-                    a[i][c][0][3] = c & 1 ? y.w : y.y;
+                    const uint4 y = k[x][0][c / 2], z = k[x][1][c / 2];
+                    a[x][c][0][0] = c & 1 ? y.z : y.x;
+                    a[x][c][0][1] = c & 1 ? z.z : z.x;
+                    a[x][c][0][2] = c & 1 ? y.w : y.y;
+                    a[x][c][0][3] = c & 1 ? z.w : z.y;
                 }
             }
         float sum[kGroups][2] = {};
 #pragma unroll 1
-        for (int r0 = start; r0 < rows; r0 += G::kChunk) {
-            const int n = min(G::kChunk, rows - r0);
-            if (!once) {
-                __syncthreads();  // everyone is done with the rows before
-                stage(r0, n);
-            }
-            if (!once || round == 0) __syncthreads();
-            for (int b = 0; 8 * b < n; ++b) {
-                float sums[4][kGroups][4] = {};  // (of their own, so that products do not wait for each other; the last the largest)
+        for (int b = 0; 8 * b < rows; ++b) {
+            float sums[4][kGroups][4] = {};  // (of their own, so that products do not wait for each other; the last the largest)
 #pragma unroll
-                for (int c = 0; c < kTiles; ++c) {
-                    const uint2 *x = q_s + (size_t)((b * kTiles + c) * 32 + lane) * kTerms;
+            for (int c = 0; c < kTiles; ++c) {
+                const uint2 *qf = q_s + (size_t)((b * kTiles + c) * 32 + lane) * kTerms;
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i) {
-                        if constexpr (G::kSplit) {
-                            mma16816(sums[0][i], a[i][c][2], x[0].x, x[0].y);
-                            mma16816(sums[1][i], a[i][c][1], x[1].x, x[1].y);
-                            mma16816(sums[2][i], a[i][c][0], x[1].x, x[1].y);
-                            mma16816(sums[3][i], a[i][c][0], x[0].x, x[0].y);
-                            mma16816(sums[0][i], a[i][c][0], x[2].x, x[2].y);
-                            mma16816(sums[1][i], a[i][c][1], x[0].x, x[0].y);
-                        } else {
-                            mma16816(sums[c & 3][i], a[i][c][0], x[0].x, x[0].y);
-                        }
+                for (int x = 0; x < kGroups; ++x) {
+                    if constexpr (G::kSplit) {
+                        mma16816(sums[0][x], a[x][c][2], qf[0].x, qf[0].y);
+                        mma16816(sums[1][x], a[x][c][1], qf[1].x, qf[1].y);
+                        mma16816(sums[2][x], a[x][c][0], qf[1].x, qf[1].y);
+                        mma16816(sums[3][x], a[x][c][0], qf[0].x, qf[0].y);
+                        mma16816(sums[0][x], a[x][c][0], qf[2].x, qf[2].y);
+                        mma16816(sums[1][x], a[x][c][1], qf[0].x, qf[0].y);
+                    } else {
+                        mma16816(sums[c & 3][x], a[x][c][0], qf->x, qf->y);
                     }
                 }
+            }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = 8 * b + 2 * t + e, r = r0 + row;
-                    const float l = row < n ? l_s[row] : 0.f;
-                    const int last = row >= n ? -1 : p.causal ? past + r / p.group : sq.kv_len - 1;
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * b + 2 * t + e;
+                const float l = row < rows ? l_s[row] : 0.f;
+                const int last = row >= rows ? -1 : p.causal ? past + row / p.group : it.key1 - 1;
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i)
+                for (int x = 0; x < kGroups; ++x)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float s = sums[3][i][2 * h + e] + (sums[2][i][2 * h + e] + (sums[1][i][2 * h + e] + sums[0][i][2 * h + e]));
-                            sum[i][h] += base + 16 * i + 8 * h + g <= last ? ex2(fmaf(s, scale2, -l)) : 0.f;
-                        }
-                }
+                    for (int h = 0; h < 2; ++h) {
+                        const float s = sums[3][x][2 * h + e] + (sums[2][x][2 * h + e] + (sums[1][x][2 * h + e] + sums[0][x][2 * h + e]));
+                        sum[x][h] += base + 16 * x + 8 * h + g <= last ? ex2(fmaf(s, scale2, -l)) : 0.f;
+                    }
             }
         }
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i)
+        for (int x = 0; x < kGroups; ++x)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                sum[i][h] += __shfl_xor_sync(0xffffffffu, sum[i][h], 1);
-                sum[i][h] += __shfl_xor_sync(0xffffffffu, sum[i][h], 2);
-                if (t == 0 && base + 16 * i + 8 * h + g < sq.kv_len) p.mass[at[i][h]] += sum[i][h];
+                sum[x][h] += __shfl_xor_sync(0xffffffffu, sum[x][h], 1);
+                sum[x][h] += __shfl_xor_sync(0xffffffffu, sum[x][h], 2);
+                if (t == 0 && base + 16 * x + 8 * h + g < it.key1) p.mass[at[x][h]] = had[x][h] + sum[x][h];
             }
     }
 }
@@ -569,49 +582,44 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
 }
 
-dim3 grid_of(const PagedMassArgs &a, const PagedView &v, int keys, int n) { return dim3((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)v.h_kv, (unsigned)n); }
+template <typename T, int D>
+int launch_few(lumen_ctx *ctx, const PagedView &v, const PagedMassArgs &a, cudaStream_t s) {
+    const size_t bytes = (size_t)(a.few_rows + 7) / 8 * 8 * D * 2 * FewMass<T, D>::kTerms;
+    LUMEN_TRY(allow_smem(ctx, paged_mass_few_kernel<T, D>, (size_t)kFewRows * D * 2 * FewMass<T, D>::kTerms));
+    return launch_paged(ctx, paged_mass_few_kernel<T, D>, dim3((unsigned)a.n_few), kFewWarps * 32, bytes, s, v, a.few, static_cast<const T *>(a.q), a.scale, a.lse);
+}
 
 template <int D>
 int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
+    if (a.n_few) LUMEN_TRY(g.dtype == LUMEN_F32 ? (launch_few<float, D>(ctx, all, a, s)) : (launch_few<__nv_bfloat16, D>(ctx, all, a, s)));
+    if (a.max_rows <= kFewRows) return LUMEN_OK;
     for (int s0 = 0; s0 < all.n_seq; s0 += 32768) {  // (the grid's third extent)
-        const int n = std::min(all.n_seq - s0, 32768);
+        const int keys = g.dtype == LUMEN_F32 ? kSplitKeys : kTcKeys;
+        const dim3 grid((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)all.h_kv, (unsigned)std::min(all.n_seq - s0, 32768));
         PagedView v = all;
         v.seqs += s0;
-        const bool few = a.min_rows <= kFewRows, many = a.max_rows > kFewRows;
         if (g.dtype == LUMEN_F32) {
-            const auto *q = static_cast<const float *>(a.q);
-            if (few) {
-                const size_t bytes = (size_t)(std::min(FewMass<float, D>::kChunk, a.max_rows) + 7) / 8 * 8 * D * 6;
-                LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<float, D>, grid_of(a, v, FewMass<float, D>::kKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
-            }
-            if (many) {
-                static const int regs = [] {  // (what the warpgroups trade has to be there)
-                    cudaFuncAttributes attr;
-                    return cudaFuncGetAttributes(&attr, paged_mass_f32_kernel<D>) == cudaSuccess ? attr.numRegs : 0;
-                }();
-                if (regs * kSplitThreads < (2 * 128 + kRegsLoad + kRegsIssue) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention_mass: kernel built with %d registers", regs);
-                LUMEN_TRY(allow_smem(ctx, paged_mass_f32_kernel<D>, SplitMass<D>::kSmem));
-                LUMEN_TRY(launch_paged(ctx, paged_mass_f32_kernel<D>, grid_of(a, v, kSplitKeys, n), kSplitThreads, SplitMass<D>::kSmem, s, v, q, a.scale, a.lse, ctx->d_status));
-            }
-            continue;
-        }
-        const auto *q = static_cast<const __nv_bfloat16 *>(a.q);
-        if (few) {
-            const size_t bytes = (size_t)(std::min(kFewRows, a.max_rows) + 7) / 8 * 8 * D * 2;
-            LUMEN_TRY(launch_paged(ctx, paged_mass_few_kernel<__nv_bfloat16, D>, grid_of(a, v, FewMass<__nv_bfloat16, D>::kKeys, n), kFewThreads, bytes, s, v, q, a.scale, a.lse));
-        }
-        if (many) {
+            static const int regs = [] {  // (what the warpgroups trade has to be there)
+                cudaFuncAttributes attr;
+                return cudaFuncGetAttributes(&attr, paged_mass_f32_kernel<D>) == cudaSuccess ? attr.numRegs : 0;
+            }();
+            if (regs * kSplitThreads < (2 * 128 + kRegsLoad + kRegsIssue) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention_mass: kernel built with %d registers", regs);
+            LUMEN_TRY(allow_smem(ctx, paged_mass_f32_kernel<D>, SplitMass<D>::kSmem));
+            LUMEN_TRY(launch_paged(ctx, paged_mass_f32_kernel<D>, grid, kSplitThreads, SplitMass<D>::kSmem, s, v, static_cast<const float *>(a.q), a.scale, a.lse, ctx->d_status));
+        } else {
             CUtensorMap q_map;
             const size_t row = (size_t)all.n_head * D;
-            LUMEN_TRY(make_map_3d(ctx, &q_map, q, D, (size_t)all.n_head, D, (size_t)all.tokens, row, all.group, kTcRows / all.group));
+            LUMEN_TRY(make_map_3d(ctx, &q_map, a.q, D, (size_t)all.n_head, D, (size_t)all.tokens, row, all.group, kTcRows / all.group));
             LUMEN_TRY(allow_smem(ctx, paged_mass_tc_kernel<D>, MassGeom<D>::kSmem));
-            LUMEN_TRY(launch_paged(ctx, paged_mass_tc_kernel<D>, grid_of(a, v, kTcKeys, n), kTcThreads, MassGeom<D>::kSmem, s, k_map, q_map, v, a.scale, a.lse, ctx->d_status));
+            LUMEN_TRY(launch_paged(ctx, paged_mass_tc_kernel<D>, grid, kTcThreads, MassGeom<D>::kSmem, s, k_map, q_map, v, a.scale, a.lse, ctx->d_status));
         }
     }
     return LUMEN_OK;
 }
 
 }  // namespace
+
+PagedShape paged_mass_shape(int num_sms) { return {kFewRows, kFewKeys, num_sms * kFewPerSm}; }
 
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
     return g.d == 64 ? launch<64>(ctx, g, v, k_map, a, s) : launch<128>(ctx, g, v, k_map, a, s);
