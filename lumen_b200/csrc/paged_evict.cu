@@ -1,9 +1,10 @@
 // Eviction: the positions of a sequence that received most attention, and its last ones, go to new pages.
 //
 // paged_select_kernel, a CTA or a cluster of CTAs per sequence and key head: the weights as ordered 32-bit integers, in shared memory where they fit;
-// four passes over 8 bits each narrow the value of the last one that stays, and a last one writes the positions in order, of the equal ones the
-// lowest.  The histograms have a column per lane, so that the many equal weights (nothing at all, say) do not queue for one counter: whole
-// numbers, so the order of the atomics changes nothing.  paged_move_kernel copies the rows: bound by HBM.
+// up to four passes over 8 bits each narrow the value of the last one that stays (fewer, once all that share the bits found so far stay: three
+// for most long caches), and a last one writes the positions in order, of the equal ones the lowest.  The histograms have a column per lane, so that the
+// many equal weights (nothing at all, say) do not queue for one counter: whole numbers, so the order of the atomics changes nothing.  Bound by the
+// chain of its passes.  paged_move_kernel copies the rows: bound by HBM.
 #include "paged.cuh"
 
 namespace lumen {
@@ -37,7 +38,7 @@ template <bool HELD>
 __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView from, const PagedSeq *to_seqs, int recent, int *kept, size_t kept_stride, int ctas) {
     extern __shared__ uint4 held[];
     __shared__ __align__(16) unsigned hist[256][32];
-    __shared__ unsigned own[2][256], sums[256], prefix_s, want_s, above_s[kWarps], equal_s[kWarps], counts_s[2];
+    __shared__ unsigned own[2][256], sums[256], prefix_s, want_s, whole_s, above_s[kWarps], equal_s[kWarps], counts_s[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)blockIdx.x % ctas, kvh = (int)blockIdx.x / ctas, s = blockIdx.y;
     const PagedSeq sq = from.seqs[s];
     const int len = sq.kv_len, keep = to_seqs[s].kv_len, last = min(recent, keep), old = len - last, pick = keep - last;
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView 
                     if (before < want && want <= before + c[i]) {
                         prefix_s = prefix | (unsigned)(255 - 8 * lane - i) << shift;
                         want_s = want - before;
+                        whole_s = want - before == c[i];
                     }
                     before += c[i];
                 }
@@ -122,6 +124,11 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedView 
         __syncthreads();
         prefix = prefix_s;
         want = want_s;
+        if (whole_s && prefix) {  // all that share these bits stay: the last of them need not be found
+            --prefix;
+            want = 0u;
+            break;
+        }
     }
     const uint32_t edge = prefix;  // all above it stay, and the first `want` equal to it
     // every warp has a run of groups: it counts them, learns what the warps and CTAs before it have, and writes its own
