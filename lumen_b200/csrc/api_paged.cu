@@ -170,7 +170,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         }
         for (const PagedJoin &j : p.joins) b->join_rows = std::max(b->join_rows, j.rows), b->join_splits = std::max(b->join_splits, j.splits);
         PagedPlan mass;  // (its parts are positions of their own: nothing is joined)
-        const PagedShape mass_shape = paged_mass_shape(ctx->num_sms);
+        const PagedShape mass_shape = paged_mass_shape(b->g, ctx->num_sms);
         mass.seqs = p.seqs;
         mass.group = p.group;
         mass.causal = p.causal;

@@ -116,7 +116,7 @@ struct PagedMassArgs {
     const PagedItem *few;    // the work of the sequences with few rows
     int n_few, few_rows;
 };
-PagedShape paged_mass_shape(int num_sms);  // (its rows: up to which the items are taken)
+PagedShape paged_mass_shape(const PagedGeom &g, int num_sms);  // (its rows: up to which the items are taken)
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s);
 int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_len, int max_keep, int *kept,
                        size_t kept_stride, cudaStream_t s);

@@ -2,8 +2,8 @@
 // of the query heads that read the key head.)
 //
 // Every position belongs to one thread or one group of lanes, which walks the rows in their order: no atomics, the same sum every time.
-//   up to 64 rows: paged_mass_few_kernel, bound by reading the keys once (16 sequences of 2000 to 8000 positions, 8 key heads of 128, one token: 37 us
-//   behind the attention, 165 MB at 4.5 TB/s; half of the time for the first use of an SM by each CTA)
+//   few rows: paged_mass_few_kernel, bound by reading the keys once (16 sequences of 2000 to 8000 positions, 8 key heads of 128, a token each:
+//   37 us by events, 165 MB at 4.5 TB/s)
 //   more: scores on the 5th-generation tensor cores: paged_mass_tc_kernel (16 bits; two chunks of 200 to 512 tokens over up to 6500 positions, 32 over 8 heads of
 //   128: 97 us, exponential unit 41 % and tensor pipe 29 % busy), and paged_mass_f32_kernel, bound by the six products of three bf16 terms (390 us there; 1550 as
 //   m16n8k16 products)
@@ -18,7 +18,10 @@ namespace {
 
 using namespace tc;
 
-constexpr int kFewRows = 64;  // rows of a sequence and key head up to which the first kernel is taken
+// Rows of a sequence and key head up to which the first kernel is taken.  8 sequences of 2000 to 8000 positions, 8 key heads of 128: 16 bits, 64 rows 57 us
+// there and 73 in the second, 96 rows 77 and 76, 128 rows 98 and 72; 32 bits, 64 rows 121 and 219, 96 rows 169 and 224, 128 rows 216 and 235 (one short
+// sequence, 96 rows: 21 and 14).
+constexpr int kFewRows = 64, kFewRowsSplit = 96;
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
 constexpr int kFewWarps = 4, kFewPerSm = 2, kFewKeys = 128;  // (kFewKeys: in what steps an item's positions are cut)
@@ -27,6 +30,7 @@ template <typename T, int D>
 struct FewMass {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kTerms = kSplit ? 3 : 1;
+    static constexpr int kRows = kSplit ? kFewRowsSplit : kFewRows;
     static constexpr int kTiles = D / 16;                     // of 16 numbers
     static constexpr int kPieces = D * (int)sizeof(T) / 64;   // of 16 bytes, per lane and key
     static constexpr int kGroups = kSplit ? 1 : 2;            // of 16 positions that a warp takes at once
@@ -41,7 +45,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewPerSm) paged_mass_few_kern
     using G = FewMass<T, D>;
     constexpr int kTiles = G::kTiles, kTerms = G::kTerms, kGroups = G::kGroups, kPieces = G::kPieces;
     extern __shared__ uint2 q_s[];   // [blocks of 8 rows][tiles][32 lanes][terms]
-    __shared__ float l_s[kFewRows];
+    __shared__ float l_s[G::kRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const PagedItem it = items[blockIdx.x];
     const PagedSeq sq = it.sq;
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
     const int tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
     const int rows = sq.q_len * p.group, key0 = blockIdx.x * kSplitKeys, past = sq.kv_len - sq.q_len;
-    if (key0 >= sq.kv_len || rows <= kFewRows) return pdl_wait();
+    if (key0 >= sq.kv_len || rows <= kFewRowsSplit) return pdl_wait();
     const int start = p.causal ? max(0, key0 - past) * p.group : 0, steps = (rows - start + 127) / 128;  // (start < rows: key0 < kv_len)
     const int *table = p.tables + sq.table;
     if (tid == 0) {
@@ -585,14 +589,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
 template <typename T, int D>
 int launch_few(lumen_ctx *ctx, const PagedView &v, const PagedMassArgs &a, cudaStream_t s) {
     const size_t bytes = (size_t)(a.few_rows + 7) / 8 * 8 * D * 2 * FewMass<T, D>::kTerms;
-    LUMEN_TRY(allow_smem(ctx, paged_mass_few_kernel<T, D>, (size_t)kFewRows * D * 2 * FewMass<T, D>::kTerms));
+    LUMEN_TRY(allow_smem(ctx, paged_mass_few_kernel<T, D>, (size_t)FewMass<T, D>::kRows * D * 2 * FewMass<T, D>::kTerms));
     return launch_paged(ctx, paged_mass_few_kernel<T, D>, dim3((unsigned)a.n_few), kFewWarps * 32, bytes, s, v, a.few, static_cast<const T *>(a.q), a.scale, a.lse);
 }
 
 template <int D>
 int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
     if (a.n_few) LUMEN_TRY(g.dtype == LUMEN_F32 ? (launch_few<float, D>(ctx, all, a, s)) : (launch_few<__nv_bfloat16, D>(ctx, all, a, s)));
-    if (a.max_rows <= kFewRows) return LUMEN_OK;
+    if (a.max_rows <= (g.dtype == LUMEN_F32 ? kFewRowsSplit : kFewRows)) return LUMEN_OK;
     for (int s0 = 0; s0 < all.n_seq; s0 += 32768) {  // (the grid's third extent)
         const int keys = g.dtype == LUMEN_F32 ? kSplitKeys : kTcKeys;
         const dim3 grid((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)all.h_kv, (unsigned)std::min(all.n_seq - s0, 32768));
@@ -619,7 +623,7 @@ int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUten
 
 }  // namespace
 
-PagedShape paged_mass_shape(int num_sms) { return {kFewRows, kFewKeys, num_sms * kFewPerSm}; }
+PagedShape paged_mass_shape(const PagedGeom &g, int num_sms) { return {g.dtype == LUMEN_F32 ? kFewRowsSplit : kFewRows, kFewKeys, num_sms * kFewPerSm}; }
 
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
     return g.d == 64 ? launch<64>(ctx, g, v, k_map, a, s) : launch<128>(ctx, g, v, k_map, a, s);

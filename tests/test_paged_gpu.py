@@ -413,6 +413,30 @@ def test_observed_weights(L, dtype, heads, lens, causal):
     assert torch.equal(w.mass.nan_to_num(5.0), before.nan_to_num(5.0))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [8, 16, 17, 24, 25])
+def test_observed_weights_by_every_kernel(L, dtype, d, n):
+    """Four heads to a key head: 64 and 96 rows are the most that the kernel for few rows takes; long sequences are cut, the new tokens lie on a cut."""
+    w = World(L, dtype, (8, 2, d), 16, [n, 1, n, 2], [3001, 40, n, 1024], seed=n)
+    q = w.randn(2 * n + 3, w.Hq, w.D).mul_(2).to(w.t)
+    scale = w.D ** -0.5
+    _, lse, batch = attend(w, q, scale)
+    lse = lse.float().to(DEV)
+    before = w.mass.clone()
+    torch.cuda.synchronize()
+    L.paged_attention_mass(w.pool, batch, q.data_ptr(), scale, lse.data_ptr())
+    w.pool.ctx.synchronize()
+    mass = reference(w, q, scale)[4]
+    for b, kv in enumerate(w.kv_lens):
+        page, slot = w.at(w.tables[b], kv)
+        had = before[page, :, slot].double().cpu()
+        gain, tol = mass[b]
+        close(w.mass[page, :, slot].double().cpu(), had + gain, tol + (had + gain) * 2.0 ** -22)
+        before[page, :, slot] = w.mass[page, :, slot]
+    assert torch.equal(w.mass.nan_to_num(5.0), before.nan_to_num(5.0))
+
+
 def test_observed_weights_have_the_same_bits_every_time(L):
     for dtype in ("bf16", "f32"):
         got = []
