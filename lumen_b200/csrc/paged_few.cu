@@ -401,9 +401,9 @@ int pick(lumen_ctx *ctx, const PagedView &v, const PagedAttnArgs &a, cudaStream_
 
 }  // namespace
 
-// Rows of a sequence and key head up to which this kernel is taken.  8 sequences of 2000 positions: 16 bits, 32 heads of 128 by themselves, 16 rows 62 us
-// here and 67 with the tensor-core tiles of 128 rows, 20 rows (in blocks of 32) 101 and 61; 32 bits, 32 rows (16 at a time) 259 and 363 us,
-// 48 rows about 390 and 369.
+// Rows of a sequence and key head up to which this kernel is taken; by events, here and with tensor-core tiles.  8 sequences of 2000 to 8000 positions, 8 key
+// heads of 128: 16 bits, 12 rows 47 and 46 us, 16 rows 48 and 48 (32 key heads, 2000 positions: 62 and 67; 20 rows, in blocks of 32: 101 and 61); 32 bits, 32 rows
+// (16 at a time) 182 and 188 us.
 int paged_few_rows(const PagedGeom &g) { return g.dtype == LUMEN_F32 ? 32 : 16; }
 
 PagedShape paged_few_shape(int num_sms) { return {16, 64, num_sms * kBlocksPerSm}; }
