@@ -33,8 +33,10 @@ namespace {
 using namespace tc;
 
 constexpr int kMma = 128;       // rows per tile
-constexpr float kLazy = 8.f;    // how far a maximum may grow before O is rescaled
-constexpr int kPolyOf8 = 2;      // pairs of eight whose exponentials go to the FMA pipe (one to five: within 1 % of this, none 3 % slower)
+constexpr float kLazy = 8.f;    // how far a maximum may grow before O is rescaled (0: the same call 571 us for 525)
+// Pairs of eight whose exponentials go to the FMA pipe.  2048 tokens over 16384 positions, one call behind another: none 530 us, one 530, two 525, three 544,
+// four 593.
+constexpr int kPolyOf8 = 2;
 
 template <int D, int QT>
 struct TcGeom {
