@@ -1,10 +1,9 @@
 // New tokens into a paged cache: norm, rotation, rounding and the write to the slots in one pass over the projections.
 //
 // y = x / sqrt(mean(x^2) + eps) * w per head, then (a, b) -> (a c - b s, b c + a s) over the pairs (i, i + d/2); values are copied.  A lane
-// holds eight neighbours, d / 8 lanes a head, so the partner of a pair is the lane d / 16 further, and a warp works on 256 / d heads at once
-// (one head a warp took 173 instructions per head, and twice the time).  Every number is read once and written once: bound by HBM, by the launch for a
-// decode step.  Measured, 48 heads of 128 with norms and rotation to bf16: 6726 tokens 57 us, 251 MB at 4.4 TB/s (a copy moves 6.5); 64 tokens 4.9 us,
-// one behind another.  Registers hold the loads in flight: 62 a thread, 46 % of the warps an SM can have.
+// holds four neighbours of a head's first half and their partners in the second, d / 8 lanes a head, so the rotation stays in the lane and a warp works on 256 / d
+// heads at once (one head a warp took 173 instructions per head, and twice the time).  Every number is read once and written once: bound by HBM, by
+// the launch for a decode step.
 #include "paged.cuh"
 
 namespace lumen {
@@ -12,32 +11,35 @@ namespace {
 
 constexpr int kWarps = 4;
 
-__device__ __forceinline__ void load8(float (&v)[8], const float *src, bool vec) {
+__device__ __forceinline__ void load4(float *v, const float *src, bool vec) {
     if (vec) {
-        const float4 x = __ldcs(reinterpret_cast<const float4 *>(src)), y = __ldcs(reinterpret_cast<const float4 *>(src) + 1);
+        const float4 x = *reinterpret_cast<const float4 *>(src);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = src[i];
+        for (int i = 0; i < 4; ++i) v[i] = src[i];
     }
 }
-__device__ __forceinline__ void store8(float *dst, const float (&v)[8]) {
-    reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16 *dst, const float (&v)[8]) {
-    __nv_bfloat162 b[4];
+__device__ __forceinline__ void load4_once(float *v, const float *src, bool vec) {  // (numbers that nobody reads again)
+    if (vec) {
+        const float4 x = __ldcs(reinterpret_cast<const float4 *>(src));
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<uint4 *>(b);
+        for (int i = 0; i < 4; ++i) v[i] = src[i];
+    }
+}
+__device__ __forceinline__ void store4(float *dst, const float *v) { *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *dst, const float *v) {
+    __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+    *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<uint2 *>(b);
 }
 
 // grid (tokens, parts of a token's heads); a warp takes N groups of 256 / D heads (of q, then k, then v) whose loads go out together
 template <typename T, int D, int N>
-__global__ void __launch_bounds__(kWarps * 32) paged_append_kernel(const PagedView p, const PagedAppendArgs a, bool vec) {
+__global__ void __launch_bounds__(kWarps * 32) paged_append_kernel(const PagedView p, const PagedAppendArgs a, bool vec, bool vec_gain) {
     constexpr int kLanes = D / 8, kHeads = 32 / kLanes;
-    const int lane = threadIdx.x & 31, first = (int)(blockIdx.y * kWarps + (threadIdx.x >> 5)) * kHeads * N, e0 = lane % kLanes * 8, mine = lane / kLanes;
+    const int lane = threadIdx.x & 31, first = (int)(blockIdx.y * kWarps + (threadIdx.x >> 5)) * kHeads * N, e0 = lane % kLanes * 4, mine = lane / kLanes;
     const int heads_k = p.n_head + p.h_kv, all = heads_k + p.h_kv;
     const size_t t = blockIdx.x;
     const int slot = p.tok_slot[t], pos = p.tok_pos[t];
@@ -45,26 +47,23 @@ __global__ void __launch_bounds__(kWarps * 32) paged_append_kernel(const PagedVi
     pdl_launch();
     pdl_wait();
     const float *q = a.q + t * a.q_stride, *k = a.k + t * a.kv_stride, *v = a.v + t * a.kv_stride;
-    float co[8], sn[8], x[N][8];
+    float co[4], sn[4], x[N][8];  // (of a head: numbers e0 .., then D / 2 + e0 ..)
     const bool rot = a.cos_t != nullptr;
 #pragma unroll
     for (int i = 0; i < N; ++i) {  // (these do not wait for the position, as the tables do)
         const int h = first + i * kHeads + mine;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-        if (h < all) load8(x[i], (h < p.n_head ? q + (size_t)h * D : h < heads_k ? k + (size_t)(h - p.n_head) * D : v + (size_t)(h - heads_k) * D) + e0, vec);
+        if (h < all) {
+            const float *src = (h < p.n_head ? q + (size_t)h * D : h < heads_k ? k + (size_t)(h - p.n_head) * D : v + (size_t)(h - heads_k) * D) + e0;
+            load4_once(x[i], src, vec);
+            load4_once(x[i] + 4, src + D / 2, vec);
+        }
     }
     if (rot) {
-        const size_t at = (size_t)pos * (D / 2) + (size_t)(e0 & (D / 2 - 1));
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-            const float4 c = *reinterpret_cast<const float4 *>(a.cos_t + at + i), s = *reinterpret_cast<const float4 *>(a.sin_t + at + i);
-            co[i] = c.x; co[i + 1] = c.y; co[i + 2] = c.z; co[i + 3] = c.w;
-            sn[i] = s.x; sn[i + 1] = s.y; sn[i + 2] = s.z; sn[i + 3] = s.w;
-        }
-        if (e0 < D / 2)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
+        const size_t at = (size_t)pos * (D / 2) + (size_t)e0;
+        load4(co, a.cos_t + at, true);
+        load4(sn, a.sin_t + at, true);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -80,23 +79,30 @@ __global__ void __launch_bounds__(kWarps * 32) paged_append_kernel(const PagedVi
             for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (gain) {
                 const float inv = __fdiv_rn(1.0f, sqrtf(ss / (float)D + a.eps));
+                float w[8];
+                load4(w, gain + e0, vec_gain);
+                load4(w + 4, gain + D / 2 + e0, vec_gain);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * inv * gain[e0 + e];
+                for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * inv * w[e];
             }
         }
-        if (rot) {
-            float other[8];
+        if (rot && (is_q || is_k)) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) other[e] = __shfl_xor_sync(0xffffffffu, x[i][e], kLanes / 2);
-            if (is_q || is_k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * co[e] + other[e] * sn[e];
+            for (int e = 0; e < 4; ++e) {
+                const float u = x[i][e], w = x[i][4 + e];
+                x[i][e] = u * co[e] - w * sn[e];
+                x[i][4 + e] = w * co[e] + u * sn[e];
+            }
         }
         if (is_q) {
-            store8(static_cast<T *>(a.q_out) + (t * p.n_head + h) * D + e0, x[i]);
+            T *dst = static_cast<T *>(a.q_out) + (t * p.n_head + h) * D + e0;
+            store4(dst, x[i]);
+            store4(dst + D / 2, x[i] + 4);
         } else if (h < all) {
             const size_t row = slot_row + ((size_t)(is_k ? h - p.n_head : h - heads_k) << p.page_shift);
-            store8(static_cast<T *>(is_k ? p.k : p.v) + row * D + e0, x[i]);
+            T *dst = static_cast<T *>(is_k ? p.k : p.v) + row * D + e0;
+            store4(dst, x[i]);
+            store4(dst + D / 2, x[i] + 4);
             if (is_k && e0 == 0) p.mass[row] = 0.f;
         }
     }
@@ -106,8 +112,9 @@ template <typename T, int D, int N>
 int launch(lumen_ctx *ctx, const PagedView &v, const PagedAppendArgs &a, cudaStream_t s) {
     auto whole = [&](const float *p, size_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 4 == 0; };
     const bool vec = whole(a.q, a.q_stride) && whole(a.k, a.kv_stride) && whole(a.v, a.kv_stride);
+    auto at16 = [](const float *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };  // (no gains: not read)
     const unsigned per = 256 / D * N * kWarps, parts = ((unsigned)v.n_head + 2u * (unsigned)v.h_kv + per - 1) / per;
-    return launch_paged(ctx, paged_append_kernel<T, D, N>, dim3((unsigned)v.tokens, parts), kWarps * 32, 0, s, v, a, vec);
+    return launch_paged(ctx, paged_append_kernel<T, D, N>, dim3((unsigned)v.tokens, parts), kWarps * 32, 0, s, v, a, vec, at16(a.q_norm) && at16(a.k_norm));
 }
 template <typename T, int D>
 int pick(lumen_ctx *ctx, const PagedView &v, const PagedAppendArgs &a, cudaStream_t s) {

@@ -332,12 +332,23 @@ def test_the_same_bits_every_time(L):
 @pytest.mark.parametrize("norm,rope,odd", [(True, True, 0), (False, True, 1), (True, False, 3), (False, False, 0), (True, True, 2)])
 def test_append(L, dtype, heads, norm, rope, odd):
     """`odd` floats between rows and in front of them: parts of a wider product at any alignment."""
-    q_lens, kv_lens, first = [1, 0, 37, 2], [1, 30, 100, 33], [900, 0, 5, 63]
+    append_of(L, dtype, heads, norm, rope, odd, [1, 0, 37, 2], [1, 30, 100, 33], [900, 0, 5, 63])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,odd", [((8, 2, 64), 0), ((8, 2, 64), 4), ((7, 1, 128), 0), ((32, 8, 128), 0), ((48, 16, 128), 0), ((7, 1, 128), 2)], ids=str)
+@pytest.mark.parametrize("norm,rope", [(True, True), (False, False)])
+def test_append_of_many_tokens(L, dtype, heads, odd, norm, rope):
+    """Enough for CTAs that stay and bring several tokens through each stage of their ring; rows too long for it, and rows at odd places."""
+    append_of(L, dtype, heads, norm, rope, odd, [700, 1, 1300], [900, 33, 1300], [7, 1999, 0])
+
+
+def append_of(L, dtype, heads, norm, rope, odd, q_lens, kv_lens, first):
     w = World(L, dtype, heads, 16, q_lens, kv_lens)
     T, D, n = sum(q_lens), w.D, w.Hq + 2 * w.Hkv
     flat = w.randn(T * (n * D + odd) + odd)
     x = flat[odd:].view(T, n * D + odd)[:, : n * D].reshape(T, n, D).double().cpu()
-    angle = np.arange(1000)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
+    angle = np.arange(2000)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
     cos, sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
     tables = L.RotaryEmbedding.from_tables(cos, sin) if rope else None
     gq, gk = 1 + 0.1 * w.randn(D), 1 + 0.1 * w.randn(D)
