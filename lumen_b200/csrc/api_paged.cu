@@ -163,7 +163,9 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
         }
         paged_cut(p, b->g, paged_few_shape(ctx->num_sms), few);
         b->n_few = (int)p.items.size();
-        paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, ctx->num_sms) : paged_f32_shape(ctx->num_sms), many);
+        int many_kv = 0;
+        for (int s : many) many_kv = std::max(many_kv, p.seqs[(size_t)s].kv_len);
+        paged_cut(p, b->g, b->g.dtype == LUMEN_BF16 ? paged_tc_shape(p.max_q * p.group, many_kv, ctx->num_sms) : paged_f32_shape(ctx->num_sms), many);
         for (size_t i = 0; i < p.items.size(); ++i) {
             int &rows = (int)i < b->n_few ? b->few_rows : b->many_rows;
             rows = std::max(rows, p.items[i].rows);
@@ -182,6 +184,7 @@ int lumen_page_batch_new(const lumen_page_pool *pool, size_t n_head, size_t n_se
             b->seen_kv = std::max(b->seen_kv, q.kv_len);
             b->max_rows = std::max(b->max_rows, rows);
             if (rows <= mass_shape.rows) few.push_back(s), b->mass_rows = std::max(b->mass_rows, rows);
+            else b->many_blocks += (long long)((q.kv_len + paged_mass_block(b->g) - 1) / paged_mass_block(b->g)) * b->g.h_kv;
         }
         paged_cut(mass, b->g, mass_shape, few);
         b->n_mass = (int)mass.items.size();
@@ -316,7 +319,7 @@ int lumen_paged_attention_mass(lumen_page_pool *pool, const lumen_page_batch *ba
     if (p.shared) return set_error(ctx, LUMEN_ERR_INVALID, "paged_attention_mass: two sequences share a page");
     if (p.tokens == 0 || p.max_kv == 0) return LUMEN_OK;
     OnDevice on(ctx);
-    const PagedMassArgs a = {q_dev, scale, lse_dev, batch->seen_kv, batch->max_rows, batch->mass, batch->n_mass, batch->mass_rows};
+    const PagedMassArgs a = {q_dev, scale, lse_dev, batch->seen_kv, batch->max_rows, batch->many_blocks, batch->mass, batch->n_mass, batch->mass_rows};
     return a.max_rows ? launch_paged_mass(ctx, pool->g, view_of(pool, batch), pool->k_map[1], a, ctx->stream) : (int)LUMEN_OK;
 }
 

@@ -29,6 +29,7 @@ struct lumen_page_batch {
     int seen_kv = 0, max_rows = 0;                                    // of the sequences with new tokens and positions: most positions, rows of a key head
     lumen::PagedItem *mass = nullptr;  // what the kernel that adds up the weights of few rows takes
     int n_mass = 0, mass_rows = 0;
+    long long many_blocks = 0;         // of the sequences with more rows
     float *part = nullptr;  // partial sums [part_rows, d], then their maxima and sums [part_rows, 2]
 };
 
@@ -74,6 +75,16 @@ int launch_paged(lumen_ctx *ctx, void (*kernel)(KA...), unsigned cluster, dim3 g
 #ifdef __CUDACC__
 // Lets the next kernel start.  Kernels that take tensor memory call it behind their own allocation (the next one may take some before it waits).
 __device__ __forceinline__ void paged_start_next() { pdl_launch(); }
+// The 32-bit number at the place of `mine` in the shared memory of a CTA of the cluster.
+__device__ __forceinline__ unsigned there(const void *mine, unsigned rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 #endif
 
 struct PagedAppendArgs {
@@ -103,7 +114,7 @@ PagedShape paged_few_shape(int num_sms);
 int launch_paged_few(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
 PagedShape paged_f32_shape(int num_sms);
 int launch_paged_attn_f32(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const PagedAttnArgs &a, cudaStream_t s);
-PagedShape paged_tc_shape(int max_rows, int num_sms);
+PagedShape paged_tc_shape(int max_rows, int max_kv, int num_sms);
 int paged_tc_maps(lumen_ctx *ctx, const PagedGeom &g, const void *mem, int most, CUtensorMap *map);
 int launch_paged_attn_tc(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap (&k_map)[2], const CUtensorMap (&v_map)[2], const PagedAttnArgs &a,
                          cudaStream_t s);
@@ -113,9 +124,11 @@ struct PagedMassArgs {
     float scale;
     const float *lse;
     int max_kv, max_rows;    // of the sequences with new tokens: positions, rows of a key head
+    long long many_blocks;   // blocks of positions of a key head, of those with more than few rows
     const PagedItem *few;    // the work of the sequences with few rows
     int n_few, few_rows;
 };
+int paged_mass_block(const PagedGeom &g);  // positions
 PagedShape paged_mass_shape(const PagedGeom &g, int num_sms);  // (its rows: up to which the items are taken)
 int launch_paged_mass(lumen_ctx *ctx, const PagedGeom &g, const PagedView &v, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s);
 int launch_paged_evict(lumen_ctx *ctx, const PagedGeom &g, const PagedView &from, const PagedView &to, int recent, int max_len, int max_keep, int *kept,

@@ -452,8 +452,11 @@ int launch(lumen_ctx *ctx, const PagedView &v, const CUtensorMap &k_map, const C
 
 }  // namespace
 
-PagedShape paged_tc_shape(int max_rows, int num_sms) {
-    if (max_rows > kMma) return {2 * kMma, TcGeom<128, 2>::kKeys, num_sms};
+// Two tiles of rows together, but not over short contexts: a few tiles of positions are over before a CTA that has its SM to itself has started and ended.  Prompts
+// of 16000 tokens together, one tile and two: 32 heads of 64 over 4, 500 positions each 146 and 174 us, 1000 191 and 217, 2000 292 and 301, 4000 508 and 469; 32 of
+// 128 over 8, 500 244 and 266, 1000 306 and 312, 2000 421 and 410.
+PagedShape paged_tc_shape(int max_rows, int max_kv, int num_sms) {
+    if (max_rows > kMma && max_kv > 1024) return {2 * kMma, TcGeom<128, 2>::kKeys, num_sms};
     return {kMma, TcGeom<128, 1>::kKeys, 2 * num_sms};
 }
 

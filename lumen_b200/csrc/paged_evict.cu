@@ -21,17 +21,6 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 
 constexpr int kHeld = 40 * 1024;  // weights that the shared memory of a CTA holds
 
-// The 32-bit number at the place of `mine` in the shared memory of a CTA of the cluster.
-__device__ __forceinline__ unsigned there(const unsigned *mine, unsigned rank) {
-    uint32_t at, v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // grid (CTAs of a cluster x key heads, sequences); HELD: the weights of every sequence fit (else they are read again in every pass).  Four
 // neighbouring positions a thread: bound by the instructions of its SMs.
 template <bool HELD>

@@ -195,15 +195,30 @@ struct MassGeom {
     static constexpr size_t kSmem = (2 + kTcStages) * (size_t)kOperand + 1024;
 };
 
+// The sums of a block's positions, [halves of the columns][positions] of every CTA of its cluster, go to the slots.
+template <int KEYS>
+__device__ __forceinline__ void add_parts(const PagedView &p, const PagedSeq &sq, int kvh, int key0, const float (&part)[2][KEYS], int rank, int ctas, bool failed) {
+    if (ctas > 1) cluster_meet();
+    const int tid = threadIdx.x;
+    if (rank == 0 && tid < KEYS && key0 + tid < sq.kv_len && !failed) {
+        float sum = part[0][tid] + part[1][tid];
+        for (int r = 1; r < ctas; ++r) sum += __uint_as_float(there(&part[0][tid], (unsigned)r)) + __uint_as_float(there(&part[1][tid], (unsigned)r));
+        p.mass[paged_row(p, p.tables + sq.table, kvh, key0 + tid)] += sum;
+    }
+    __syncwarp();
+    if (ctas > 1) cluster_meet();  // (the sums may still be read)
+}
+
 // A CTA owns 256 positions of a key head (their keys stay in shared memory) and walks the rows that see any of them, up to 128 at a time (as many
 // whole tokens as fit): scores transposed, S^T = K.Q^T, so that a thread holds one position and sums over half of the columns.  Warps 0-15:
 // exponentials and sums (two warpgroups per 128 positions, two score buffers each); warps 16 and 17: products, of 128 positions each;
 // warps 18 and 19: queries (a TMA box of tokens x the heads of the group x 64 numbers) and log-sums into a ring.
-// grid (blocks of 256 positions of the longest sequence, key heads, sequences)
+// Where there are fewer blocks than SMs, the rows of a block are shared by a cluster of `ctas` CTAs, which take its steps in turn; the first adds their sums up, in order.
+// grid (blocks of 256 positions of the longest sequence x ctas, key heads, sequences)
 template <int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
 paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q, const PagedView p, float scale, const float *__restrict__ lse,
-                     DeviceStatus *status) {
+                     int ctas, DeviceStatus *status) {
     using G = MassGeom<D>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *k_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *ring = k_s + 2 * G::kOperand;
@@ -215,10 +230,12 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     volatile int *failed = &failed_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
-    const int rows = sq.q_len * p.group, key0 = blockIdx.x * kTcKeys, past = sq.kv_len - sq.q_len;
+    const int rows = sq.q_len * p.group, rank = (int)blockIdx.x % ctas, key0 = (int)blockIdx.x / ctas * kTcKeys, past = sq.kv_len - sq.q_len;
     if (key0 >= sq.kv_len || rows <= kFewRows) return pdl_wait();
     const int per = kTcRows / p.group, n_rows = per * p.group;  // tokens and rows of a step
-    const int start_tok = p.causal ? max(0, key0 - past) : 0, start = start_tok * p.group, steps = (sq.q_len - start_tok + per - 1) / per;  // (start < rows: key0 < kv_len)
+    const int first_tok = p.causal ? max(0, key0 - past) : 0, all_steps = (sq.q_len - first_tok + per - 1) / per;  // (first_tok < q_len: key0 < kv_len)
+    const int steps = (all_steps - rank + ctas - 1) / ctas;  // of this CTA: rank, rank + ctas, ...
+    auto tok_of = [&](int i) { return first_tok + (rank + i * ctas) * per; };
     const int tiles = min(2, (sq.kv_len - key0 + 127) / 128);  // of 128 positions
     if (tid == 0) {
         bar_init(&k_bar, 1);
@@ -270,7 +287,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         auto ask = [&](int i) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int r = id + h * kTcLoaders, row = start + i * n_rows + r;
+                const int r = id + h * kTcLoaders, row = tok_of(i) * p.group + r;
                 l_next[h] = i < steps && r < n_rows && row < rows ? -kLog2e * lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : -INFINITY;
             }
         };
@@ -282,7 +299,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             if (id == 0 && ok) {
                 bar_expect(&q_full[s], (uint32_t)n_rows * kBK * 2 * G::kBlocks);
 #pragma unroll
-                for (int c = 0; c < G::kBlocks; ++c) tma_load_3d(ring + (size_t)s * G::kOperand + c * G::kTile, &map_q, c * kBK, kvh * p.group, sq.tok0 + start_tok + i * per, &q_full[s]);
+                for (int c = 0; c < G::kBlocks; ++c) tma_load_3d(ring + (size_t)s * G::kOperand + c * G::kTile, &map_q, c * kBK, kvh * p.group, sq.tok0 + tok_of(i), &q_full[s]);
                 ++q_issued;
             }
 #pragma unroll
@@ -325,7 +342,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const int key_max = key0 + 128 * kt + (warp & 3) * 32 + 31;
 #pragma unroll 1
             for (int i = 0; i < steps; ++i) {
-                const int s = i % kTcStages, b = i & 1, r0 = start + i * n_rows;
+                const int s = i % kTcStages, b = i & 1, r0 = tok_of(i) * p.group;
                 wait_first(&q_full[s], (uint32_t)((i / kTcStages) & 1), failed, status, 764);  // the log-sums
                 wait_first(&s_full[kt][b], (uint32_t)((i / 2) & 1), failed, status, 765);
                 __syncwarp();
@@ -375,7 +392,7 @@ paged_mass_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         }
     }
     __syncthreads();
-    if (tid < kTcKeys && key0 + tid < sq.kv_len && !*failed) p.mass[paged_row(p, p.tables + sq.table, kvh, key0 + tid)] += part_s[0][tid] + part_s[1][tid];
+    add_parts<kTcKeys>(p, sq, kvh, key0, part_s, rank, ctas, *failed);
     if (*failed) {
         if (tid == kTcExps + 64) {  // a wait gave up
             drain_ring(&k_bar, 1, 1);
@@ -421,9 +438,9 @@ __device__ __forceinline__ void put_split(const float4 &x, const float4 &y, unsi
 
 // A CTA owns 128 positions of a key head and walks the rows that see any of them, 128 at a time, as paged_mass_tc_kernel does.  Warpgroups 0 and 1:
 // exponentials and sums (half of the columns each); 2: queries, a step ahead in registers, split into shared memory; 3: products.
-// grid (blocks of 128 positions of the longest sequence, key heads, sequences)
+// grid (blocks of 128 positions of the longest sequence x ctas, key heads, sequences)
 template <int D>
-__global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const PagedView p, const float *__restrict__ q, float scale, const float *__restrict__ lse, DeviceStatus *status) {
+__global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const PagedView p, const float *__restrict__ q, float scale, const float *__restrict__ lse, int ctas, DeviceStatus *status) {
     using G = SplitMass<D>;
     constexpr int kStages = G::kStages;
     extern __shared__ unsigned char smem_raw[];
@@ -436,9 +453,11 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
     volatile int *failed = &failed_s;
     const int tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.y;
     const PagedSeq sq = p.seqs[blockIdx.z];
-    const int rows = sq.q_len * p.group, key0 = blockIdx.x * kSplitKeys, past = sq.kv_len - sq.q_len;
+    const int rows = sq.q_len * p.group, rank = (int)blockIdx.x % ctas, key0 = (int)blockIdx.x / ctas * kSplitKeys, past = sq.kv_len - sq.q_len;
     if (key0 >= sq.kv_len || rows <= kFewRowsSplit) return pdl_wait();
-    const int start = p.causal ? max(0, key0 - past) * p.group : 0, steps = (rows - start + 127) / 128;  // (start < rows: key0 < kv_len)
+    const int start = p.causal ? max(0, key0 - past) * p.group : 0, all_steps = (rows - start + 127) / 128;  // (start < rows: key0 < kv_len)
+    const int steps = (all_steps - rank + ctas - 1) / ctas;  // of this CTA: rank, rank + ctas, ...
+    auto row_of = [&](int i) { return start + (rank + i * ctas) * 128; };
     const int *table = p.tables + sq.table;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -511,7 +530,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
         auto fetch = [&](int i) {
 #pragma unroll
             for (int n = 0; n < G::kPieces; ++n) {
-                const int row = start + i * 128 + r0 + n * kStep, tok = row / p.group;
+                const int row = row_of(i) + r0 + n * kStep, tok = row / p.group;
                 x[n][0] = x[n][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (row < rows) {
                     const float4 *src = reinterpret_cast<const float4 *>(q + ((size_t)(sq.tok0 + tok) * p.n_head + kvh * p.group + row - tok * p.group) * D + 8 * c);
@@ -519,10 +538,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
                     x[n][1] = __ldg(src + 1);
                 }
             }
-            const int row = start + i * 128 + id;
+            const int row = row_of(i) + id;
             l = row < rows ? -kLog2e * lse[(size_t)(sq.tok0 + row / p.group) * p.n_head + kvh * p.group + row % p.group] : -INFINITY;  // (no weight in columns without a row)
         };
-        fetch(0);
+        if (steps > 0) fetch(0);
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int s = i % kStages;
@@ -545,7 +564,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
         const int first = p.causal ? max(0, key - past) * p.group : 0, key_max = key0 + (warp & 3) * 32 + 31;
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
-            const int b = i & 1, r0 = start + i * 128;
+            const int b = i & 1, r0 = row_of(i);
             wait_first(&l_full[b], (uint32_t)((i / 2) & 1), failed, status, 920);
             wait_first(&s_full[b], (uint32_t)((i / 2) & 1), failed, status, 921);
             __syncwarp();
@@ -579,7 +598,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) paged_mass_f32_kernel(const 
         part_s[half][tid & 127] = s0 + s1;
     }
     __syncthreads();
-    if (tid < kSplitKeys && key0 + tid < sq.kv_len && !*failed) p.mass[paged_row(p, table, kvh, key0 + tid)] += part_s[0][tid] + part_s[1][tid];
+    add_parts<kSplitKeys>(p, sq, kvh, key0, part_s, rank, ctas, *failed);
     if (*failed && tid == 384) drain_mmas(&quiet);  // a wait gave up
     tc_before();
     __syncthreads();
@@ -597,9 +616,17 @@ template <int D>
 int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUtensorMap &k_map, const PagedMassArgs &a, cudaStream_t s) {
     if (a.n_few) LUMEN_TRY(g.dtype == LUMEN_F32 ? (launch_few<float, D>(ctx, all, a, s)) : (launch_few<__nv_bfloat16, D>(ctx, all, a, s)));
     if (a.max_rows <= (g.dtype == LUMEN_F32 ? kFewRowsSplit : kFewRows)) return LUMEN_OK;
+    // CTAs to a block: what ends soonest, where starting and ending cost a CTA as much as three steps.  By events, one CTA and as chosen: a prompt of 2048 tokens, 32
+    // heads of 128 over 8, 16 bits 112 us and 64 (four), 32 bits 267 and 204 (two); two of 150 tokens, 28 over 4, 32 bits 50 and 31 (eight).
+    const int keys = paged_mass_block(g);
+    int ctas = 1;
+    double best = 1e30;
+    for (int c = 1; c <= 8; c *= 2) {
+        const double rounds = std::max(1., (double)a.many_blocks * c / ctx->num_sms), each = (a.max_rows + kTcRows * c - 1) / (kTcRows * c) + 3;
+        if (rounds * each < best) best = rounds * each, ctas = c;
+    }
     for (int s0 = 0; s0 < all.n_seq; s0 += 32768) {  // (the grid's third extent)
-        const int keys = g.dtype == LUMEN_F32 ? kSplitKeys : kTcKeys;
-        const dim3 grid((unsigned)((a.max_kv + keys - 1) / keys), (unsigned)all.h_kv, (unsigned)std::min(all.n_seq - s0, 32768));
+        const dim3 grid((unsigned)((a.max_kv + keys - 1) / keys * ctas), (unsigned)all.h_kv, (unsigned)std::min(all.n_seq - s0, 32768));
         PagedView v = all;
         v.seqs += s0;
         if (g.dtype == LUMEN_F32) {
@@ -609,19 +636,21 @@ int launch(lumen_ctx *ctx, const PagedGeom &g, const PagedView &all, const CUten
             }();
             if (regs * kSplitThreads < (2 * 128 + kRegsLoad + kRegsIssue) * 128) return set_error(ctx, LUMEN_ERR_UNSUPPORTED, "paged_attention_mass: kernel built with %d registers", regs);
             LUMEN_TRY(allow_smem(ctx, paged_mass_f32_kernel<D>, SplitMass<D>::kSmem));
-            LUMEN_TRY(launch_paged(ctx, paged_mass_f32_kernel<D>, grid, kSplitThreads, SplitMass<D>::kSmem, s, v, static_cast<const float *>(a.q), a.scale, a.lse, ctx->d_status));
+            LUMEN_TRY(launch_paged(ctx, paged_mass_f32_kernel<D>, (unsigned)ctas, grid, kSplitThreads, SplitMass<D>::kSmem, s, v, static_cast<const float *>(a.q), a.scale, a.lse, ctas, ctx->d_status));
         } else {
             CUtensorMap q_map;
             const size_t row = (size_t)all.n_head * D;
             LUMEN_TRY(make_map_3d(ctx, &q_map, a.q, D, (size_t)all.n_head, D, (size_t)all.tokens, row, all.group, kTcRows / all.group));
             LUMEN_TRY(allow_smem(ctx, paged_mass_tc_kernel<D>, MassGeom<D>::kSmem));
-            LUMEN_TRY(launch_paged(ctx, paged_mass_tc_kernel<D>, grid, kTcThreads, MassGeom<D>::kSmem, s, k_map, q_map, v, a.scale, a.lse, ctx->d_status));
+            LUMEN_TRY(launch_paged(ctx, paged_mass_tc_kernel<D>, (unsigned)ctas, grid, kTcThreads, MassGeom<D>::kSmem, s, k_map, q_map, v, a.scale, a.lse, ctas, ctx->d_status));
         }
     }
     return LUMEN_OK;
 }
 
 }  // namespace
+
+int paged_mass_block(const PagedGeom &g) { return g.dtype == LUMEN_F32 ? kSplitKeys : kTcKeys; }
 
 PagedShape paged_mass_shape(const PagedGeom &g, int num_sms) { return {g.dtype == LUMEN_F32 ? kFewRowsSplit : kFewRows, kFewKeys, num_sms * kFewPerSm}; }
 
