@@ -5,7 +5,7 @@
 //   few rows: paged_mass_few_kernel, bound by reading the keys once (16 sequences of 2000 to 8000 positions, 8 key heads of 128, a token each:
 //   37 us by events, 165 MB at 4.5 TB/s)
 //   more: scores on the 5th-generation tensor cores: paged_mass_tc_kernel (16 bits; two chunks of 200 to 512 tokens over up to 6500 positions, 32 over 8 heads of
-//   128: 97 us, exponential unit 41 % and tensor pipe 29 % busy), and paged_mass_f32_kernel, bound by the six products of three bf16 terms (390 us there; 1550 as
+//   128: 95 us, exponential unit 41 % and tensor pipe 29 % busy), and paged_mass_f32_kernel, bound by the six products of three bf16 terms (390 us there; 1550 as
 //   m16n8k16 products)
 #include <type_traits>
 
